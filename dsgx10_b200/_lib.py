@@ -55,6 +55,11 @@ class LayerStep(C.Structure):
                 ("norm_w", C.c_void_p), ("xn_out", C.c_void_p), ("norm_eps", C.c_float), ("norm_mode", C.c_int32)]
 
 
+class LinearW(C.Structure):
+    _fields_ = [("w", C.c_void_p), ("w_up", C.c_void_p), ("N", C.c_int32), ("K", C.c_int32), ("fmt", C.c_uint32),
+                ("reserved", C.c_int32)]
+
+
 class AddNorm(C.Structure):
     _fields_ = [("res", C.c_void_p), ("res_out", C.c_void_p), ("norm_w", C.c_void_p), ("normed", C.c_void_p),
                 ("eps", C.c_float), ("norm_mode", C.c_int32), ("add_f32", C.c_int32), ("reserved", C.c_int32)]
@@ -79,6 +84,7 @@ SYMBOLS = {
     "dsgx_finalize": (_I, [_V, _V, _I, _I, _V, _I, _V]),
     "dsgx_moe_layer_decode": (_I, [C.POINTER(MoeShape), C.POINTER(LayerW), _V, _I, C.POINTER(LayerStep), _I, _V]),
     "dsgx_moe_layer_decode_host": (_I, [C.POINTER(MoeShape), C.POINTER(LayerW), _V, _I, C.POINTER(LayerStep), _V, _V]),
+    "dsgx_linear_decode": (_I, [C.POINTER(LinearW), _V, C.c_int64, _I, _V, C.c_int64, _V, C.c_int64, _I, _V, _V]),
     "dsgx_prefill_weights_bytes": (_Z, [C.POINTER(MoeShape)]),
     "dsgx_prefill_prepare": (_I, [C.POINTER(MoeShape), C.POINTER(LayerW), _V, _V]),
     "dsgx_prefill_ws_bytes": (_Z, [C.POINTER(MoeShape), _I]),

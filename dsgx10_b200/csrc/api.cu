@@ -407,6 +407,36 @@ int dsgx_moe_layer_decode_host(const dsgx_moe_shape* s, const dsgx_layer_w* L, c
   return e == cudaSuccess ? DSGX_OK : cuda_fail(e);
 }
 
+int dsgx_linear_decode(const dsgx_linear_w* W, const void* x, int64_t ldx, int M, const void* res, int64_t ldr, void* out,
+                       int64_t ldo, int out_f32, int32_t* status_word, void* stream) {
+  if (!W || !W->w || !x || !out) return DSGX_ERR_ARG;
+  if (W->fmt != DSGX_FMT_INT4) return DSGX_ERR_FORMAT;
+  if (W->N < 1 || W->K < 1 || W->N > (1 << 30) || W->K > (1 << 30)) return DSGX_ERR_SHAPE;
+  if (M < 1 || M > DSGX_MAX_STEP_ROWS || ldx < W->K || ldo < W->N || (res && ldr < W->N)) return DSGX_ERR_ARG;
+  if (res && W->w_up) return DSGX_ERR_UNSUPPORTED;
+  if (((uintptr_t)W->w | (uintptr_t)W->w_up) & 15 || ((uintptr_t)x | (uintptr_t)res) & 1 || (uintptr_t)out & (out_f32 ? 3 : 1) ||
+      (uintptr_t)status_word & 3)
+    return DSGX_ERR_ARG;
+  LinearParams p;
+  p.w = W->w, p.w_up = W->w_up, p.x = reinterpret_cast<const __nv_bfloat16*>(x), p.res = reinterpret_cast<const __nv_bfloat16*>(res);
+  p.out = out, p.ldx = ldx, p.ldr = ldr, p.ldo = ldo, p.M = M, p.N = W->N, p.K = W->K;
+  p.n8 = (W->N + 7) / 8, p.nb = (W->K + 511) / 512, p.units = W->w_up ? p.n8 : (p.n8 + 1) / 2;
+  p.out_f32 = out_f32 != 0, p.x_vec = ((uintptr_t)x & 15) == 0 && ldx % 8 == 0;
+  p.cluster = 1, p.xblocks = 0, p.status = status_word;
+  bool fits = false;
+  cudaError_t e = launch_linear_int4(p, (cudaStream_t)stream, &fits);
+  if (e != cudaSuccess) return cuda_fail(e);
+  if (fits) return DSGX_OK;
+  if (M == 1) return DSGX_ERR_SHAPE;  // (K beyond what eight CTAs' shared memory holds of one row)
+  // too many rows of too long a K for one launch: the rows in two halves, the same bits a row
+  const int h = M > 8 ? 8 : (M + 1) / 2;
+  const int rc = dsgx_linear_decode(W, x, ldx, h, res, ldr, out, ldo, out_f32, status_word, stream);
+  if (rc) return rc;
+  return dsgx_linear_decode(W, reinterpret_cast<const uint8_t*>(x) + h * ldx * 2, ldx, M - h,
+                            res ? reinterpret_cast<const uint8_t*>(res) + h * ldr * 2 : nullptr, ldr,
+                            reinterpret_cast<uint8_t*>(out) + h * ldo * (out_f32 ? 4 : 2), ldo, out_f32, status_word, stream);
+}
+
 static int check_prefill_shape(const dsgx_moe_shape* s) {
   const int rc = check_shape(s);
   if (rc) return rc;

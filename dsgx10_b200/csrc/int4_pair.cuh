@@ -1,0 +1,128 @@
+// The inner product of the 4-bit operators (linear.cu, block_int4.cu): a pair of 8-row INT4-g32 blocks (512 k each) against the
+// rows of a bf16 activation tile, and the same for bf16 blocks.
+//
+// W[n][k] = (u - z) s with one bf16 scale s and one nibble z a group of 32 along K.  u - z is a whole number of at most 15,
+// so it is exact in bf16; the scale is applied to the group's f32 sum, so W itself is never rounded.
+//
+// How a group's sum is had from m16n8k16 MMAs although the blocks' lanes mix two groups in every MMA (lane 4 g + t holds
+// k = 64 q + 16 t + 0..15 of row g, so lanes t = 0, 1 hold one group of 32 and t = 2, 3 the next): the eight columns of B are
+// (token, half) pairs.  Column 2 r + h holds token r's activations in the lanes of half h and zeros in the others, so column
+// 2 r + h of D is the sum over group h alone, and lane (g, t) ends with both sums of token t: two fused multiply-adds with
+// the row's two scales finish 64 k.  Four tokens an MMA instead of eight, but the weights' conversion (the part that bounds
+// these kernels: 28 logic and 16 subtract instructions for 32 weights a lane) loses its multiply by the scale, and a
+// token's bits depend neither on the other tokens nor on their number.
+#pragma once
+#include "common.cuh"
+#include "decode_common.cuh"
+
+namespace dsgx {
+
+constexpr int kQBlk = 2368;                          // an INT4 block: 8 rows x 512 k
+constexpr int kHBlk = 2048;                          // a bf16 block: 8 rows x 128 k
+constexpr int kPairBytes = 2 * kQBlk;
+constexpr int kPairStage = (kPairBytes + 127) & ~127;  // (two bf16 blocks, 4096 B, fit)
+
+// nibbles i and i + 4 of a word minus the zero point, as bf16x2 (zz = 128 + z in both halves): 0x4300 | u is 128 + u
+DSGX_DEV uint32_t nib_pair(uint32_t w, int i, uint32_t zz) {
+  const uint32_t v = ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&zz));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+DSGX_DEV void mma_bf16_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// Where a lane finds its column's activations.  The tile: [K / 16 groups][rows][16 bf16 in tile_pos order]; set s holds the
+// tokens 4 s .. 4 s + 3.  Lanes of the other half, and columns without a token, read 32 bytes of zeros (step 0).
+template <int S>
+struct XCols {
+  const uint8_t* p[S];
+  uint32_t step[S];  // bytes from one 64-k span to the next
+};
+// tok(s, j): the tile row of the j-th token of set s, negative: none
+template <int S, class F>
+DSGX_DEV void xcols_int4(XCols<S>& x, const uint8_t* tile, int rows, const uint8_t* zero, int lane, F tok) {
+  const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    const int r = tok(s, g >> 1);
+    const bool on = r >= 0 && (t >> 1) == (g & 1);
+    x.p[s] = on ? tile + ((size_t)t * rows + r) * 32 : zero;
+    x.step[s] = on ? 4u * rows * 32 : 0u;
+  }
+}
+
+// acc[s][0 / 1] += row g of strip a / b times token 4 s + t, over the 512 k of one block pair; x at the block's first k
+template <int S>
+DSGX_DEV void int4_pair(float (&acc)[S][2], const uint8_t* a, const uint8_t* b, XCols<S> x, int lane) {
+  const int g = lane >> 2, h = (lane >> 1) & 1;
+  const uint32_t za = *reinterpret_cast<const uint32_t*>(a + 2304 + 8 * g + 4 * h);
+  const uint32_t zb = *reinterpret_cast<const uint32_t*>(b + 2304 + 8 * g + 4 * h);
+  const uint4 sa0 = lds128(a + 2048 + 32 * g), sa1 = lds128(a + 2048 + 32 * g + 16);  // the two halves' eight scales
+  const uint4 sb0 = lds128(b + 2048 + 32 * g), sb1 = lds128(b + 2048 + 32 * g + 16);
+  const uint32_t zae = za & 0x0F0F0F0Fu, zao = (za >> 4) & 0x0F0F0F0Fu;
+  const uint32_t zbe = zb & 0x0F0F0F0Fu, zbo = (zb >> 4) & 0x0F0F0F0Fu;
+  const uint32_t* a0 = &sa0.x;
+  const uint32_t* a1 = &sa1.x;
+  const uint32_t* b0 = &sb0.x;
+  const uint32_t* b1 = &sb1.x;
+#pragma unroll
+  for (int jj = 0; jj < 4; ++jj) {
+    const uint4 va = lds128(a + 512 * jj + 16 * lane), vb = lds128(b + 512 * jj + 16 * lane);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const uint32_t zsel = 0x4040u + 0x0101u * jj;  // bytes (nibble jj, 0x43, nibble jj, 0x43): 128 + z twice
+      const uint32_t zza = __byte_perm(q ? zao : zae, 0x43434343u, zsel), zzb = __byte_perm(q ? zbo : zbe, 0x43434343u, zsel);
+      const uint32_t al = q ? va.z : va.x, ah = q ? va.w : va.y, bl = q ? vb.z : vb.x, bh = q ? vb.w : vb.y;
+      uint32_t wa[8], wb[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        wa[i] = nib_pair(al, i, zza), wa[4 + i] = nib_pair(ah, i, zza);
+        wb[i] = nib_pair(bl, i, zzb), wb[4 + i] = nib_pair(bh, i, zzb);
+      }
+      const float fa0 = __uint_as_float(q ? a0[jj] & 0xffff0000u : a0[jj] << 16), fa1 = __uint_as_float(q ? a1[jj] & 0xffff0000u : a1[jj] << 16);
+      const float fb0 = __uint_as_float(q ? b0[jj] & 0xffff0000u : b0[jj] << 16), fb1 = __uint_as_float(q ? b1[jj] & 0xffff0000u : b1[jj] << 16);
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        const uint4 x0 = lds128(x.p[s]), x1 = lds128(x.p[s] + 16);
+        x.p[s] += x.step[s];
+        float d[4];
+        mma_bf16_zero(d, wa[0], wb[0], wa[1], wb[1], x0.x, x0.y);
+        mma_bf16(d, wa[2], wb[2], wa[3], wb[3], x0.z, x0.w);
+        mma_bf16(d, wa[4], wb[4], wa[5], wb[5], x1.x, x1.y);
+        mma_bf16(d, wa[6], wb[6], wa[7], wb[7], x1.z, x1.w);
+        acc[s][0] = fmaf(fa1, d[1], fmaf(fa0, d[0], acc[s][0]));
+        acc[s][1] = fmaf(fb1, d[3], fmaf(fb0, d[2], acc[s][1]));
+      }
+    }
+  }
+}
+
+// 16 values of row r of x from column k0 on, in tile_pos order, zeros from column K on: the tile's 32 bytes of a (group, row)
+DSGX_DEV void tile_group(uint4 (&o)[2], const __nv_bfloat16* row, int k0, int K, bool vec) {
+  uint32_t w[8];
+  if (vec && k0 + 16 <= K) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(row + k0)), b = __ldg(reinterpret_cast<const uint4*>(row + k0 + 8));
+    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+  } else {
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int k = k0 + 2 * i;
+      const uint32_t lo = k < K ? p[k] : 0u, hi = k + 1 < K ? p[k + 1] : 0u;
+      w[i] = lo | hi << 16;
+    }
+  }
+  // words (v0 v1)(v2 v3)(v4 v5)(v6 v7) -> (v0 v4)(v1 v5)(v2 v6)(v3 v7), both halves of the group
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    uint32_t* d = &o[j].x;
+    d[0] = __byte_perm(w[4 * j], w[4 * j + 2], 0x5410), d[1] = __byte_perm(w[4 * j], w[4 * j + 2], 0x7632);
+    d[2] = __byte_perm(w[4 * j + 1], w[4 * j + 3], 0x5410), d[3] = __byte_perm(w[4 * j + 1], w[4 * j + 3], 0x7632);
+  }
+}
+
+}  // namespace dsgx

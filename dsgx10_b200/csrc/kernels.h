@@ -147,6 +147,21 @@ cudaError_t launch_front_route(const DecodeParams& p, uint32_t fmt, const RouteP
                                const float* wr, const float* bias, float* logits, int* idx, float* w, cudaStream_t st,
                                bool pdl);
 
+// ---- dense INT4-g32 products (linear.cu) ---------------------------------------------------------------------------------
+struct LinearParams {
+  const uint8_t* w;     // INT4 blocks [n8][nb]
+  const uint8_t* w_up;  // the second matrix (SwiGLU), or null
+  const __nv_bfloat16* x;
+  const __nv_bfloat16* res;
+  void* out;
+  long long ldx, ldr, ldo;
+  int M, N, K, n8, nb, units;  // units of 16 output rows (SwiGLU: 8 + 8)
+  int out_f32, x_vec;
+  int cluster, xblocks;        // chosen by the launch: CTAs a cluster, blocks of K a rank holds at most
+  int* status;
+};
+cudaError_t launch_linear_int4(const LinearParams& p, cudaStream_t st, bool* fits);
+
 // ---- prefill (FP8) ----------------------------------------------------------------------------------------------------
 struct PrefillWeights {  // K-major row-major copies of the layer's matrices, [E + 1 experts] each (index E: shared)
   uint8_t *g, *u, *d;

@@ -1,0 +1,63 @@
+"""Dense products with 4-bit weights for 1..16 rows over the C ABI (dsgx_linear_decode), torch tensors as device memory.
+
+The engines' weight-streaming GEMV over INT4 matrices (altar1 engine/attn/attn.h glm::gemv): projections, dense FFN layers and
+heads, next to the experts of moe.py.
+
+    w = linear.LinearW(N, K, torch.from_numpy(weights.pack_linear_int4(codes, scales, zeros)).cuda())
+    y = linear.linear_decode(w, x)                        # bf16 [M][N] = x W^T
+    y = linear.linear_decode(w, x, res=r)                 # + r, one rounding
+    h = linear.linear_decode(linear.LinearW(N, K, gate, up=up), x)   # silu(x Wg^T) * (x Wu^T)
+"""
+import ctypes as C
+
+import torch
+
+from . import _lib
+from ._lib import check, lib
+
+
+class LinearW:
+    """An INT4-g32 matrix [N][K] in blocks of 8 rows x 512 k on the device (weights.pack_linear_int4), or a gate / up pair."""
+
+    def __init__(self, N, K, blocks, up=None):
+        if N < 1 or K < 1:
+            raise ValueError(f"LinearW: N = {N}, K = {K}")
+        need = -(-N // 8) * -(-K // 512) * 2368
+        for b in (blocks,) if up is None else (blocks, up):
+            if b.dtype != torch.uint8 or not b.is_contiguous() or b.numel() != need or not b.is_cuda:
+                raise ValueError(f"LinearW: {need} contiguous bytes on the device are wanted for [{N}][{K}], got {b.numel()} of {b.dtype} on {b.device}")
+        if up is not None and up.device != blocks.device:
+            raise ValueError("LinearW: the two matrices are on different devices")
+        self.N, self.K, self.blocks, self.up = N, K, blocks, up
+        self.c = _lib.LinearW(blocks.data_ptr(), None if up is None else up.data_ptr(), N, K, _lib.FMT_INT4, 0)
+
+
+def _rows(t, M, width, what, dtypes, device):
+    if t.dim() != 2 or t.shape[0] != M or t.shape[1] != width or t.dtype not in dtypes or t.device != device:
+        raise ValueError(f"linear_decode: {what} {tuple(t.shape)} of {t.dtype} on {t.device}; wanted ({M}, {width}) of {dtypes} on {device}")
+    if width > 1 and t.stride(1) != 1 or M > 1 and t.stride(0) < width:
+        raise ValueError(f"linear_decode: {what} has strides {t.stride()}: the last dimension must be contiguous")
+    return t.stride(0) if M > 1 else max(t.stride(0), width)
+
+
+def linear_decode(w, x, res=None, out=None, out_dtype=torch.bfloat16, status=None):
+    """x bf16 [M][K], M = 1..16 -> out [M][N] (bf16 or f32): x W^T (+ res bf16 [M][N]), or silu(x W^T) * (x Wup^T) where w has
+    an `up` matrix.  x, res and out may be rows of larger tensors (last dimension contiguous); out may be res.
+    status: an int32 device tensor that gets DSGX_ERR_DEVICE_WAIT where a bounded wait ran out."""
+    if x.dim() != 2:
+        raise ValueError(f"linear_decode: x has shape {tuple(x.shape)}")
+    M, dev = x.shape[0], w.blocks.device
+    if not 1 <= M <= _lib.MAX_STEP_ROWS:
+        raise ValueError(f"linear_decode: {M} rows; 1..{_lib.MAX_STEP_ROWS} are taken")
+    ldx = _rows(x, M, w.K, "x", (torch.bfloat16,), dev)
+    if out is None:
+        out = torch.empty(M, w.N, dtype=out_dtype, device=dev)
+    ldo = _rows(out, M, w.N, "out", (torch.bfloat16, torch.float32), dev)
+    ldr = 0 if res is None else _rows(res, M, w.N, "res", (torch.bfloat16,), dev)
+    if status is not None and (status.dtype != torch.int32 or status.device != dev or status.numel() < 1):
+        raise ValueError("linear_decode: status is an int32 tensor on the weights' device")
+    with torch.cuda.device(dev):
+        check(lib().dsgx_linear_decode(C.byref(w.c), x.data_ptr(), ldx, M, None if res is None else res.data_ptr(), ldr, out.data_ptr(),
+                                       ldo, int(out.dtype == torch.float32), None if status is None else status.data_ptr(),
+                                       torch.cuda.current_stream(dev).cuda_stream), "dsgx_linear_decode")
+    return out

@@ -129,6 +129,22 @@ def pack_int4(wp, s, zp=None):
     return out.reshape(-1)
 
 
+def pack_linear_int4(wp, s, zp=None, K=None):
+    """An INT4-g32 matrix of any size for the dense products (dsgx_linear_decode): wp uint8 [N][ceil(K/2)] and s bf16 bits
+    [N][ceil(K/32)] as pack_int4 takes them, zp uint32 [ceil(N/8)][ceil(K/32)] or None; K: the row length where wp has an odd
+    one.  Rows are filled up to a multiple of 8 and K to a multiple of 512 with weights of scale 0."""
+    wp, s = np.ascontiguousarray(wp, np.uint8), np.ascontiguousarray(s, np.uint16)
+    N, K = wp.shape[0], wp.shape[1] * 2 if K is None else K
+    if wp.shape[1] != (K + 1) // 2 or s.shape != (N, (K + 31) // 32):
+        raise ValueError(f"pack_linear_int4: codes {wp.shape} and scales {s.shape} do not fit N = {N}, K = {K}")
+    if zp is not None and np.shape(zp) != ((N + 7) // 8, (K + 31) // 32):
+        raise ValueError(f"pack_linear_int4: zero points {np.shape(zp)} do not fit N = {N}, K = {K}")
+    Np, Kp = _al(N, 8), _al(K, 512)
+    fill = lambda a, rows, cols: np.pad(a, ((0, rows - a.shape[0]), (0, cols - a.shape[1])))
+    return pack_int4(fill(wp, Np, Kp // 2), fill(s, Np, Kp // 32),
+                     None if zp is None else fill(np.ascontiguousarray(zp, np.uint32), Np // 8, Kp // 32))
+
+
 def pack_bf16(w):
     """bf16 bits uint16 [N][K] -> blocks of 8 rows x 128 k, 2048 B, [N/8][K/128]: the lane's 16 B at 512 p + 16 (4 g + t)
     are k = 64 (p >> 1) + 16 t + 8 (p & 1) + 0..7 (layout.h:96-107; int4_pack.py:165-170)."""

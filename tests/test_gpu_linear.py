@@ -1,0 +1,183 @@
+"""The dense INT4 products (dsgx_linear_decode) against the formula in 64 bits.
+
+Tolerance, by arithmetic.  A product x (u - z) has at most 8 + 4 significant bits: exact in f32.  A group's sum is four MMAs of 16
+products, each adding with at most one truncation (2^-23 of the running magnitude) a product and one for its accumulator: 68;
+two fused multiply-adds 64 k (16 in a block of 512) and the sums of the blocks and runs (at most nb / 8 + 1 + 3) round by
+2^-24 each.  So |y - exact| <= GAMMA A with A = sum |x| |W| and GAMMA = (68 + 8 + nb / 16 + 2) 2^-23 < (80 + nb) 2^-23; the one
+rounding of the output adds 2^-8 |y| (bf16) or 2^-24 |y| (f32)."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+def _make(N, K, seed, zeros=True):
+    from dsgx10_b200 import weights
+    from tests.linear_util import random_int4
+    wp, s, zp, w = random_int4(N, K, seed, zeros)
+    return torch.from_numpy(weights.pack_linear_int4(wp, s, zp, K=K)).cuda(), torch.from_numpy(w)
+
+
+def _x(M, K, seed):
+    return torch.randn(M, K, generator=torch.Generator().manual_seed(seed)).to(torch.bfloat16)
+
+
+def _gamma(K):
+    return (80 + -(-K // 512)) * 2.0 ** -23
+
+
+def _check(got, y, A, K, extra=0.0):
+    half = 2.0 ** -8 if got.dtype == torch.bfloat16 else 2.0 ** -24
+    err = (got.double().cpu() - y).abs()
+    tol = (half * y.abs() + _gamma(K) * A + extra) * (1 + 2.0 ** -7) + 1e-38
+    assert bool((err <= tol).all()), float((err / tol).max())
+
+
+SHAPES = [(1, 1, 1), (1, 8, 512), (2, 9, 513), (3, 17, 31), (4, 16, 32), (1, 33, 64), (5, 100, 1000), (8, 257, 2049), (9, 300, 1537),
+          (16, 1000, 4100), (16, 40, 12800), (8, 24, 20000), (1, 5000, 700), (4, 4744, 1024), (7, 2400, 3600), (12, 6000, 600), (2, 20001, 96)]
+
+
+@pytest.mark.parametrize("M,N,K", SHAPES)
+@pytest.mark.parametrize("f32", [False, True])
+def test_product(M, N, K, f32):
+    from dsgx10_b200 import linear
+    blocks, w = _make(N, K, 11 * N + K)
+    x = _x(M, K, M + K)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = linear.linear_decode(linear.LinearW(N, K, blocks), x.cuda(), out_dtype=torch.float32 if f32 else torch.bfloat16, status=status)
+    assert int(status) == 0
+    _check(got, x.double() @ w.T, x.double().abs() @ w.abs().T, K)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 7, 40), (4, 1000, 1024), (6, 129, 3000), (16, 520, 5120), (1, 9000, 2048)])
+def test_swiglu(M, N, K):
+    """h = silu(g) u: an error dg moves silu by at most 1.1 dg (its slope is below 1.1); expf, the division and the product
+    are within 8 x 2^-24 of the value."""
+    from dsgx10_b200 import linear
+    (bg, wg), (bu, wu) = _make(N, K, 5), _make(N, K, 6, zeros=False)
+    x = _x(M, K, 3)
+    got = linear.linear_decode(linear.LinearW(N, K, bg, up=bu), x.cuda())
+    g, u = x.double() @ wg.T, x.double() @ wu.T
+    dg, du = (_gamma(K) * (x.double().abs() @ w.abs().T) for w in (wg, wu))
+    act = g * torch.sigmoid(g)
+    h = act * u
+    _check(got, h, 0 * h, K, extra=1.1 * dg * (u.abs() + du) + act.abs() * du + h.abs() * 8 * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("f32", [False, True])
+def test_residual_and_in_place(f32):
+    """One rounding after the residual's add (which rounds once more in f32: 2^-24 of the sum)."""
+    from dsgx10_b200 import linear
+    M, N, K = 5, 333, 1500
+    blocks, w = _make(N, K, 21)
+    x, res = _x(M, K, 22), _x(M, N, 23)
+    lw = linear.LinearW(N, K, blocks)
+    y = x.double() @ w.T + res.double()
+    got = linear.linear_decode(lw, x.cuda(), res=res.cuda(), out_dtype=torch.float32 if f32 else torch.bfloat16)
+    _check(got, y, x.double().abs() @ w.abs().T, K, extra=2.0 ** -24 * y.abs())
+    if not f32:
+        r = res.cuda()
+        assert linear.linear_decode(lw, x.cuda(), res=r, out=r) is r and torch.equal(r, got)
+
+
+def test_rows_do_not_depend_on_each_other():
+    """A row alone, among four, eight or sixteen (another kernel, another split of K): the same bits; twice: the same bits."""
+    from dsgx10_b200 import linear
+    for N, K in ((500, 6144), (2000, 1111), (16, 9000)):
+        blocks, _ = _make(N, K, N)
+        lw = linear.LinearW(N, K, blocks)
+        x = _x(16, K, K).cuda()
+        all16 = linear.linear_decode(lw, x, out_dtype=torch.float32)
+        assert torch.equal(all16, linear.linear_decode(lw, x, out_dtype=torch.float32))
+        for m in (1, 3, 4, 5, 8, 9, 13):
+            assert torch.equal(linear.linear_decode(lw, x[16 - m:], out_dtype=torch.float32), all16[16 - m:]), (N, K, m)
+
+
+def test_inf_and_nan_stay_in_their_row():
+    from dsgx10_b200 import linear
+    N, K = 200, 1030
+    blocks, _ = _make(N, K, 41)
+    lw = linear.LinearW(N, K, blocks)
+    for M in (2, 7, 12):
+        x = _x(M, K, 42).cuda()
+        clean = linear.linear_decode(lw, x)
+        bad = x.clone()
+        bad[1, 5], bad[M - 1, K - 1] = float("nan"), float("inf")
+        got = linear.linear_decode(lw, bad)
+        keep = [r for r in range(M) if r not in (1, M - 1)]
+        assert torch.equal(got[keep], clean[keep]) and bool(got[1].isnan().all()) and not bool(got[M - 1].isfinite().any())
+
+
+def test_strided_and_unaligned_rows():
+    """Rows of larger tensors, at addresses that are no multiples of 16 bytes: the bits of the packed call; nothing
+    outside the rows is written."""
+    from dsgx10_b200 import linear
+    M, N, K = 6, 77, 1001
+    blocks, _ = _make(N, K, 51)
+    lw = linear.LinearW(N, K, blocks)
+    x, res = _x(M, K, 52).cuda(), _x(M, N, 53).cuda()
+    want = linear.linear_decode(lw, x, res=res)
+    for off, pad in ((0, 7), (3, 12), (8, 8)):
+        xs = torch.full((M, K + pad + off), float("nan"), dtype=torch.bfloat16, device="cuda")
+        xs[:, off:off + K] = x
+        rs = torch.full((M, N + pad + off), float("nan"), dtype=torch.bfloat16, device="cuda")
+        rs[:, off:off + N] = res
+        os_ = torch.full((M, N + pad + off), 7.0, dtype=torch.bfloat16, device="cuda")
+        linear.linear_decode(lw, xs[:, off:off + K], res=rs[:, off:off + N], out=os_[:, off:off + N])
+        assert torch.equal(os_[:, off:off + N], want)
+        rest = torch.cat([os_[:, :off], os_[:, off + N:]], 1)
+        assert bool((rest == 7.0).all())
+
+
+def test_streams_and_graph():
+    """Two streams at once, and a captured chain (gate/up, down with the residual in place) replayed on new inputs: the bits
+    of the eager calls."""
+    from dsgx10_b200 import linear
+    H, I, M = 1024, 1536, 2
+    gate, up, down = (linear.LinearW(n, k, _make(n, k, 60 + i)[0]) for i, (n, k) in enumerate(((I, H), (I, H), (H, I))))
+    gu = linear.LinearW(I, H, gate.blocks, up=up.blocks)
+
+    def layer(x, out=None):
+        return linear.linear_decode(down, linear.linear_decode(gu, x), res=x, out=out)
+
+    xs = [_x(M, H, 70 + i).cuda() for i in range(6)]
+    want = [layer(x) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for i, x in enumerate(xs):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(layer(x))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    x, out = xs[0].clone(), torch.empty_like(xs[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        layer(x, out=out)
+    for i in (3, 1, 5):
+        x.copy_(xs[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[i])
+
+
+def test_python_refusals():
+    from dsgx10_b200 import linear
+    N, K = 64, 700
+    blocks, _ = _make(N, K, 81)
+    lw = linear.LinearW(N, K, blocks)
+    x = _x(2, K, 82).cuda()
+    for bad in (x.float(), x[:, :-1], x.cpu(), x[0], _x(17, K, 1).cuda(), torch.empty(K, 2, dtype=torch.bfloat16, device="cuda").T,
+                x[:0], x[:1].expand(2, K)):
+        with pytest.raises(ValueError):
+            linear.linear_decode(lw, bad)
+    for kw in (dict(res=x), dict(out=x), dict(out=torch.empty(2, N, dtype=torch.float16, device="cuda"))):
+        with pytest.raises(ValueError):
+            linear.linear_decode(lw, x, **kw)
+    for bad in (blocks[:-1], blocks.cpu(), blocks.view(torch.int16)):
+        with pytest.raises(ValueError):
+            linear.LinearW(N, K, bad)
+    from dsgx10_b200 import _lib
+    with pytest.raises(_lib.DsgxError):
+        linear.linear_decode(linear.LinearW(N, K, blocks, up=blocks), x, res=torch.zeros(2, N, dtype=torch.bfloat16, device="cuda"))

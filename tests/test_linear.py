@@ -1,0 +1,47 @@
+"""The dense INT4 products without a GPU: the packing of any size, and the calls that are refused."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from dsgx10_b200 import _lib, weights
+from tests.linear_util import random_int4, unpack
+
+
+@pytest.mark.parametrize("N,K", [(1, 1), (8, 512), (9, 513), (17, 31), (40, 1000), (3, 32)])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_pack_linear_int4_keeps_every_weight(N, K, zeros):
+    wp, s, zp, w = random_int4(N, K, 7 * N + K, zeros)
+    blocks = weights.pack_linear_int4(wp, s, zp, K=K)
+    assert blocks.size == -(-N // 8) * -(-K // 512) * 2368
+    full = unpack(blocks, -(-N // 8) * 8, -(-K // 512) * 512)
+    assert (full[:N, :K] == w).all()
+    kg = -(-K // 32) * 32   # (what shares a group with a real weight has its scale; behind that the scales are 0)
+    assert (full[N:] == 0).all() and (full[:, kg:] == 0).all()
+
+
+def test_pack_linear_int4_refuses_what_does_not_fit():
+    wp, s, zp, _ = random_int4(9, 100, 1, True)
+    for bad in ((wp[:, :-1], s, zp), (wp, s[:, :-1], zp), (wp, s[:-1], zp), (wp, s, zp[:-1])):
+        with pytest.raises(ValueError):
+            weights.pack_linear_int4(*bad, K=100)
+
+
+def test_refused_calls():
+    """Every refusal comes before anything is launched, so it shows without a GPU."""
+    L = _lib.lib()
+    one = 1 << 20   # (an aligned address that nothing reads)
+
+    def call(w=one, up=None, N=64, K=512, fmt=_lib.FMT_INT4, x=one, ldx=512, M=1, res=None, ldr=64, out=one, ldo=64, f32=0, status=None):
+        W = _lib.LinearW(w, up, N, K, fmt, 0)
+        return L.dsgx_linear_decode(C.byref(W), x, ldx, M, res, ldr, out, ldo, f32, status, None)
+
+    assert L.dsgx_linear_decode(None, one, 512, 1, None, 0, one, 64, 0, None, None) == _lib.ERR_ARG
+    for kw in (dict(w=None), dict(x=None), dict(out=None), dict(M=0), dict(M=17), dict(ldx=511), dict(ldo=63), dict(res=one, ldr=63),
+               dict(w=one + 8), dict(up=one + 4), dict(x=one + 1), dict(out=one + 1), dict(out=one + 2, f32=1), dict(res=one + 1), dict(status=one + 2)):
+        assert call(**kw) == _lib.ERR_ARG, kw
+    for fmt in (_lib.FMT_NVFP4, _lib.FMT_RETIRED, _lib.FMT_BF16, _lib.FMT_FP8, _lib.FMT_MXFP4, 77):
+        assert call(fmt=fmt) == _lib.ERR_FORMAT
+    for kw in (dict(N=0), dict(K=0), dict(N=-5), dict(K=(1 << 30) + 1, ldx=1 << 31)):
+        assert call(**kw) == _lib.ERR_SHAPE, kw
+    assert call(up=one, res=one) == _lib.ERR_UNSUPPORTED
