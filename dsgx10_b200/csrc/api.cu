@@ -422,7 +422,7 @@ int dsgx_linear_decode(const dsgx_linear_w* W, const void* x, int64_t ldx, int M
   p.out = out, p.ldx = ldx, p.ldr = ldr, p.ldo = ldo, p.M = M, p.N = W->N, p.K = W->K;
   p.n8 = (W->N + 7) / 8, p.nb = (W->K + 511) / 512, p.units = W->w_up ? p.n8 : (p.n8 + 1) / 2;
   p.out_f32 = out_f32 != 0, p.x_vec = ((uintptr_t)x & 15) == 0 && ldx % 8 == 0;
-  p.cluster = 1, p.xblocks = 0, p.status = status_word;
+  p.cluster = 1, p.lc = 0, p.xblocks = 0, p.lq = 0, p.status = status_word;
   bool fits = false;
   cudaError_t e = launch_linear_int4(p, (cudaStream_t)stream, &fits);
   if (e != cudaSuccess) return cuda_fail(e);

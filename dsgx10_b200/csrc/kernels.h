@@ -157,7 +157,8 @@ struct LinearParams {
   long long ldx, ldr, ldo;
   int M, N, K, n8, nb, units;  // units of 16 output rows (SwiGLU: 8 + 8)
   int out_f32, x_vec;
-  int cluster, xblocks;        // chosen by the launch: CTAs a cluster, blocks of K a rank holds at most
+  // chosen by the launch: CTAs a cluster (and its logarithm), blocks of K a rank holds at most, 2^lq tasks a unit
+  int cluster, lc, xblocks, lq;
   int* status;
 };
 cudaError_t launch_linear_int4(const LinearParams& p, cudaStream_t st, bool* fits);

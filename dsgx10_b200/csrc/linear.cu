@@ -2,20 +2,20 @@
 // residual added, or with a second matrix silu(x W^T) * (x W_up^T).  (The expert kernels' weight blocks, decode_int4.cu.)
 //
 // Bound: the weights are read once (0.578 bytes a weight), so HBM; the conversion of the nibbles in registers is the next
-// limit (int4_pair.cuh).  Work is cut in units of 16 output rows (SwiGLU: 8 gate + 8 up) and a unit in pairs of 8 x 512
-// blocks.  A CTA owns a run of units and its 16 stream warps take the run's block pairs in turn, each through a private
-// ring of bulk copies: every SM streams from one contiguous run whatever N and K are, no warp owns more than a block pair
-// at a time, and the launch ends within one unit on every SM.  A warp's sums of a block pair go to shared memory; one more
-// warp adds a unit's partial sums in ascending k and writes the outputs, so that the stream never waits for a reduction.
+// limit (int4_pair.cuh).  Work is cut in units of 16 output rows (SwiGLU: 8 gate + 8 up), a unit along K in 1, 2, 4 or 8 tasks,
+// a task in pairs of 8 x 512 blocks.  A CTA owns a run of units and its stream warps take the run's tasks in turn, each
+// through a private ring of bulk copies, so that every SM streams one contiguous run and the launch ends within a task
+// on every SM.  A task's sums go to shared memory; one more warp joins the tasks of a unit and writes the outputs, so
+// that the stream never waits for a reduction.
 //
-// K over a cluster: with C > 1 (1, 2, 4 or 8 CTAs) the ranks of a cluster take consecutive runs of K of the same units.  The
-// activations of M rows are held in shared memory for a rank's own run only, and a matrix with few units still occupies
-// every SM.  A rank's partial sums of a unit go to the unit's owner (unit modulo C) through distributed shared memory, and the
-// owner adds the ranks.
+// K over a cluster: with C > 1 (2, 4 or 8 CTAs) the ranks of a cluster take consecutive parts of K of the same units.  The
+// activations of M rows are held in shared memory for a rank's own part only, and a matrix with few units still occupies
+// every SM.  A rank's sums of a unit go to the unit's owner (unit modulo C) through distributed shared memory; the owner's
+// adding warp joins them a few units later, when the others' have arrived.
 //
-// The order of a sum is the same for every cluster size: K's blocks fall into eight runs (block nb r / 8 on), a run is summed
-// in ascending order from zero, and the runs are joined as a binary tree, ((r0 + r1) + (r2 + r3)) + ((r4 + r5) + (r6 + r7)),
-// of which a rank holds a whole subtree.  So a row's bits do not depend on the rows beside it or on their number.
+// The order of a sum is the same for every division of the work: K's blocks fall into eight runs (block nb r / 8 on), a run
+// is summed in ascending order from zero, and the runs are joined as a binary tree, ((r0 + r1) + (r2 + r3)) + ((r4 + r5) + (r6 +
+// r7)), of which a task and a rank hold whole subtrees.  So a row's bits do not depend on the rows beside it or their number.
 #include <atomic>
 
 #include "common.cuh"
@@ -26,12 +26,12 @@ namespace dsgx {
 
 namespace {
 
-constexpr int kSlotsOwned = 2;   // a rank's receive buffers for units that the cluster has in flight
+constexpr int kSlotsOwned = 4;   // a rank's receive buffers: units of its own that the cluster has in flight
 constexpr int kMaxCluster = 8;
 constexpr int kRuns = 8;         // the parts of K whose sums are joined as a tree
 constexpr size_t kSmemMax = 227 * 1024;
 
-// W stream warps, P partial sums in flight; S sets of four tokens
+// W stream warps with NST ring stages each, P tasks' sums in flight (a power of two); S sets of four tokens
 template <int S_, int W_, int NST_, int P_>
 struct LinVar {
   static constexpr int S = S_, W = W_, NST = NST_, P = P_;
@@ -39,7 +39,7 @@ struct LinVar {
   static constexpr int kPart = 256 * S;  // bytes of a block pair's (or a rank's) sums: [S][32 lanes][2] f32
   static constexpr size_t kFixed = (size_t)W * NST * kPairStage + (size_t)P * kPart + 128;
   static size_t smem(int M, int kblocks, int C) {
-    return kFixed + (C > 1 ? (size_t)kSlotsOwned * kMaxCluster * kPart : 0) + (size_t)kblocks * M * 1024 + 32 +
+    return kFixed + (C > 1 ? (size_t)kSlotsOwned * kMaxCluster * kPart : 0) + (size_t)kblocks * M * 1024 + 64 +
            (W * NST + kSlotsOwned * (1 + kMaxCluster)) * 8 + P * 4 + 64;
   }
 };
@@ -105,8 +105,8 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
   uint8_t* part = ring + (size_t)W * NST * kPairStage;                 // [P][S][32][2] f32
   uint8_t* recv = part + (size_t)P * kPart;                            // [kSlotsOwned][C][S][32][2] f32
   uint8_t* xt = recv + (C > 1 ? (size_t)kSlotsOwned * kMaxCluster * kPart : 0);
-  uint8_t* zero = xt + (size_t)p.xblocks * p.M * 1024;                  // 32 bytes
-  uint64_t* bars = reinterpret_cast<uint64_t*>(zero + 32);
+  uint8_t* zero = xt + (size_t)p.xblocks * p.M * 1024 + 16;             // 32 bytes
+  uint64_t* bars = reinterpret_cast<uint64_t*>(zero + 48);
   uint64_t* rfull = bars + W * NST;                                    // [kSlotsOwned] every rank's sums are in my buffer
   uint64_t* rfree = rfull + kSlotsOwned;                               // [owner][kSlotsOwned] that owner's buffer may be written
   int* cnt = reinterpret_cast<int*>(rfree + kMaxCluster * kSlotsOwned);  // [P] block pairs summed of a unit in flight
@@ -128,7 +128,9 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
   else __syncthreads();
   pdl_launch_dependents();
 
-  const int total = (u1 - u0) * nbk;  // this CTA's block pairs
+  const int lq = p.lq, Q = 1 << lq, RPT = (kRuns / C) >> lq;  // tasks a unit (this rank's part), runs a task
+  const int total = (u1 - u0) << lq;                          // this CTA's tasks
+  const int r0 = (int)rank * (kRuns / C);                     // this rank's first run
   const size_t strip = (size_t)p.nb * kQBlk;
   const bool glu = p.w_up != nullptr;
 
@@ -136,38 +138,50 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
   uint8_t* myring = ring + (size_t)warp * NST * kPairStage;
   uint64_t* mybar = bars + warp * NST;
   uint32_t issued = 0;
-  int pj = warp;
+  int pj = warp, pb = 0, pe = 0;  // the producer's task and its next and last block
+  const uint8_t *pa = nullptr, *pc = nullptr;
   const uint64_t pol = policy_evict_first();
-  auto issue = [&]() {
-    const int u = u0 + pj / nbk, b = b0 + pj % nbk;
-    const uint8_t *a, *c;
-    if (glu) {
-      a = p.w + (size_t)u * strip, c = p.w_up + (size_t)u * strip;
-    } else {
-      a = p.w + (size_t)(2 * u) * strip;
-      c = 2 * u + 1 < p.n8 ? a + strip : a;  // (an odd number of strips: the last unit's second half is not written)
+  auto open_task = [&]() {  // the next task with a block in it (K shorter than eight blocks: some runs are empty)
+    while (pb == pe && pj < total) {
+      const int u = u0 + (pj >> lq), r = r0 + (pj & (Q - 1)) * RPT;
+      pb = p.nb * r / kRuns, pe = p.nb * (r + RPT) / kRuns;
+      if (pb == pe) {
+        pj += W;
+        continue;
+      }
+      if (glu) {
+        pa = p.w + (size_t)u * strip, pc = p.w_up + (size_t)u * strip;
+      } else {
+        pa = p.w + (size_t)(2 * u) * strip;
+        pc = 2 * u + 1 < p.n8 ? pa + strip : pa;  // (an odd number of strips: the last unit's second half is not written)
+      }
     }
+    return pj < total;
+  };
+  auto issue = [&]() {
     uint8_t* st = myring + (issued % NST) * kPairStage;
     uint64_t* bar = mybar + issued % NST;
     mbar_expect_tx(bar, kPairBytes);
-    bulk_g2s_hint(st, a + (size_t)b * kQBlk, kQBlk, bar, pol);
-    bulk_g2s_hint(st + kQBlk, c + (size_t)b * kQBlk, kQBlk, bar, pol);
-    ++issued, pj += W;
+    bulk_g2s_hint(st, pa + (size_t)pb * kQBlk, kQBlk, bar, pol);
+    bulk_g2s_hint(st + kQBlk, pc + (size_t)pb * kQBlk, kQBlk, bar, pol);
+    ++issued;
+    if (++pb == pe) pj += W;
   };
   if (warp < W && lane == 0)
-    for (int s = 0; s < NST && pj < total; ++s) issue();
+    for (int s = 0; s < NST && open_task(); ++s) issue();
 
   // ---- this rank's activations ------------------------------------------------------------------------------------------
   pdl_wait();
   {
     const bool vec = p.x_vec != 0;
-    for (int i = threadIdx.x; i < nbk * 32 * p.M; i += V::kThreads) {
-      const int kg = i / p.M, r = i % p.M;
-      uint4 o[2];
-      tile_group(o, p.x + (size_t)r * p.ldx, b0 * 512 + 16 * kg, p.K, vec);
-      uint4* d = reinterpret_cast<uint4*>(xt + (size_t)i * 32);
-      d[0] = o[0], d[1] = o[1];
-    }
+    const int n = nbk * 32;
+    for (int r = 0; r < p.M; ++r)
+      for (int kg = threadIdx.x; kg < n; kg += V::kThreads) {
+        uint4 o[2];
+        tile_group(o, p.x + (size_t)r * p.ldx, b0 * 512 + 16 * kg, p.K, vec);
+        uint4* d = reinterpret_cast<uint4*>(xt + ((size_t)((kg >> 2) * p.M + r) * 4 + (kg & 3)) * 32);
+        d[0] = o[0], d[1] = o[1];
+      }
   }
   __syncthreads();
 
@@ -176,135 +190,146 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
     XCols<S> cols;
     xcols_int4<S>(cols, xt, p.M, zero, lane, [&](int s, int j) { return 4 * s + j < p.M ? 4 * s + j : -1; });
     uint32_t consumed = 0;
-    for (int j = warp; j < total; j += W) {
-      const uint32_t si = consumed % NST;
-      if (!mbar_wait(mybar + si, (consumed / NST) & 1)) {
-        *fail = 1;
-        break;
-      }
-      float acc[S][2];
+    bool ok = true;
+    for (int j = warp; j < total && ok; j += W) {
+      const int rt = r0 + (j & (Q - 1)) * RPT;
+      float2 sum[S], lv[3][S];  // the run or subtree just finished; the subtrees that wait for their right halves
+      int b = p.nb * rt / kRuns;
+      for (int r = 0; r < RPT && ok; ++r) {
+        const int e = p.nb * (rt + r + 1) / kRuns;
+        float acc[S][2];
 #pragma unroll
-      for (int s = 0; s < S; ++s) acc[s][0] = acc[s][1] = 0.f;
-      XCols<S> xc = cols;
+        for (int s = 0; s < S; ++s) acc[s][0] = acc[s][1] = 0.f;
+        for (; b < e; ++b) {
+          const uint32_t si = consumed % NST;
+          if (!mbar_wait(mybar + si, (consumed / NST) & 1)) {
+            ok = false;
+            break;
+          }
+          XCols<S> xc = cols;
 #pragma unroll
-      for (int s = 0; s < S; ++s) xc.p[s] += (size_t)(j % nbk) * 8 * xc.step[s];
-      const uint8_t* st = myring + si * kPairStage;
-      int4_pair<S>(acc, st, st + kQBlk, xc, lane);
-      ++consumed;
-      __syncwarp();
-      if (lane == 0 && pj < total) issue();
-      // the sums into the partial buffer, once the buffer's last unit has been added up
-      if (j >= ld_shared_acquire(done) + P) {
-        const long long t0 = clock64();
-        bool ok = true;
-        while (ok && j >= ld_shared_acquire(done) + P) ok = clock64() - t0 < kWaitCycles;
-        if (!ok) {
-          *fail = 1;
-          break;
+          for (int s = 0; s < S; ++s) xc.p[s] += (size_t)(b - b0) * 8 * xc.step[s];
+          const uint8_t* st = myring + si * kPairStage;
+          int4_pair<S>(acc, st, st + kQBlk, xc, lane);
+          ++consumed;
+          __syncwarp();
+          if (lane == 0 && open_task()) issue();
+        }
+        const bool j0 = r & 1, j1 = (r & 3) == 3, j2 = r == 7;  // how many waiting subtrees this run completes
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+          sum[s] = make_float2(acc[s][0], acc[s][1]);
+          if (j0) sum[s] = add2(lv[0][s], sum[s]);
+          if (j1) sum[s] = add2(lv[1][s], sum[s]);
+          if (j2) sum[s] = add2(lv[2][s], sum[s]);
+          if (!j0) lv[0][s] = sum[s];
+          else if (!j1) lv[1][s] = sum[s];
+          else if (!j2) lv[2][s] = sum[s];
         }
       }
-      float2* d = reinterpret_cast<float2*>(part + (size_t)(j % P) * kPart) + lane;
+      // the sums into the partial buffer, once the unit that had the place has been added up
+      if (ok && j >= ld_shared_acquire(done) + P) {
+        const long long t0 = clock64();
+        while (ok && j >= ld_shared_acquire(done) + P) {
+          __nanosleep(100);
+          ok = clock64() - t0 < kWaitCycles;
+        }
+      }
+      if (!ok) break;
+      float2* d = reinterpret_cast<float2*>(part + (size_t)(j & (P - 1)) * kPart) + lane;
 #pragma unroll
-      for (int s = 0; s < S; ++s) d[32 * s] = make_float2(acc[s][0], acc[s][1]);
+      for (int s = 0; s < S; ++s) d[32 * s] = sum[s];
       __threadfence_block();
       __syncwarp();
-      if (lane == 0) atomicAdd(cnt + (j / nbk) % P, 1);
+      if (lane == 0) atomicAdd(cnt + ((j >> lq) & (P - 1)), 1);
     }
+    if (!ok) *fail = 1;
     if (lane == 0)  // (only after a wait that ran out: no copy is left in flight)
       for (; consumed < issued; ++consumed) mbar_wait(mybar + consumed % NST, (consumed / NST) & 1);
   } else {
     // ---- the adding warp ------------------------------------------------------------------------------------------------
-    const int g = lane >> 2, t = lane & 3;
-    bool ok = true;
-    for (int i = 0; i < u1 - u0 && ok; ++i) {
-      const int* c = cnt + i % P;
-      if (ld_shared_acquire(c) < nbk) {
-        const long long t0 = clock64();
-        while (ok && ld_shared_acquire(c) < nbk) ok = clock64() - t0 < kWaitCycles;
-        if (!ok) break;
+    const int g = lane >> 2, t = lane & 3, n = u1 - u0, lc = p.lc;
+    const int lag = C > 1 ? C * (kSlotsOwned / 2) : 0;  // an owner joins the ranks' sums this many units later
+    float2 a[S];
+    auto join = [&](const float2* d, int stride, int parts) {  // parts sums (1, 2, 4 or 8), as a tree
+      auto two = [&](int i, int s) { return add2(d[i * stride + 32 * s], d[(i + 1) * stride + 32 * s]); };
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        if (parts == 1) a[s] = d[32 * s];
+        else if (parts == 2) a[s] = two(0, s);
+        else if (parts == 4) a[s] = add2(two(0, s), two(2, s));
+        else a[s] = add2(add2(two(0, s), two(2, s)), add2(two(4, s), two(6, s)));
       }
-      // this rank's runs of K (kRuns / C of the eight), each in ascending order, joined pairwise
-      float2 a[S], lv[3][S];
-      int b = 0;
+    };
+    auto write = [&](int unit) {
 #pragma unroll
-      for (int r = 0; r < kRuns; ++r) {
-        if (r < kRuns / C) {
-          const int e = p.nb * ((int)rank * (kRuns / C) + r + 1) / kRuns - b0;
-#pragma unroll
-          for (int s = 0; s < S; ++s) a[s] = make_float2(0.f, 0.f);
-          for (; b < e; ++b) {
-            const float2* d = reinterpret_cast<const float2*>(part + (size_t)((i * nbk + b) % P) * kPart) + lane;
-#pragma unroll
-            for (int s = 0; s < S; ++s) a[s] = add2(a[s], d[32 * s]);
+      for (int s = 0; s < S; ++s) {
+        const int m = 4 * s + t;
+        if (m >= p.M) continue;
+        if (glu) {
+          const int c = 8 * unit + g;
+          if (c < p.N) {
+            const float h = __fmul_rn(silu(a[s].x), a[s].y);
+            if (p.out_f32) reinterpret_cast<float*>(p.out)[(size_t)m * p.ldo + c] = h;
+            else reinterpret_cast<__nv_bfloat16*>(p.out)[(size_t)m * p.ldo + c] = __float2bfloat16_rn(h);
           }
-          int l = 0;
+        } else {
 #pragma unroll
-          for (int k = r; k & 1; k >>= 1, ++l)
-#pragma unroll
-            for (int s = 0; s < S; ++s) a[s] = add2(lv[l][s], a[s]);
-          if (l < 3)
-#pragma unroll
-            for (int s = 0; s < S; ++s) lv[l][s] = a[s];
+          for (int hi = 0; hi < 2; ++hi) {
+            const int c = 16 * unit + 8 * hi + g;
+            if (c < p.N) {
+              float y = hi ? a[s].y : a[s].x;
+              if (p.res) y = __fadd_rn(y, __bfloat162float(p.res[(size_t)m * p.ldr + c]));
+              if (p.out_f32) reinterpret_cast<float*>(p.out)[(size_t)m * p.ldo + c] = y;
+              else reinterpret_cast<__nv_bfloat16*>(p.out)[(size_t)m * p.ldo + c] = __float2bfloat16_rn(y);
+            }
+          }
         }
       }
-      __syncwarp();
-      if (lane == 0) {
-        cnt[i % P] = 0;
-        st_shared_release(done, (i + 1) * nbk);
-      }
-      if (C > 1) {
-        // to the unit's owner, once it has let go of the unit that had the buffer before; the owner adds the ranks in order
-        const int owner = i % C, slot = (i / C) % kSlotsOwned, turn = i / C / kSlotsOwned;
-        if (turn > 0 && !mbar_wait_cluster(rfree + owner * kSlotsOwned + slot, (turn - 1) & 1)) {
-          ok = false;
-          break;
+    };
+    bool ok = true;
+    for (int i = 0; i < n + lag && ok; ++i) {
+      if (i < n) {
+        int* c = cnt + (i & (P - 1));
+        if (ld_shared_acquire(c) < Q) {
+          const long long t0 = clock64();
+          while (ok && ld_shared_acquire(c) < Q) {
+            __nanosleep(40);
+            ok = clock64() - t0 < kWaitCycles;
+          }
+          if (!ok) break;
         }
-        const uint32_t to = map_rank(smem_u32(recv) + (uint32_t)((slot * kMaxCluster + (int)rank) * kPart + lane * 8), owner);
+        join(reinterpret_cast<const float2*>(part + (size_t)((i << lq) & (P - 1)) * kPart) + lane, kPart / 8, Q);
+        __syncwarp();
+        if (lane == 0) {
+          *c = 0;
+          st_shared_release(done, (i + 1) << lq);
+        }
+        if (C == 1) {
+          write(u0 + i);
+        } else {  // to the unit's owner, once it has let go of the unit that had the buffer before
+          const int owner = i & (C - 1), slot = (i >> lc) % kSlotsOwned, turn = (i >> lc) / kSlotsOwned;
+          if (turn > 0 && !mbar_wait_cluster(rfree + owner * kSlotsOwned + slot, (turn - 1) & 1)) {
+            ok = false;
+            break;
+          }
+          const uint32_t to = map_rank(smem_u32(recv) + (uint32_t)((slot * kMaxCluster + (int)rank) * kPart + lane * 8), owner);
 #pragma unroll
-        for (int s = 0; s < S; ++s) st_remote(to + 256 * s, a[s]);
-        remote_arrive(map_rank(smem_u32(rfull + slot), owner));
-        if (owner != (int)rank) continue;
+          for (int s = 0; s < S; ++s) st_remote(to + 256 * s, a[s]);
+          remote_arrive(map_rank(smem_u32(rfull + slot), owner));
+        }
+      }
+      const int o = i - lag;
+      if (C > 1 && o >= 0 && o < n && (o & (C - 1)) == (int)rank) {
+        const int slot = (o >> lc) % kSlotsOwned, turn = (o >> lc) / kSlotsOwned;
         if (!mbar_wait_cluster(rfull + slot, turn & 1)) {
           ok = false;
           break;
         }
-        const float2* d = reinterpret_cast<const float2*>(recv + (size_t)slot * kMaxCluster * kPart) + lane;
-        constexpr int kStep = kPart / 8;  // the ranks' sums, joined pairwise like the runs
-        auto rank_pair = [&](int r, int s) { return add2(d[r * kStep + 32 * s], d[(r + 1) * kStep + 32 * s]); };
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-          a[s] = rank_pair(0, s);
-          if (C >= 4) a[s] = add2(a[s], rank_pair(2, s));
-          if (C >= 8) a[s] = add2(a[s], add2(rank_pair(4, s), rank_pair(6, s)));
-        }
+        join(reinterpret_cast<const float2*>(recv + (size_t)slot * kMaxCluster * kPart) + lane, kPart / 8, C);
         __syncwarp();
         if (lane < C) remote_arrive(map_rank(smem_u32(rfree + rank * kSlotsOwned + slot), lane));
-      }
-      const int unit = u0 + i;
-#pragma unroll
-      for (int s = 0; s < S; ++s) {
-        const int m = 4 * s + t;
-        if (m < p.M) {
-          if (glu) {
-            const int n = 8 * unit + g;
-            if (n < p.N) {
-              const float h = __fmul_rn(silu(a[s].x), a[s].y);
-              if (p.out_f32) reinterpret_cast<float*>(p.out)[(size_t)m * p.ldo + n] = h;
-              else reinterpret_cast<__nv_bfloat16*>(p.out)[(size_t)m * p.ldo + n] = __float2bfloat16_rn(h);
-            }
-          } else {
-#pragma unroll
-            for (int hi = 0; hi < 2; ++hi) {
-              const int n = 16 * unit + 8 * hi + g;
-              if (n < p.N) {
-                float y = hi ? a[s].y : a[s].x;
-                if (p.res) y = __fadd_rn(y, __bfloat162float(p.res[(size_t)m * p.ldr + n]));
-                if (p.out_f32) reinterpret_cast<float*>(p.out)[(size_t)m * p.ldo + n] = y;
-                else reinterpret_cast<__nv_bfloat16*>(p.out)[(size_t)m * p.ldo + n] = __float2bfloat16_rn(y);
-              }
-            }
-          }
-        }
+        write(u0 + o);
       }
     }
     if (!ok) *fail = 1;
@@ -370,6 +395,12 @@ cudaError_t launch(LinearParams p, cudaStream_t st, bool* fits) {
   *fits = best != 0;
   if (!best) return cudaSuccess;
   p.cluster = best, p.xblocks = (p.nb + best - 1) / best;
+  p.lc = best == 8 ? 3 : best == 4 ? 2 : best == 2 ? 1 : 0;
+  // Tasks a unit: as few as leave every stream warp of a CTA eight tasks (the last task of a launch is idle time of the
+  // others), at most one a block or a run.
+  const int per_cta = (p.units + clusters - 1) / clusters;
+  p.lq = 0;
+  while ((2 << p.lq) <= kRuns / best && (2 << p.lq) <= p.xblocks && (per_cta << p.lq) < 8 * V::W) ++p.lq;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((p.units < clusters ? p.units : clusters) * best), cfg.blockDim = dim3(V::kThreads);
   cfg.dynamicSmemBytes = V::smem(p.M, p.xblocks, best), cfg.stream = st;
@@ -386,9 +417,9 @@ cudaError_t launch(LinearParams p, cudaStream_t st, bool* fits) {
 
 // One launch for M rows, or *fits = false where their activations do not fit shared memory.
 cudaError_t launch_linear_int4(const LinearParams& p, cudaStream_t st, bool* fits) {
-  if (p.M <= 4) return launch<LinVar<1, 16, 2, 64>>(p, st, fits);
-  if (p.M <= 8) return launch<LinVar<2, 16, 2, 32>>(p, st, fits);
-  return launch<LinVar<4, 12, 2, 24>>(p, st, fits);
+  if (p.M <= 4) return launch<LinVar<1, 15, 2, 64>>(p, st, fits);
+  if (p.M <= 8) return launch<LinVar<2, 15, 2, 32>>(p, st, fits);
+  return launch<LinVar<4, 11, 2, 16>>(p, st, fits);
 }
 
 }  // namespace dsgx
