@@ -22,11 +22,30 @@ constexpr int kHBlk = 2048;                          // a bf16 block: 8 rows x 1
 constexpr int kPairBytes = 2 * kQBlk;
 constexpr int kPairStage = (kPairBytes + 127) & ~127;  // (two bf16 blocks, 4096 B, fit)
 
+// shared memory by 32-bit addresses (a generic pointer costs 64-bit arithmetic in the inner loop)
+DSGX_DEV uint4 lds_v4(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+DSGX_DEV uint32_t lds_u32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
 // nibbles i and i + 4 of a word minus the zero point, as bf16x2 (zz = 128 + z in both halves): 0x4300 | u is 128 + u
 DSGX_DEV uint32_t nib_pair(uint32_t w, int i, uint32_t zz) {
-  const uint32_t v = ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+  uint32_t v;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(w >> (4 * i)), "r"(0x000F000Fu), "r"(0x43004300u));  // (w & m) | c
   const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&zz));
   return *reinterpret_cast<const uint32_t*>(&r);
+}
+// c += a b on both halves of a register pair
+DSGX_DEV void fma2(float2& c, float2 a, float2 b) {
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%0, %1};\n\t"
+      "fma.rn.f32x2 z, x, y, z;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "+f"(c.x), "+f"(c.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
 }
 DSGX_DEV void mma_bf16_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -41,30 +60,31 @@ DSGX_DEV void mma_bf16_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2
 // without a token, read 32 bytes of zeros (step 0) that lie 16 bytes off a multiple of 32: the banks the others leave free.
 template <int S>
 struct XCols {
-  const uint8_t* p[S];
+  uint32_t p[S];     // shared-memory address
   uint32_t step[S];  // bytes from one 64-k span to the next
 };
 // tok(s, j): the tile row of the j-th token of set s, negative: none
 template <int S, class F>
-DSGX_DEV void xcols_int4(XCols<S>& x, const uint8_t* tile, int rows, const uint8_t* zero, int lane, F tok) {
+DSGX_DEV void xcols_int4(XCols<S>& x, uint32_t tile, int rows, uint32_t zero, int lane, F tok) {
   const int g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int s = 0; s < S; ++s) {
     const int r = tok(s, g >> 1);
     const bool on = r >= 0 && (t >> 1) == (g & 1);
-    x.p[s] = on ? tile + ((size_t)r * 4 + t) * 32 : zero;
+    x.p[s] = on ? tile + (r * 4 + t) * 32 : zero;
     x.step[s] = on ? 4u * rows * 32 : 0u;
   }
 }
 
-// acc[s][0 / 1] += row g of strip a / b times token 4 s + t, over the 512 k of one block pair; x at the block's first k
+// acc[s][0 / 1] += row g of strip a / b times token 4 s + t over the 512 k of one block pair, the two halves of the groups
+// apart (.x, .y); st: the pair's stage, strip b kQBlk after strip a; x at the block's first k
 template <int S>
-DSGX_DEV void int4_pair(float (&acc)[S][2], const uint8_t* a, const uint8_t* b, XCols<S> x, int lane) {
+DSGX_DEV void int4_pair(float2 (&acc)[S][2], uint32_t st, XCols<S> x, int lane) {
   const int g = lane >> 2, h = (lane >> 1) & 1;
-  const uint32_t za = *reinterpret_cast<const uint32_t*>(a + 2304 + 8 * g + 4 * h);
-  const uint32_t zb = *reinterpret_cast<const uint32_t*>(b + 2304 + 8 * g + 4 * h);
-  const uint4 sa0 = lds128(a + 2048 + 32 * g), sa1 = lds128(a + 2048 + 32 * g + 16);  // the two halves' eight scales
-  const uint4 sb0 = lds128(b + 2048 + 32 * g), sb1 = lds128(b + 2048 + 32 * g + 16);
+  const uint32_t a = st, az = a + 2304 + 8 * g + 4 * h, as = a + 2048 + 32 * g, av = a + 16 * lane;
+  const uint32_t za = lds_u32(az), zb = lds_u32(az + kQBlk);
+  const uint4 sa0 = lds_v4(as), sa1 = lds_v4(as + 16);  // the two halves' eight scales
+  const uint4 sb0 = lds_v4(as + kQBlk), sb1 = lds_v4(as + kQBlk + 16);
   const uint32_t zae = za & 0x0F0F0F0Fu, zao = (za >> 4) & 0x0F0F0F0Fu;
   const uint32_t zbe = zb & 0x0F0F0F0Fu, zbo = (zb >> 4) & 0x0F0F0F0Fu;
   const uint32_t* a0 = &sa0.x;
@@ -73,7 +93,7 @@ DSGX_DEV void int4_pair(float (&acc)[S][2], const uint8_t* a, const uint8_t* b, 
   const uint32_t* b1 = &sb1.x;
 #pragma unroll
   for (int jj = 0; jj < 4; ++jj) {
-    const uint4 va = lds128(a + 512 * jj + 16 * lane), vb = lds128(b + 512 * jj + 16 * lane);
+    const uint4 va = lds_v4(av + 512 * jj), vb = lds_v4(av + kQBlk + 512 * jj);
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       const uint32_t zsel = 0x4040u + 0x0101u * jj;  // bytes (nibble jj, 0x43, nibble jj, 0x43): 128 + z twice
@@ -85,19 +105,21 @@ DSGX_DEV void int4_pair(float (&acc)[S][2], const uint8_t* a, const uint8_t* b, 
         wa[i] = nib_pair(al, i, zza), wa[4 + i] = nib_pair(ah, i, zza);
         wb[i] = nib_pair(bl, i, zzb), wb[4 + i] = nib_pair(bh, i, zzb);
       }
-      const float fa0 = __uint_as_float(q ? a0[jj] & 0xffff0000u : a0[jj] << 16), fa1 = __uint_as_float(q ? a1[jj] & 0xffff0000u : a1[jj] << 16);
-      const float fb0 = __uint_as_float(q ? b0[jj] & 0xffff0000u : b0[jj] << 16), fb1 = __uint_as_float(q ? b1[jj] & 0xffff0000u : b1[jj] << 16);
+      const float2 fa = q ? make_float2(__uint_as_float(a0[jj] & 0xffff0000u), __uint_as_float(a1[jj] & 0xffff0000u))
+                          : make_float2(__uint_as_float(a0[jj] << 16), __uint_as_float(a1[jj] << 16));
+      const float2 fb = q ? make_float2(__uint_as_float(b0[jj] & 0xffff0000u), __uint_as_float(b1[jj] & 0xffff0000u))
+                          : make_float2(__uint_as_float(b0[jj] << 16), __uint_as_float(b1[jj] << 16));
 #pragma unroll
       for (int s = 0; s < S; ++s) {
-        const uint4 x0 = lds128(x.p[s]), x1 = lds128(x.p[s] + 16);
+        const uint4 x0 = lds_v4(x.p[s]), x1 = lds_v4(x.p[s] + 16);
         x.p[s] += x.step[s];
         float d[4];
         mma_bf16_zero(d, wa[0], wb[0], wa[1], wb[1], x0.x, x0.y);
         mma_bf16(d, wa[2], wb[2], wa[3], wb[3], x0.z, x0.w);
         mma_bf16(d, wa[4], wb[4], wa[5], wb[5], x1.x, x1.y);
         mma_bf16(d, wa[6], wb[6], wa[7], wb[7], x1.z, x1.w);
-        acc[s][0] = fmaf(fa1, d[1], fmaf(fa0, d[0], acc[s][0]));
-        acc[s][1] = fmaf(fb1, d[3], fmaf(fb0, d[2], acc[s][1]));
+        fma2(acc[s][0], fa, make_float2(d[0], d[1]));
+        fma2(acc[s][1], fb, make_float2(d[2], d[3]));
       }
     }
   }

@@ -188,7 +188,8 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
   if (warp < W) {
     // ---- stream warps ---------------------------------------------------------------------------------------------------
     XCols<S> cols;
-    xcols_int4<S>(cols, xt, p.M, zero, lane, [&](int s, int j) { return 4 * s + j < p.M ? 4 * s + j : -1; });
+    xcols_int4<S>(cols, smem_u32(xt), p.M, smem_u32(zero), lane, [&](int s, int j) { return 4 * s + j < p.M ? 4 * s + j : -1; });
+    const uint32_t ring_at = smem_u32(myring);
     uint32_t consumed = 0;
     bool ok = true;
     for (int j = warp; j < total && ok; j += W) {
@@ -197,9 +198,9 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
       int b = p.nb * rt / kRuns;
       for (int r = 0; r < RPT && ok; ++r) {
         const int e = p.nb * (rt + r + 1) / kRuns;
-        float acc[S][2];
+        float2 acc[S][2];
 #pragma unroll
-        for (int s = 0; s < S; ++s) acc[s][0] = acc[s][1] = 0.f;
+        for (int s = 0; s < S; ++s) acc[s][0] = acc[s][1] = make_float2(0.f, 0.f);
         for (; b < e; ++b) {
           const uint32_t si = consumed % NST;
           if (!mbar_wait(mybar + si, (consumed / NST) & 1)) {
@@ -208,9 +209,8 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
           }
           XCols<S> xc = cols;
 #pragma unroll
-          for (int s = 0; s < S; ++s) xc.p[s] += (size_t)(b - b0) * 8 * xc.step[s];
-          const uint8_t* st = myring + si * kPairStage;
-          int4_pair<S>(acc, st, st + kQBlk, xc, lane);
+          for (int s = 0; s < S; ++s) xc.p[s] += (b - b0) * 8 * xc.step[s];
+          int4_pair<S>(acc, ring_at + si * kPairStage, xc, lane);
           ++consumed;
           __syncwarp();
           if (lane == 0 && open_task()) issue();
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
         const bool j0 = r & 1, j1 = (r & 3) == 3, j2 = r == 7;  // how many waiting subtrees this run completes
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-          sum[s] = make_float2(acc[s][0], acc[s][1]);
+          sum[s] = make_float2(__fadd_rn(acc[s][0].x, acc[s][0].y), __fadd_rn(acc[s][1].x, acc[s][1].y));
           if (j0) sum[s] = add2(lv[0][s], sum[s]);
           if (j1) sum[s] = add2(lv[1][s], sum[s]);
           if (j2) sum[s] = add2(lv[2][s], sum[s]);
