@@ -56,8 +56,7 @@ class LayerStep(C.Structure):
 
 
 class LinearW(C.Structure):
-    _fields_ = [("w", C.c_void_p), ("w_up", C.c_void_p), ("N", C.c_int32), ("K", C.c_int32), ("fmt", C.c_uint32),
-                ("reserved", C.c_int32)]
+    _fields_ = [("w", C.c_void_p), ("N", C.c_int32), ("K", C.c_int32), ("fmt", C.c_uint32), ("glu", C.c_int32)]
 
 
 class AddNorm(C.Structure):
@@ -84,6 +83,8 @@ SYMBOLS = {
     "dsgx_finalize": (_I, [_V, _V, _I, _I, _V, _I, _V]),
     "dsgx_moe_layer_decode": (_I, [C.POINTER(MoeShape), C.POINTER(LayerW), _V, _I, C.POINTER(LayerStep), _I, _V]),
     "dsgx_moe_layer_decode_host": (_I, [C.POINTER(MoeShape), C.POINTER(LayerW), _V, _I, C.POINTER(LayerStep), _V, _V]),
+    "dsgx_linear_bytes": (_Z, [_I, _I, _I]),
+    "dsgx_linear_prepare": (_I, [_V, _V, C.c_uint32, _I, _I, _V, _V]),
     "dsgx_linear_decode": (_I, [C.POINTER(LinearW), _V, C.c_int64, _I, _V, C.c_int64, _V, C.c_int64, _I, _V, _V]),
     "dsgx_prefill_weights_bytes": (_Z, [C.POINTER(MoeShape)]),
     "dsgx_prefill_prepare": (_I, [C.POINTER(MoeShape), C.POINTER(LayerW), _V, _V]),

@@ -407,20 +407,35 @@ int dsgx_moe_layer_decode_host(const dsgx_moe_shape* s, const dsgx_layer_w* L, c
   return e == cudaSuccess ? DSGX_OK : cuda_fail(e);
 }
 
+static bool linear_shape_ok(int N, int K) {
+  return N >= 1 && K >= 1 && N <= (1 << 30) && K <= (1 << 30) && (((size_t)N + 7) / 8) * (((size_t)K + 511) / 512) < ((size_t)1 << 31);
+}
+
+size_t dsgx_linear_bytes(int N, int K, int glu) { return linear_shape_ok(N, K) ? linear_bytes(N, K, glu != 0) : 0; }
+
+int dsgx_linear_prepare(const void* w, const void* w_up, uint32_t fmt, int N, int K, void* out, void* stream) {
+  if (!w || !out) return DSGX_ERR_ARG;
+  if (fmt != DSGX_FMT_INT4) return DSGX_ERR_FORMAT;
+  if (!linear_shape_ok(N, K)) return DSGX_ERR_SHAPE;
+  if (((uintptr_t)w | (uintptr_t)w_up | (uintptr_t)out) & 15) return DSGX_ERR_ARG;
+  cudaError_t e = launch_linear_prepare(reinterpret_cast<const uint8_t*>(w), reinterpret_cast<const uint8_t*>(w_up), N, K,
+                                        reinterpret_cast<uint8_t*>(out), (cudaStream_t)stream);
+  return e == cudaSuccess ? DSGX_OK : cuda_fail(e);
+}
+
 int dsgx_linear_decode(const dsgx_linear_w* W, const void* x, int64_t ldx, int M, const void* res, int64_t ldr, void* out,
                        int64_t ldo, int out_f32, int32_t* status_word, void* stream) {
   if (!W || !W->w || !x || !out) return DSGX_ERR_ARG;
   if (W->fmt != DSGX_FMT_INT4) return DSGX_ERR_FORMAT;
-  if (W->N < 1 || W->K < 1 || W->N > (1 << 30) || W->K > (1 << 30)) return DSGX_ERR_SHAPE;
+  if (!linear_shape_ok(W->N, W->K)) return DSGX_ERR_SHAPE;
   if (M < 1 || M > DSGX_MAX_STEP_ROWS || ldx < W->K || ldo < W->N || (res && ldr < W->N)) return DSGX_ERR_ARG;
-  if (res && W->w_up) return DSGX_ERR_UNSUPPORTED;
-  if (((uintptr_t)W->w | (uintptr_t)W->w_up) & 15 || ((uintptr_t)x | (uintptr_t)res) & 1 || (uintptr_t)out & (out_f32 ? 3 : 1) ||
-      (uintptr_t)status_word & 3)
+  if (res && W->glu) return DSGX_ERR_UNSUPPORTED;
+  if (((uintptr_t)W->w & 15) || ((uintptr_t)x | (uintptr_t)res) & 1 || (uintptr_t)out & (out_f32 ? 3 : 1) || (uintptr_t)status_word & 3)
     return DSGX_ERR_ARG;
   LinearParams p;
-  p.w = W->w, p.w_up = W->w_up, p.x = reinterpret_cast<const __nv_bfloat16*>(x), p.res = reinterpret_cast<const __nv_bfloat16*>(res);
+  p.w = W->w, p.glu = W->glu != 0, p.x = reinterpret_cast<const __nv_bfloat16*>(x), p.res = reinterpret_cast<const __nv_bfloat16*>(res);
   p.out = out, p.ldx = ldx, p.ldr = ldr, p.ldo = ldo, p.M = M, p.N = W->N, p.K = W->K;
-  p.n8 = (W->N + 7) / 8, p.nb = (W->K + 511) / 512, p.units = W->w_up ? p.n8 : (p.n8 + 1) / 2;
+  p.nb = (W->K + 511) / 512, p.units = p.glu ? (W->N + 7) / 8 : (W->N + 15) / 16;
   p.out_f32 = out_f32 != 0, p.x_vec = ((uintptr_t)x & 15) == 0 && ldx % 8 == 0;
   p.cluster = 1, p.lc = 0, p.xblocks = 0, p.lq = 0, p.status = status_word;
   bool fits = false;

@@ -80,48 +80,64 @@ DSGX_DEV void xcols_int4(XCols<S>& x, uint32_t tile, int rows, uint32_t zero, in
 // apart (.x, .y); st: the pair's stage, strip b kQBlk after strip a; x at the block's first k
 template <int S>
 DSGX_DEV void int4_pair(float2 (&acc)[S][2], uint32_t st, XCols<S> x, int lane) {
+  constexpr int QI = 1, UNR = S == 1 ? 4 : 1;
   const int g = lane >> 2, h = (lane >> 1) & 1;
-  const uint32_t a = st, az = a + 2304 + 8 * g + 4 * h, as = a + 2048 + 32 * g, av = a + 16 * lane;
+  const uint32_t az = st + 2304 + 8 * g + 4 * h;
   const uint32_t za = lds_u32(az), zb = lds_u32(az + kQBlk);
-  const uint4 sa0 = lds_v4(as), sa1 = lds_v4(as + 16);  // the two halves' eight scales
-  const uint4 sb0 = lds_v4(as + kQBlk), sb1 = lds_v4(as + kQBlk + 16);
   const uint32_t zae = za & 0x0F0F0F0Fu, zao = (za >> 4) & 0x0F0F0F0Fu;
   const uint32_t zbe = zb & 0x0F0F0F0Fu, zbo = (zb >> 4) & 0x0F0F0F0Fu;
-  const uint32_t* a0 = &sa0.x;
-  const uint32_t* a1 = &sa1.x;
-  const uint32_t* b0 = &sb0.x;
-  const uint32_t* b1 = &sb1.x;
-#pragma unroll
+  uint32_t av = st + 16 * lane, as = st + 2048 + 32 * g, zsel = 0x4040u;  // bytes (nibble jj, 0x43, nibble jj, 0x43): 128 + z twice
+#pragma unroll UNR
   for (int jj = 0; jj < 4; ++jj) {
-    const uint4 va = lds_v4(av + 512 * jj), vb = lds_v4(av + kQBlk + 512 * jj);
+    const uint4 va = lds_v4(av), vb = lds_v4(av + kQBlk);
+    const uint32_t sa0 = lds_u32(as), sa1 = lds_u32(as + 16), sb0 = lds_u32(as + kQBlk), sb1 = lds_u32(as + kQBlk + 16);
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const uint32_t zsel = 0x4040u + 0x0101u * jj;  // bytes (nibble jj, 0x43, nibble jj, 0x43): 128 + z twice
-      const uint32_t zza = __byte_perm(q ? zao : zae, 0x43434343u, zsel), zzb = __byte_perm(q ? zbo : zbe, 0x43434343u, zsel);
-      const uint32_t al = q ? va.z : va.x, ah = q ? va.w : va.y, bl = q ? vb.z : vb.x, bh = q ? vb.w : vb.y;
-      uint32_t wa[8], wb[8];
+    for (int q0 = 0; q0 < 2; q0 += QI) {
+      uint32_t wa[QI][8], wb[QI][8];
+      uint4 x0[QI][S], x1[QI][S];
+      float d[QI][S][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        wa[i] = nib_pair(al, i, zza), wa[4 + i] = nib_pair(ah, i, zza);
-        wb[i] = nib_pair(bl, i, zzb), wb[4 + i] = nib_pair(bh, i, zzb);
+      for (int c = 0; c < QI; ++c) {
+        const int q = q0 + c;
+        const uint32_t zza = __byte_perm(q ? zao : zae, 0x43434343u, zsel), zzb = __byte_perm(q ? zbo : zbe, 0x43434343u, zsel);
+        const uint32_t al = q ? va.z : va.x, ah = q ? va.w : va.y, bl = q ? vb.z : vb.x, bh = q ? vb.w : vb.y;
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+          x0[c][s] = lds_v4(x.p[s]), x1[c][s] = lds_v4(x.p[s] + 16);
+          x.p[s] += x.step[s];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          wa[c][i] = nib_pair(al, i, zza), wa[c][4 + i] = nib_pair(ah, i, zza);
+          wb[c][i] = nib_pair(bl, i, zzb), wb[c][4 + i] = nib_pair(bh, i, zzb);
+        }
       }
-      const float2 fa = q ? make_float2(__uint_as_float(a0[jj] & 0xffff0000u), __uint_as_float(a1[jj] & 0xffff0000u))
-                          : make_float2(__uint_as_float(a0[jj] << 16), __uint_as_float(a1[jj] << 16));
-      const float2 fb = q ? make_float2(__uint_as_float(b0[jj] & 0xffff0000u), __uint_as_float(b1[jj] & 0xffff0000u))
-                          : make_float2(__uint_as_float(b0[jj] << 16), __uint_as_float(b1[jj] << 16));
 #pragma unroll
-      for (int s = 0; s < S; ++s) {
-        const uint4 x0 = lds_v4(x.p[s]), x1 = lds_v4(x.p[s] + 16);
-        x.p[s] += x.step[s];
-        float d[4];
-        mma_bf16_zero(d, wa[0], wb[0], wa[1], wb[1], x0.x, x0.y);
-        mma_bf16(d, wa[2], wb[2], wa[3], wb[3], x0.z, x0.w);
-        mma_bf16(d, wa[4], wb[4], wa[5], wb[5], x1.x, x1.y);
-        mma_bf16(d, wa[6], wb[6], wa[7], wb[7], x1.z, x1.w);
-        fma2(acc[s][0], fa, make_float2(d[0], d[1]));
-        fma2(acc[s][1], fb, make_float2(d[2], d[3]));
+      for (int m = 0; m < 4; ++m)
+#pragma unroll
+        for (int c = 0; c < QI; ++c)
+#pragma unroll
+          for (int s = 0; s < S; ++s) {
+            const uint4& xv = m < 2 ? x0[c][s] : x1[c][s];
+            const uint32_t b0 = m & 1 ? xv.z : xv.x, b1 = m & 1 ? xv.w : xv.y;
+            if (m == 0) mma_bf16_zero(d[c][s], wa[c][0], wb[c][0], wa[c][1], wb[c][1], b0, b1);
+            else mma_bf16(d[c][s], wa[c][2 * m], wb[c][2 * m], wa[c][2 * m + 1], wb[c][2 * m + 1], b0, b1);
+          }
+#pragma unroll
+      for (int c = 0; c < QI; ++c) {
+        const bool q = q0 + c;
+        const float2 fa = q ? make_float2(__uint_as_float(sa0 & 0xffff0000u), __uint_as_float(sa1 & 0xffff0000u))
+                            : make_float2(__uint_as_float(sa0 << 16), __uint_as_float(sa1 << 16));
+        const float2 fb = q ? make_float2(__uint_as_float(sb0 & 0xffff0000u), __uint_as_float(sb1 & 0xffff0000u))
+                            : make_float2(__uint_as_float(sb0 << 16), __uint_as_float(sb1 << 16));
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+          fma2(acc[s][0], fa, make_float2(d[c][s][0], d[c][s][1]));
+          fma2(acc[s][1], fb, make_float2(d[c][s][2], d[c][s][3]));
+        }
       }
     }
+    av += 512, as += 4, zsel += 0x0101u;
   }
 }
 

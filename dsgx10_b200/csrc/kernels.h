@@ -149,18 +149,19 @@ cudaError_t launch_front_route(const DecodeParams& p, uint32_t fmt, const RouteP
 
 // ---- dense INT4-g32 products (linear.cu) ---------------------------------------------------------------------------------
 struct LinearParams {
-  const uint8_t* w;     // INT4 blocks [n8][nb]
-  const uint8_t* w_up;  // the second matrix (SwiGLU), or null
+  const uint8_t* w;     // the prepared matrix (or gate / up pair: glu): [units][nb] blocks of 16 rows x 512 k
   const __nv_bfloat16* x;
   const __nv_bfloat16* res;
   void* out;
   long long ldx, ldr, ldo;
-  int M, N, K, n8, nb, units;  // units of 16 output rows (SwiGLU: 8 + 8)
+  int M, N, K, nb, units, glu;  // units of 16 output rows (SwiGLU: 8 + 8)
   int out_f32, x_vec;
   // chosen by the launch: CTAs a cluster (and its logarithm), blocks of K a rank holds at most, 2^lq tasks a unit
   int cluster, lc, xblocks, lq;
   int* status;
 };
+size_t linear_bytes(int N, int K, bool glu);
+cudaError_t launch_linear_prepare(const uint8_t* w, const uint8_t* w_up, int N, int K, uint8_t* out, cudaStream_t st);
 cudaError_t launch_linear_int4(const LinearParams& p, cudaStream_t st, bool* fits);
 
 // ---- prefill (FP8) ----------------------------------------------------------------------------------------------------

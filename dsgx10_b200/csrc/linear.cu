@@ -1,12 +1,20 @@
 // Dense INT4-g32 matrix-vector products for 1..16 rows: out[m][n] = sum_k x[m][k] W[n][k], W = (u - z) s, f32 sums; the
-// residual added, or with a second matrix silu(x W^T) * (x W_up^T).  (The expert kernels' weight blocks, decode_int4.cu.)
+// residual added, or with a second matrix silu(x W^T) * (x W_up^T).
 //
 // Bound: the weights are read once (0.578 bytes a weight), so HBM; the conversion of the nibbles in registers is the next
-// limit (int4_pair.cuh).  Work is cut in units of 16 output rows (SwiGLU: 8 gate + 8 up), a unit along K in 1, 2, 4 or 8 tasks,
-// a task in pairs of 8 x 512 blocks.  A CTA owns a run of units and its stream warps take the run's tasks in turn, each
-// through a private ring of bulk copies, so that every SM streams one contiguous run and the launch ends within a task
-// on every SM.  A task's sums go to shared memory; one more warp joins the tasks of a unit and writes the outputs, so
-// that the stream never waits for a reduction.
+// limit.  Work is cut in units of 16 output rows (SwiGLU: 8 gate + 8 up), a unit along K in 1, 2, 4 or 8 tasks, a task in
+// blocks of 16 rows x 512 k.  A CTA owns a run of units and its stream warps take the run's tasks in turn, each through a
+// private ring of bulk copies (one a block), so that every SM streams one contiguous run and the launch ends within a
+// task on every SM.  A task's sums go to shared memory; one more warp joins the tasks of a unit and writes the outputs,
+// so that the stream never waits for a reduction.
+//
+// Weight layout (k_linear_prepare makes it from the experts' 8-row blocks): the blocks of a unit one after the other, 4736
+// bytes each, [8 spans of 64 k][32 lanes][four words: row g of the first strip and of the second in the span's first group of
+// 32, then both in its second], a word = the 8 nibbles k = 32 group + 8 t + 0..7 of lane 4 g + t; [4 x 128 k][8 g][eight bf16
+// scales: (strip, group) by (first span, second span)]; [8 g][4 x 128 k][the eight zero points' nibbles in that order].
+// In the experts' blocks a lane's 16 bytes mix two groups in every MMA, so their scales have to go onto the weights (and
+// round them) or the MMAs' columns be halved (int4_pair.cuh: twice the MMAs and activation loads from five rows on); here
+// an MMA stays inside one group, its f32 sums take the scale, and all eight columns are rows of x.
 //
 // K over a cluster: with C > 1 (2, 4 or 8 CTAs) the ranks of a cluster take consecutive parts of K of the same units.  The
 // activations of M rows are held in shared memory for a rank's own part only, and a matrix with few units still occupies
@@ -19,6 +27,7 @@
 #include <atomic>
 
 #include "common.cuh"
+#include "decode_common.cuh"
 #include "int4_pair.cuh"
 #include "kernels.h"
 
@@ -31,18 +40,95 @@ constexpr int kMaxCluster = 8;
 constexpr int kRuns = 8;         // the parts of K whose sums are joined as a tree
 constexpr size_t kSmemMax = 227 * 1024;
 
-// W stream warps with NST ring stages each, P tasks' sums in flight (a power of two); S sets of four tokens
+constexpr int kUnitBlk = 4736;    // 16 rows x 512 k
+
+// S sets of eight rows; W stream warps with NST ring stages each, P tasks' sums in flight (a power of two)
 template <int S_, int W_, int NST_, int P_>
 struct LinVar {
   static constexpr int S = S_, W = W_, NST = NST_, P = P_;
   static constexpr int kThreads = (W + 1) * 32;
-  static constexpr int kPart = 256 * S;  // bytes of a block pair's (or a rank's) sums: [S][32 lanes][2] f32
-  static constexpr size_t kFixed = (size_t)W * NST * kPairStage + (size_t)P * kPart + 128;
+  static constexpr int kPart = 512 * S;  // bytes of a task's (or a rank's) sums: [S][32 lanes][4] f32
   static size_t smem(int M, int kblocks, int C) {
-    return kFixed + (C > 1 ? (size_t)kSlotsOwned * kMaxCluster * kPart : 0) + (size_t)kblocks * M * 1024 + 64 +
-           (W * NST + kSlotsOwned * (1 + kMaxCluster)) * 8 + P * 4 + 64;
+    return (size_t)W * NST * kUnitBlk + (size_t)P * kPart + (C > 1 ? (size_t)kSlotsOwned * C * kPart : 0) +
+           (size_t)kblocks * M * 1024 + (W * NST + kSlotsOwned * (1 + kMaxCluster)) * 8 + P * 4 + 16 + 128;
   }
 };
+
+// acc[s] += the products of one block (a lane's four sums: first strip's row g with rows 8 s + 2 t and + 1 of x, then the
+// second strip's).  st: the stage; x[s]: this lane's activations at the block's first span; span: bytes from one to the next.
+template <int S>
+DSGX_DEV void unit_block(float (&acc)[S][4], uint32_t st, const uint32_t (&x_at)[S], uint32_t span, int lane) {
+  const int g = lane >> 2;
+  const uint4 zq = lds_v4(st + 4608 + 16 * g);
+  const uint32_t* zw = &zq.x;
+  uint32_t x[S];
+#pragma unroll
+  for (int s = 0; s < S; ++s) x[s] = x_at[s];
+#pragma unroll
+  for (int jj = 0; jj < 4; ++jj) {
+    const uint4 sc = lds_v4(st + 4096 + 128 * jj + 16 * g);
+    const uint32_t* sw = &sc.x;
+    const uint32_t ze = zw[jj] & 0x0F0F0F0Fu, zo = (zw[jj] >> 4) & 0x0F0F0F0Fu;  // first span's four, second span's four
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const uint4 w = lds_v4(st + 512 * (2 * jj + q) + 16 * lane);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {  // the span's two groups
+        const uint32_t wa = c ? w.z : w.x, wb = c ? w.w : w.y;
+        const uint32_t zza = __byte_perm(q ? zo : ze, 0x43434343u, 0x4040u + 0x0101u * (2 * c)),
+                       zzb = __byte_perm(q ? zo : ze, 0x43434343u, 0x4040u + 0x0101u * (2 * c + 1));
+        uint32_t a[4], b[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = nib_pair(wa, i, zza), b[i] = nib_pair(wb, i, zzb);
+        const float fa = __uint_as_float(q ? sw[2 * c] & 0xffff0000u : sw[2 * c] << 16);
+        const float fb = __uint_as_float(q ? sw[2 * c + 1] & 0xffff0000u : sw[2 * c + 1] << 16);
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+          const uint4 xv = lds_v4(x[s] ^ (c ? 64u : 0u));
+          float d[4];
+          mma_bf16_zero(d, a[0], b[0], a[1], b[1], xv.x, xv.y);
+          mma_bf16(d, a[2], b[2], a[3], b[3], xv.z, xv.w);
+          acc[s][0] = fmaf(fa, d[0], acc[s][0]), acc[s][1] = fmaf(fa, d[1], acc[s][1]);
+          acc[s][2] = fmaf(fb, d[2], acc[s][2]), acc[s][3] = fmaf(fb, d[3], acc[s][3]);
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < S; ++s) x[s] += span;
+    }
+  }
+}
+
+// ---- the weights' own layout, once at load ------------------------------------------------------------------------------
+// One CTA a block: strips a and b of a unit (b null: an odd number of strips, zeros) at one 512-k block.
+__global__ void __launch_bounds__(256) k_linear_prepare(const uint8_t* __restrict__ w, const uint8_t* __restrict__ w_up, int n8, int nb,
+                                                        uint8_t* __restrict__ out) {
+  const size_t blk = blockIdx.x;
+  const int u = (int)(blk / nb), b = (int)(blk % nb);
+  const size_t strip = (size_t)nb * kQBlk;
+  const uint8_t* src[2];
+  src[0] = (w_up ? w + (size_t)u * strip : w + (size_t)(2 * u) * strip) + (size_t)b * kQBlk;
+  src[1] = w_up ? w_up + (size_t)u * strip + (size_t)b * kQBlk : 2 * u + 1 < n8 ? src[0] + strip : nullptr;
+  uint8_t* o = out + blk * kUnitBlk;
+  {  // thread: span, lane; the word of (strip, group c): 8 nibbles k = 32 c + 8 t of the span
+    const int sp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    uint32_t v[4];
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int m = 0; m < 2; ++m)  // in the 8-row block: unit sp / 2, lane 4 g + 2 c + t / 2, half sp % 2, word t % 2
+        v[2 * c + m] = src[m] ? *reinterpret_cast<const uint32_t*>(src[m] + 512 * (sp >> 1) + 16 * (4 * g + 2 * c + (t >> 1)) + 8 * (sp & 1) + 4 * (t & 1)) : 0u;
+    *reinterpret_cast<uint4*>(o + 512 * sp + 16 * lane) = make_uint4(v[0], v[1], v[2], v[3]);
+  }
+  {  // thread: one scale (128-k part jj, row g, group c, strip m, span q)
+    const int jj = threadIdx.x >> 6, g = (threadIdx.x >> 3) & 7, c = (threadIdx.x >> 2) & 1, m = (threadIdx.x >> 1) & 1, q = threadIdx.x & 1;
+    reinterpret_cast<uint16_t*>(o + 4096)[threadIdx.x] =
+        src[m] ? *reinterpret_cast<const uint16_t*>(src[m] + 2048 + 32 * g + 16 * c + 2 * (2 * jj + q)) : (uint16_t)0;
+  }
+  if (threadIdx.x < 128) {  // thread: one byte of zero points (row g, part jj, group c, strip m): first span low, second high
+    const int g = threadIdx.x >> 4, jj = (threadIdx.x >> 2) & 3, c = (threadIdx.x >> 1) & 1, m = threadIdx.x & 1;
+    o[4608 + threadIdx.x] = src[m] ? src[m][2304 + 8 * g + 4 * c + jj] : (uint8_t)0;
+  }
+}
 
 DSGX_DEV uint32_t cluster_rank() {
   uint32_t r;
@@ -60,8 +146,8 @@ DSGX_DEV void cluster_sync_all() {
 DSGX_DEV void remote_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-DSGX_DEV void st_remote(uint32_t addr, float2 v) {
-  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(addr), "f"(v.x), "f"(v.y) : "memory");
+DSGX_DEV void st_remote(uint32_t addr, float4 v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
 // bounded wait with the cluster's scope (the barrier's arrivals come from other CTAs)
 DSGX_DEV bool mbar_wait_cluster(uint64_t* bar, uint32_t parity) {
@@ -79,7 +165,9 @@ DSGX_DEV bool mbar_wait_cluster(uint64_t* bar, uint32_t parity) {
     if (clock64() - t0 > kWaitCycles) return false;
   }
 }
-DSGX_DEV float2 add2(float2 a, float2 b) { return make_float2(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y)); }
+DSGX_DEV float4 add4(float4 a, float4 b) {
+  return make_float4(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y), __fadd_rn(a.z, b.z), __fadd_rn(a.w, b.w));
+}
 DSGX_DEV int ld_shared_acquire(const int* p) {
   int v;
   asm volatile("ld.acquire.cta.shared::cta.s32 %0, [%1];" : "=r"(v) : "r"(smem_u32(p)) : "memory");
@@ -102,11 +190,10 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
   const int b0 = p.nb * (int)rank / C, nbk = p.nb * ((int)rank + 1) / C - b0;
 
   uint8_t* ring = smem;
-  uint8_t* part = ring + (size_t)W * NST * kPairStage;                 // [P][S][32][2] f32
-  uint8_t* recv = part + (size_t)P * kPart;                            // [kSlotsOwned][C][S][32][2] f32
-  uint8_t* xt = recv + (C > 1 ? (size_t)kSlotsOwned * kMaxCluster * kPart : 0);
-  uint8_t* zero = xt + (size_t)p.xblocks * p.M * 1024 + 16;             // 32 bytes
-  uint64_t* bars = reinterpret_cast<uint64_t*>(zero + 48);
+  uint8_t* part = ring + (size_t)W * NST * kUnitBlk;                   // [P][S][32][4] f32
+  uint8_t* recv = part + (size_t)P * kPart;                            // [kSlotsOwned][C][S][32][4] f32
+  uint8_t* xt = recv + (C > 1 ? (size_t)kSlotsOwned * C * kPart : 0);  // [spans][M rows][128 B]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(xt + (size_t)p.xblocks * p.M * 1024);
   uint64_t* rfull = bars + W * NST;                                    // [kSlotsOwned] every rank's sums are in my buffer
   uint64_t* rfree = rfull + kSlotsOwned;                               // [owner][kSlotsOwned] that owner's buffer may be written
   int* cnt = reinterpret_cast<int*>(rfree + kMaxCluster * kSlotsOwned);  // [P] block pairs summed of a unit in flight
@@ -121,7 +208,6 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
     *done = 0, *fail = 0;
   }
   for (int i = threadIdx.x; i < P; i += V::kThreads) cnt[i] = 0;
-  if (threadIdx.x < 8) reinterpret_cast<uint32_t*>(zero)[threadIdx.x] = 0;
   mbar_fence_init();
   __syncwarp();
   if (C > 1) cluster_sync_all();
@@ -131,40 +217,29 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
   const int lq = p.lq, Q = 1 << lq, RPT = (kRuns / C) >> lq;  // tasks a unit (this rank's part), runs a task
   const int total = (u1 - u0) << lq;                          // this CTA's tasks
   const int r0 = (int)rank * (kRuns / C);                     // this rank's first run
-  const size_t strip = (size_t)p.nb * kQBlk;
-  const bool glu = p.w_up != nullptr;
+  const bool glu = p.glu != 0;
 
   // ---- the first weights are requested before the activations are there (they do not depend on the launches before) ------
-  uint8_t* myring = ring + (size_t)warp * NST * kPairStage;
+  uint8_t* myring = ring + (size_t)warp * NST * kUnitBlk;
   uint64_t* mybar = bars + warp * NST;
   uint32_t issued = 0;
   int pj = warp, pb = 0, pe = 0;  // the producer's task and its next and last block
-  const uint8_t *pa = nullptr, *pc = nullptr;
+  const uint8_t* pa = nullptr;
   const uint64_t pol = policy_evict_first();
   auto open_task = [&]() {  // the next task with a block in it (K shorter than eight blocks: some runs are empty)
     while (pb == pe && pj < total) {
       const int u = u0 + (pj >> lq), r = r0 + (pj & (Q - 1)) * RPT;
       pb = p.nb * r / kRuns, pe = p.nb * (r + RPT) / kRuns;
-      if (pb == pe) {
-        pj += W;
-        continue;
-      }
-      if (glu) {
-        pa = p.w + (size_t)u * strip, pc = p.w_up + (size_t)u * strip;
-      } else {
-        pa = p.w + (size_t)(2 * u) * strip;
-        pc = 2 * u + 1 < p.n8 ? pa + strip : pa;  // (an odd number of strips: the last unit's second half is not written)
-      }
+      if (pb == pe) pj += W;
+      else pa = p.w + ((size_t)u * p.nb + pb) * kUnitBlk;
     }
     return pj < total;
   };
   auto issue = [&]() {
-    uint8_t* st = myring + (issued % NST) * kPairStage;
-    uint64_t* bar = mybar + issued % NST;
-    mbar_expect_tx(bar, kPairBytes);
-    bulk_g2s_hint(st, pa + (size_t)pb * kQBlk, kQBlk, bar, pol);
-    bulk_g2s_hint(st + kQBlk, pc + (size_t)pb * kQBlk, kQBlk, bar, pol);
-    ++issued;
+    const uint32_t slot = issued % NST;
+    mbar_expect_tx(mybar + slot, kUnitBlk);
+    bulk_g2s_hint(myring + slot * kUnitBlk, pa, kUnitBlk, mybar + slot, pol);
+    ++issued, pa += kUnitBlk;
     if (++pb == pe) pj += W;
   };
   if (warp < W && lane == 0)
@@ -173,58 +248,81 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
   // ---- this rank's activations ------------------------------------------------------------------------------------------
   pdl_wait();
   {
+    // tile: [span of 64 k][row][the span's 8 pieces of 8 bf16], a piece = the k a lane's word covers, in the words' nibble
+    // order; odd rows with the span's two groups exchanged, so that two rows' reads of one group do not meet in the banks
     const bool vec = p.x_vec != 0;
-    const int n = nbk * 32;
-    for (int r = 0; r < p.M; ++r)
-      for (int kg = threadIdx.x; kg < n; kg += V::kThreads) {
-        uint4 o[2];
-        tile_group(o, p.x + (size_t)r * p.ldx, b0 * 512 + 16 * kg, p.K, vec);
-        uint4* d = reinterpret_cast<uint4*>(xt + ((size_t)((kg >> 2) * p.M + r) * 4 + (kg & 3)) * 32);
-        d[0] = o[0], d[1] = o[1];
-      }
+    const int n = nbk * 32;  // groups of 16 a row
+    for (int i = threadIdx.x; i < n * p.M; i += V::kThreads) {
+      const int r = i / n, kg = i - r * n;
+      uint4 o[2];
+      tile_group(o, p.x + (size_t)r * p.ldx, b0 * 512 + 16 * kg, p.K, vec);
+      uint4* d = reinterpret_cast<uint4*>(xt + (size_t)((kg >> 2) * p.M + r) * 128 + (((kg & 3) * 32) ^ ((r & 1) * 64)));
+      d[0] = o[0], d[1] = o[1];
+    }
   }
   __syncthreads();
 
   if (warp < W) {
     // ---- stream warps ---------------------------------------------------------------------------------------------------
-    XCols<S> cols;
-    xcols_int4<S>(cols, smem_u32(xt), p.M, smem_u32(zero), lane, [&](int s, int j) { return 4 * s + j < p.M ? 4 * s + j : -1; });
-    const uint32_t ring_at = smem_u32(myring);
+    const int g = lane >> 2, t = lane & 3;
+    const uint32_t span = p.M * 128, ring_at = smem_u32(myring);
+    uint32_t xl[S];  // row 8 s + g of the tile (columns without a row: the last row, their sums are not used)
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const int r = min(8 * s + g, p.M - 1);
+      xl[s] = smem_u32(xt) + r * 128 + ((t * 16) ^ ((r & 1) * 64));
+    }
     uint32_t consumed = 0;
     bool ok = true;
     for (int j = warp; j < total && ok; j += W) {
       const int rt = r0 + (j & (Q - 1)) * RPT;
-      float2 sum[S], lv[3][S];  // the run or subtree just finished; the subtrees that wait for their right halves
-      int b = p.nb * rt / kRuns;
-      for (int r = 0; r < RPT && ok; ++r) {
-        const int e = p.nb * (rt + r + 1) / kRuns;
-        float2 acc[S][2];
+      float acc[S][4], lv[3][S][4];  // the run's sums; the subtrees that wait for their right halves
+      int b = p.nb * rt / kRuns, r = 0;
+      uint32_t xb[S];
 #pragma unroll
-        for (int s = 0; s < S; ++s) acc[s][0] = acc[s][1] = make_float2(0.f, 0.f);
+      for (int s = 0; s < S; ++s) xb[s] = xl[s] + (b - b0) * 8 * span;
+      for (; r < RPT; ++r) {
+        const int e = p.nb * (rt + r + 1) / kRuns;
+#pragma unroll
+        for (int s = 0; s < S; ++s) acc[s][0] = acc[s][1] = acc[s][2] = acc[s][3] = 0.f;
         for (; b < e; ++b) {
           const uint32_t si = consumed % NST;
           if (!mbar_wait(mybar + si, (consumed / NST) & 1)) {
             ok = false;
             break;
           }
-          XCols<S> xc = cols;
+          unit_block<S>(acc, ring_at + si * kUnitBlk, xb, span, lane);
 #pragma unroll
-          for (int s = 0; s < S; ++s) xc.p[s] += (b - b0) * 8 * xc.step[s];
-          int4_pair<S>(acc, ring_at + si * kPairStage, xc, lane);
+          for (int s = 0; s < S; ++s) xb[s] += 8 * span;
           ++consumed;
           __syncwarp();
           if (lane == 0 && open_task()) issue();
         }
-        const bool j0 = r & 1, j1 = (r & 3) == 3, j2 = r == 7;  // how many waiting subtrees this run completes
+        if (!ok) break;
+        // run r closes as many waiting subtrees as it has trailing ones
+        auto fold = [&](float (&l)[S][4]) {
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-          sum[s] = make_float2(__fadd_rn(acc[s][0].x, acc[s][0].y), __fadd_rn(acc[s][1].x, acc[s][1].y));
-          if (j0) sum[s] = add2(lv[0][s], sum[s]);
-          if (j1) sum[s] = add2(lv[1][s], sum[s]);
-          if (j2) sum[s] = add2(lv[2][s], sum[s]);
-          if (!j0) lv[0][s] = sum[s];
-          else if (!j1) lv[1][s] = sum[s];
-          else if (!j2) lv[2][s] = sum[s];
+          for (int s = 0; s < S; ++s)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[s][c] = __fadd_rn(l[s][c], acc[s][c]);
+        };
+        auto keep = [&](float (&l)[S][4]) {
+#pragma unroll
+          for (int s = 0; s < S; ++s)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) l[s][c] = acc[s][c];
+        };
+        if (r + 1 == RPT || (r & 1)) {
+          if (r & 1) fold(lv[0]);
+          if ((r & 3) == 3) {
+            fold(lv[1]);
+            if (r == 7) fold(lv[2]);
+            else keep(lv[2]);
+          } else {
+            keep(lv[1]);
+          }
+        } else {
+          keep(lv[0]);
         }
       }
       // the sums into the partial buffer, once the unit that had the place has been added up
@@ -236,9 +334,9 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
         }
       }
       if (!ok) break;
-      float2* d = reinterpret_cast<float2*>(part + (size_t)(j & (P - 1)) * kPart) + lane;
+      float4* d = reinterpret_cast<float4*>(part + (size_t)(j & (P - 1)) * kPart) + lane;
 #pragma unroll
-      for (int s = 0; s < S; ++s) d[32 * s] = sum[s];
+      for (int s = 0; s < S; ++s) d[32 * s] = make_float4(acc[s][0], acc[s][1], acc[s][2], acc[s][3]);
       __threadfence_block();
       __syncwarp();
       if (lane == 0) atomicAdd(cnt + ((j >> lq) & (P - 1)), 1);
@@ -250,38 +348,37 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
     // ---- the adding warp ------------------------------------------------------------------------------------------------
     const int g = lane >> 2, t = lane & 3, n = u1 - u0, lc = p.lc;
     const int lag = C > 1 ? C * (kSlotsOwned / 2) : 0;  // an owner joins the ranks' sums this many units later
-    float2 a[S];
-    auto join = [&](const float2* d, int stride, int parts) {  // parts sums (1, 2, 4 or 8), as a tree
-      auto two = [&](int i, int s) { return add2(d[i * stride + 32 * s], d[(i + 1) * stride + 32 * s]); };
+    float4 a[S];
+    auto join = [&](const float4* d, int parts) {  // parts sums (1, 2, 4 or 8), as a tree
+      auto two = [&](int i, int s) { return add4(d[i * (kPart / 16) + 32 * s], d[(i + 1) * (kPart / 16) + 32 * s]); };
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         if (parts == 1) a[s] = d[32 * s];
         else if (parts == 2) a[s] = two(0, s);
-        else if (parts == 4) a[s] = add2(two(0, s), two(2, s));
-        else a[s] = add2(add2(two(0, s), two(2, s)), add2(two(4, s), two(6, s)));
+        else if (parts == 4) a[s] = add4(two(0, s), two(2, s));
+        else a[s] = add4(add4(two(0, s), two(2, s)), add4(two(4, s), two(6, s)));
       }
+    };
+    auto put = [&](int m, int c, float y) {
+      if (p.out_f32) reinterpret_cast<float*>(p.out)[(size_t)m * p.ldo + c] = y;
+      else reinterpret_cast<__nv_bfloat16*>(p.out)[(size_t)m * p.ldo + c] = __float2bfloat16_rn(y);
     };
     auto write = [&](int unit) {
 #pragma unroll
       for (int s = 0; s < S; ++s) {
-        const int m = 4 * s + t;
-        if (m >= p.M) continue;
-        if (glu) {
-          const int c = 8 * unit + g;
-          if (c < p.N) {
-            const float h = __fmul_rn(silu(a[s].x), a[s].y);
-            if (p.out_f32) reinterpret_cast<float*>(p.out)[(size_t)m * p.ldo + c] = h;
-            else reinterpret_cast<__nv_bfloat16*>(p.out)[(size_t)m * p.ldo + c] = __float2bfloat16_rn(h);
-          }
-        } else {
+        const float v[4] = {a[s].x, a[s].y, a[s].z, a[s].w};
 #pragma unroll
-          for (int hi = 0; hi < 2; ++hi) {
-            const int c = 16 * unit + 8 * hi + g;
-            if (c < p.N) {
-              float y = hi ? a[s].y : a[s].x;
-              if (p.res) y = __fadd_rn(y, __bfloat162float(p.res[(size_t)m * p.ldr + c]));
-              if (p.out_f32) reinterpret_cast<float*>(p.out)[(size_t)m * p.ldo + c] = y;
-              else reinterpret_cast<__nv_bfloat16*>(p.out)[(size_t)m * p.ldo + c] = __float2bfloat16_rn(y);
+        for (int e = 0; e < 2; ++e) {
+          const int m = 8 * s + 2 * t + e;
+          if (m >= p.M) continue;
+          if (glu) {
+            const int c = 8 * unit + g;
+            if (c < p.N) put(m, c, __fmul_rn(silu(v[e]), v[2 + e]));
+          } else {
+#pragma unroll
+            for (int hi = 0; hi < 2; ++hi) {
+              const int c = 16 * unit + 8 * hi + g;
+              if (c < p.N) put(m, c, p.res ? __fadd_rn(v[2 * hi + e], __bfloat162float(p.res[(size_t)m * p.ldr + c])) : v[2 * hi + e]);
             }
           }
         }
@@ -299,7 +396,7 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
           }
           if (!ok) break;
         }
-        join(reinterpret_cast<const float2*>(part + (size_t)((i << lq) & (P - 1)) * kPart) + lane, kPart / 8, Q);
+        join(reinterpret_cast<const float4*>(part + (size_t)((i << lq) & (P - 1)) * kPart) + lane, Q);
         __syncwarp();
         if (lane == 0) {
           *c = 0;
@@ -313,9 +410,9 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
             ok = false;
             break;
           }
-          const uint32_t to = map_rank(smem_u32(recv) + (uint32_t)((slot * kMaxCluster + (int)rank) * kPart + lane * 8), owner);
+          const uint32_t to = map_rank(smem_u32(recv) + (uint32_t)((slot * C + (int)rank) * kPart + lane * 16), owner);
 #pragma unroll
-          for (int s = 0; s < S; ++s) st_remote(to + 256 * s, a[s]);
+          for (int s = 0; s < S; ++s) st_remote(to + 512 * s, a[s]);
           remote_arrive(map_rank(smem_u32(rfull + slot), owner));
         }
       }
@@ -326,7 +423,7 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
           ok = false;
           break;
         }
-        join(reinterpret_cast<const float2*>(recv + (size_t)slot * kMaxCluster * kPart) + lane, kPart / 8, C);
+        join(reinterpret_cast<const float4*>(recv + (size_t)slot * C * kPart) + lane, C);
         __syncwarp();
         if (lane < C) remote_arrive(map_rank(smem_u32(rfree + rank * kSlotsOwned + slot), lane));
         write(u0 + o);
@@ -417,9 +514,17 @@ cudaError_t launch(LinearParams p, cudaStream_t st, bool* fits) {
 
 // One launch for M rows, or *fits = false where their activations do not fit shared memory.
 cudaError_t launch_linear_int4(const LinearParams& p, cudaStream_t st, bool* fits) {
-  if (p.M <= 4) return launch<LinVar<1, 15, 2, 64>>(p, st, fits);
-  if (p.M <= 8) return launch<LinVar<2, 15, 2, 32>>(p, st, fits);
-  return launch<LinVar<4, 11, 2, 16>>(p, st, fits);
+  if (p.M <= 8) return launch<LinVar<1, 15, 2, 32>>(p, st, fits);
+  return launch<LinVar<2, 15, 2, 16>>(p, st, fits);
+}
+
+size_t linear_bytes(int N, int K, bool glu) {
+  const size_t n8 = ((size_t)N + 7) / 8, nb = ((size_t)K + 511) / 512;
+  return (glu ? n8 : (n8 + 1) / 2) * nb * kUnitBlk;
+}
+cudaError_t launch_linear_prepare(const uint8_t* w, const uint8_t* w_up, int N, int K, uint8_t* out, cudaStream_t st) {
+  const int n8 = (N + 7) / 8, nb = (K + 511) / 512;
+  return launch_k(k_linear_prepare, dim3((unsigned)((w_up ? n8 : (n8 + 1) / 2) * (long long)nb)), dim3(256), 0, st, false, w, w_up, n8, nb, out);
 }
 
 }  // namespace dsgx

@@ -17,7 +17,8 @@ from ._lib import check, lib
 
 
 class LinearW:
-    """An INT4-g32 matrix [N][K] in blocks of 8 rows x 512 k on the device (weights.pack_linear_int4), or a gate / up pair."""
+    """An INT4-g32 matrix [N][K], or a gate / up pair, prepared for linear_decode from the experts' blocks of 8 rows x 512 k on
+    the device (weights.pack_linear_int4).  The prepared copy is made once, on the current stream; the blocks are not kept."""
 
     def __init__(self, N, K, blocks, up=None):
         if N < 1 or K < 1:
@@ -28,8 +29,12 @@ class LinearW:
                 raise ValueError(f"LinearW: {need} contiguous bytes on the device are wanted for [{N}][{K}], got {b.numel()} of {b.dtype} on {b.device}")
         if up is not None and up.device != blocks.device:
             raise ValueError("LinearW: the two matrices are on different devices")
-        self.N, self.K, self.blocks, self.up = N, K, blocks, up
-        self.c = _lib.LinearW(blocks.data_ptr(), None if up is None else up.data_ptr(), N, K, _lib.FMT_INT4, 0)
+        self.N, self.K, self.glu, self.device = N, K, up is not None, blocks.device
+        with torch.cuda.device(self.device):
+            self.data = torch.empty(lib().dsgx_linear_bytes(N, K, int(self.glu)), dtype=torch.uint8, device=self.device)
+            check(lib().dsgx_linear_prepare(blocks.data_ptr(), up.data_ptr() if self.glu else None, _lib.FMT_INT4, N, K, self.data.data_ptr(),
+                                            torch.cuda.current_stream(self.device).cuda_stream), "dsgx_linear_prepare")
+        self.c = _lib.LinearW(self.data.data_ptr(), N, K, _lib.FMT_INT4, int(self.glu))
 
 
 def _rows(t, M, width, what, dtypes, device):
@@ -46,7 +51,7 @@ def linear_decode(w, x, res=None, out=None, out_dtype=torch.bfloat16, status=Non
     status: an int32 device tensor that gets DSGX_ERR_DEVICE_WAIT where a bounded wait ran out."""
     if x.dim() != 2:
         raise ValueError(f"linear_decode: x has shape {tuple(x.shape)}")
-    M, dev = x.shape[0], w.blocks.device
+    M, dev = x.shape[0], w.device
     if not 1 <= M <= _lib.MAX_STEP_ROWS:
         raise ValueError(f"linear_decode: {M} rows; 1..{_lib.MAX_STEP_ROWS} are taken")
     ldx = _rows(x, M, w.K, "x", (torch.bfloat16,), dev)

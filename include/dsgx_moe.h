@@ -310,27 +310,34 @@ int dsgx_moe_layer_decode_host(const dsgx_moe_shape* shape, const dsgx_layer_w* 
                                const dsgx_layer_step* step, void* out_host, void* stream);
 
 /* ---- dense products with 4-bit weights (1..DSGX_MAX_STEP_ROWS rows) ---------------------------------------------------
- * out[m][n] = sum_k x[m][k] W[n][k], W[n][k] = (u - z) s of an INT4-g32 matrix (DSGX_FMT_INT4's blocks of 8 rows x 512 k,
- * [ceil(N / 8)][ceil(K / 512)], made by dsgx10_b200/weights.py pack_linear_int4): the projections, dense FFN layers and heads
- * of a model whose experts this library runs; stands in for the engines' weight-streaming GEMV over INT4 weights
- * (altar1 engine/attn/attn.h glm::gemv).  W is not rounded: the scale is applied to a group's f32 sum (the expert kernels'
- * contract rounds every weight to bf16).  N and K are any numbers >= 1: rows past N in the last block are not written,
- * columns past K are taken as zero activations (their scales must be finite).
- *   w_up set: two matrices of one shape, out = silu(x W^T) * (x W_up^T) (a dense layer's gate and up in one launch).
- *   res set (not with w_up): res[m][n] (bf16) is added to the f32 sum; out may be res.
+ * out[m][n] = sum_k x[m][k] W[n][k], W[n][k] = (u - z) s of an INT4-g32 matrix: the projections, dense FFN layers and heads of
+ * a model whose experts this library runs; stands in for the engines' weight-streaming GEMV over INT4 weights (altar1
+ * engine/attn/attn.h glm::gemv).  W is not rounded: the scale is applied to a group's f32 sum (the expert kernels' contract
+ * rounds every weight to bf16).
+ *
+ * dsgx_linear_prepare re-tiles a matrix once at load, from the experts' blocks (DSGX_FMT_INT4: 8 rows x 512 k,
+ * [ceil(N / 8)][ceil(K / 512)], made by dsgx10_b200/weights.py pack_linear_int4 for any N and K >= 1) into the order the
+ * product's MMAs want: dsgx_linear_bytes(N, K, glu) bytes at out, 0 for sizes beyond the limits.  w_up not null (glu): two
+ * matrices of one shape, gate and up, in one.  One small kernel, nothing allocated; w and w_up may be released after it.
+ * What the packer fills rows and columns up with is never seen: rows past N are not written, and columns past K meet
+ * zero activations (their scales must be finite). */
+size_t dsgx_linear_bytes(int N, int K, int glu);
+int dsgx_linear_prepare(const void* w, const void* w_up, uint32_t fmt, int N, int K, void* out, void* stream);
+
+/* The product.  glu: out = silu(x W^T) * (x W_up^T) (a dense layer's gate and up in one launch), one rounding.
+ * res set (not with glu): res[m][n] (bf16) is added to the f32 sum; out may be res.
  * x bf16 [M][ldx], res bf16 [M][ldr], out [M][ldo] bf16, or f32 with out_f32; leading dimensions in elements, any values >= K
- * or N, rows need no alignment beyond their type's (16-byte aligned rows of x are read faster); w, w_up 16-byte aligned.
- * out must not overlap x or the weights.  One rounding, at the end.  A row's bits depend neither on the other rows of the
- * call nor on their number, and are the same run after run.  No workspace; asynchronous, graph capturable; calls on several streams may
- * overlap.  The weights must be complete before the launch in front of this one in the stream ends (they are requested
- * early: programmatic dependent launch).  status_word (device, may be null): gets DSGX_ERR_DEVICE_WAIT where a bounded wait
- * ran out.  DSGX_ERR_SHAPE: K too long for one row's activations in shared memory (beyond 180,000). */
+ * or N, rows need no alignment beyond their type's (16-byte aligned rows of x are read faster).  out must not overlap x
+ * or the weights.  A row's bits depend neither on the other rows of the call nor on their number, and are the same run
+ * after run.  No workspace; asynchronous, graph capturable; calls on several streams may overlap.  The weights must be
+ * complete before the launch in front of this one in the stream starts (they are requested early: programmatic dependent
+ * launch).  status_word (device, may be null) gets DSGX_ERR_DEVICE_WAIT where a bounded wait ran out.
+ * DSGX_ERR_SHAPE: K too long for one row's activations in the shared memory of eight CTAs (K up to 260,000 fits). */
 typedef struct dsgx_linear_w {
-  const uint8_t* w;
-  const uint8_t* w_up;
+  const uint8_t* w; /* from dsgx_linear_prepare */
   int32_t N, K;
-  uint32_t fmt; /* DSGX_FMT_INT4 */
-  int32_t reserved;
+  uint32_t fmt;     /* DSGX_FMT_INT4 */
+  int32_t glu;      /* 1: a gate / up pair of [N][K] each */
 } dsgx_linear_w;
 int dsgx_linear_decode(const dsgx_linear_w* W, const void* x_bf16, int64_t ldx, int M, const void* res_bf16, int64_t ldr,
                        void* out, int64_t ldo, int out_f32, int32_t* status_word, void* stream);

@@ -1,9 +1,9 @@
 """The dense INT4 products (dsgx_linear_decode) against the formula in 64 bits.
 
-Tolerance, by arithmetic.  A product x (u - z) has at most 8 + 4 significant bits: exact in f32.  A group's sum is four MMAs of 16
-products, each adding with at most one truncation (2^-23 of the running magnitude) a product and one for its accumulator: 68;
-two fused multiply-adds 64 k (16 in a block of 512) and the sums of the blocks and runs (at most nb / 8 + 1 + 3) round by
-2^-24 each.  So |y - exact| <= GAMMA A with A = sum |x| |W| and GAMMA = (68 + 8 + nb / 16 + 2) 2^-23 < (80 + nb) 2^-23; the one
+Tolerance, by arithmetic.  A product x (u - z) has at most 8 + 4 significant bits: exact in f32.  A group's sum is two MMAs of 16
+products, each adding with at most one truncation (2^-23 of the running magnitude) a product and one for its accumulator: 34;
+a fused multiply-add a group (16 in a block of 512, 2 nb in a run's nb / 8 blocks) and the runs' three levels round by 2^-24
+each.  So |y - exact| <= GAMMA A with A = sum |x| |W| and GAMMA = (34 + 8 + nb + 2) 2^-23 < (80 + nb) 2^-23; the one
 rounding of the output adds 2^-8 |y| (bf16) or 2^-24 |y| (f32)."""
 import numpy as np
 import pytest
@@ -135,8 +135,8 @@ def test_streams_and_graph():
     of the eager calls."""
     from dsgx10_b200 import linear
     H, I, M = 1024, 1536, 2
-    gate, up, down = (linear.LinearW(n, k, _make(n, k, 60 + i)[0]) for i, (n, k) in enumerate(((I, H), (I, H), (H, I))))
-    gu = linear.LinearW(I, H, gate.blocks, up=up.blocks)
+    gate, up, down = (_make(n, k, 60 + i)[0] for i, (n, k) in enumerate(((I, H), (I, H), (H, I))))
+    gu, down = linear.LinearW(I, H, gate, up=up), linear.LinearW(H, I, down)
 
     def layer(x, out=None):
         return linear.linear_decode(down, linear.linear_decode(gu, x), res=x, out=out)

@@ -32,16 +32,21 @@ def test_refused_calls():
     L = _lib.lib()
     one = 1 << 20   # (an aligned address that nothing reads)
 
-    def call(w=one, up=None, N=64, K=512, fmt=_lib.FMT_INT4, x=one, ldx=512, M=1, res=None, ldr=64, out=one, ldo=64, f32=0, status=None):
-        W = _lib.LinearW(w, up, N, K, fmt, 0)
+    def call(w=one, N=64, K=512, fmt=_lib.FMT_INT4, glu=0, x=one, ldx=512, M=1, res=None, ldr=64, out=one, ldo=64, f32=0, status=None):
+        W = _lib.LinearW(w, N, K, fmt, glu)
         return L.dsgx_linear_decode(C.byref(W), x, ldx, M, res, ldr, out, ldo, f32, status, None)
 
     assert L.dsgx_linear_decode(None, one, 512, 1, None, 0, one, 64, 0, None, None) == _lib.ERR_ARG
     for kw in (dict(w=None), dict(x=None), dict(out=None), dict(M=0), dict(M=17), dict(ldx=511), dict(ldo=63), dict(res=one, ldr=63),
-               dict(w=one + 8), dict(up=one + 4), dict(x=one + 1), dict(out=one + 1), dict(out=one + 2, f32=1), dict(res=one + 1), dict(status=one + 2)):
+               dict(w=one + 8), dict(x=one + 1), dict(out=one + 1), dict(out=one + 2, f32=1), dict(res=one + 1), dict(status=one + 2)):
         assert call(**kw) == _lib.ERR_ARG, kw
     for fmt in (_lib.FMT_NVFP4, _lib.FMT_RETIRED, _lib.FMT_BF16, _lib.FMT_FP8, _lib.FMT_MXFP4, 77):
         assert call(fmt=fmt) == _lib.ERR_FORMAT
-    for kw in (dict(N=0), dict(K=0), dict(N=-5), dict(K=(1 << 30) + 1, ldx=1 << 31)):
-        assert call(**kw) == _lib.ERR_SHAPE, kw
-    assert call(up=one, res=one) == _lib.ERR_UNSUPPORTED
+        assert L.dsgx_linear_prepare(one, None, fmt, 64, 512, one, None) == _lib.ERR_FORMAT
+    for N, K in ((0, 512), (64, 0), (-5, 512), (64, (1 << 30) + 1), (1 << 29, 1 << 20)):
+        assert call(N=N, K=K, ldx=1 << 31, ldo=1 << 31) == _lib.ERR_SHAPE, (N, K)
+        assert L.dsgx_linear_bytes(N, K, 0) == 0 and L.dsgx_linear_prepare(one, None, _lib.FMT_INT4, N, K, one, None) == _lib.ERR_SHAPE
+    assert call(glu=1, res=one) == _lib.ERR_UNSUPPORTED
+    for a in ((None, None, one), (one, None, None), (one + 8, None, one), (one, one + 4, one), (one, None, one + 2)):
+        assert L.dsgx_linear_prepare(a[0], a[1], _lib.FMT_INT4, 64, 512, a[2], None) == _lib.ERR_ARG
+    assert L.dsgx_linear_bytes(17, 513, 0) == 2 * 2 * 4736 and L.dsgx_linear_bytes(17, 513, 1) == 3 * 2 * 4736
