@@ -8,9 +8,17 @@
 // task on every SM.  A task's sums go to shared memory; one more warp joins the tasks of a unit and writes the outputs,
 // so that the stream never waits for a reduction.
 //
+// The conversion that is left: a nibble n in the low byte of a half-word is, as it stands, the f16 subnormal n 2^-24 (bits 0-3)
+// or n 2^-20 (bits 4-7), and the MMA takes subnormals exactly, so a word of eight weights costs four ANDs and one shift and no
+// arithmetic at all.  x goes to f16 for that: per row and block of 512 k a power of two 2^E brings the largest magnitude into
+// [2^14, 2^15), where bf16's eight bits are exact down to 2^-32 of it (smaller values round at 2^-40 of the largest, far below
+// an f32 sum's last bit); values that meet a nibble in bits 4-7 are taken times 2^-4.  The zero point leaves the sum in f32:
+// sum (n - z) x = sum n x - z sum x, the second sum of a group once a row.  Whatever is infinite or NaN in a row makes the
+// whole row NaN.
+//
 // Weight layout (k_linear_prepare makes it from the experts' 8-row blocks): the blocks of a unit one after the other, 4736
 // bytes each, [8 spans of 64 k][32 lanes][four words: row g of the first strip and of the second in the span's first group of
-// 32, then both in its second], a word = the 8 nibbles k = 32 group + 8 t + 0..7 of lane 4 g + t; [4 x 128 k][8 g][eight bf16
+// 32, then both in its second], a word = the 8 nibbles k = 32 group + 8 t + 0..7 of lane 4 g + t (nibbles i and i + 4 meet in one f16 pair); [4 x 128 k][8 g][eight bf16
 // scales: (strip, group) by (first span, second span)]; [8 g][4 x 128 k][the eight zero points' nibbles in that order].
 // In the experts' blocks a lane's 16 bytes mix two groups in every MMA, so their scales have to go onto the weights (and
 // round them) or the MMAs' columns be halved (int4_pair.cuh: twice the MMAs and activation loads from five rows on); here
@@ -25,6 +33,7 @@
 // is summed in ascending order from zero, and the runs are joined as a binary tree, ((r0 + r1) + (r2 + r3)) + ((r4 + r5) + (r6 +
 // r7)), of which a task and a rank hold whole subtrees.  So a row's bits do not depend on the rows beside it or their number.
 #include <atomic>
+#include <cuda_fp16.h>
 
 #include "common.cuh"
 #include "decode_common.cuh"
@@ -50,20 +59,39 @@ struct LinVar {
   static constexpr int kPart = 512 * S;  // bytes of a task's (or a rank's) sums: [S][32 lanes][4] f32
   static size_t smem(int M, int kblocks, int C) {
     return (size_t)W * NST * kUnitBlk + (size_t)P * kPart + (C > 1 ? (size_t)kSlotsOwned * C * kPart : 0) +
-           (size_t)kblocks * M * 1024 + (W * NST + kSlotsOwned * (1 + kMaxCluster)) * 8 + P * 4 + 16 + 128;
+           (size_t)kblocks * (M * 1024 + even(M) * 68) + (W * NST + kSlotsOwned * (1 + kMaxCluster)) * 8 + P * 4 + 16 + 128;
   }
+  __host__ __device__ static int even(int M) { return (M + 1) & ~1; }
 };
 
-// acc[s] += the products of one block (a lane's four sums: first strip's row g with rows 8 s + 2 t and + 1 of x, then the
-// second strip's).  st: the stage; x[s]: this lane's activations at the block's first span; span: bytes from one to the next.
+DSGX_DEV void mma_f16_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+DSGX_DEV void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The products of one block, times 2^(E - 24): blk[s] = a lane's four sums (first strip's row g with rows 8 s + 2 t and + 1 of x,
+// then the second strip's).  st: the stage; x[s], sx[s]: this lane's activations and group sums at the block's first span;
+// span, sspan: bytes from one span to the next.
 template <int S>
-DSGX_DEV void unit_block(float (&acc)[S][4], uint32_t st, const uint32_t (&x_at)[S], uint32_t span, int lane) {
+DSGX_DEV void unit_block(float (&blk)[S][4], uint32_t st, const uint32_t (&x_at)[S], uint32_t span, const uint32_t (&sx_at)[S], uint32_t sspan,
+                         int lane) {
   const int g = lane >> 2;
   const uint4 zq = lds_v4(st + 4608 + 16 * g);
   const uint32_t* zw = &zq.x;
-  uint32_t x[S];
+  uint32_t x[S], sx[S];
 #pragma unroll
-  for (int s = 0; s < S; ++s) x[s] = x_at[s];
+  for (int s = 0; s < S; ++s) {
+    x[s] = x_at[s], sx[s] = sx_at[s];
+    blk[s][0] = blk[s][1] = blk[s][2] = blk[s][3] = 0.f;
+  }
 #pragma unroll
   for (int jj = 0; jj < 4; ++jj) {
     const uint4 sc = lds_v4(st + 4096 + 128 * jj + 16 * g);
@@ -72,30 +100,83 @@ DSGX_DEV void unit_block(float (&acc)[S][4], uint32_t st, const uint32_t (&x_at)
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       const uint4 w = lds_v4(st + 512 * (2 * jj + q) + 16 * lane);
+      float4 sum[S];  // of the two groups, the lane's two rows each
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        const uint4 v = lds_v4(sx[s]);
+        sum[s] = make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+      }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {  // the span's two groups
-        const uint32_t wa = c ? w.z : w.x, wb = c ? w.w : w.y;
-        const uint32_t zza = __byte_perm(q ? zo : ze, 0x43434343u, 0x4040u + 0x0101u * (2 * c)),
-                       zzb = __byte_perm(q ? zo : ze, 0x43434343u, 0x4040u + 0x0101u * (2 * c + 1));
-        uint32_t a[4], b[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) a[i] = nib_pair(wa, i, zza), b[i] = nib_pair(wb, i, zzb);
+        const uint32_t wa = c ? w.z : w.x, wb = c ? w.w : w.y, wa8 = wa >> 8, wb8 = wb >> 8;
+        // -z as a float: 0x4B0000zz is 2^23 + z
+        const float za = 8388608.f - __uint_as_float(__byte_perm(q ? zo : ze, 0x4B000000u, 0x7440u + 2 * c));
+        const float zb = 8388608.f - __uint_as_float(__byte_perm(q ? zo : ze, 0x4B000000u, 0x7440u + 2 * c + 1));
         const float fa = __uint_as_float(q ? sw[2 * c] & 0xffff0000u : sw[2 * c] << 16);
         const float fb = __uint_as_float(q ? sw[2 * c + 1] & 0xffff0000u : sw[2 * c + 1] << 16);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
           const uint4 xv = lds_v4(x[s] ^ (c ? 64u : 0u));
           float d[4];
-          mma_bf16_zero(d, a[0], b[0], a[1], b[1], xv.x, xv.y);
-          mma_bf16(d, a[2], b[2], a[3], b[3], xv.z, xv.w);
-          acc[s][0] = fmaf(fa, d[0], acc[s][0]), acc[s][1] = fmaf(fa, d[1], acc[s][1]);
-          acc[s][2] = fmaf(fb, d[2], acc[s][2]), acc[s][3] = fmaf(fb, d[3], acc[s][3]);
+          mma_f16_zero(d, wa & 0x000F000Fu, wb & 0x000F000Fu, wa & 0x00F000F0u, wb & 0x00F000F0u, xv.x, xv.y);
+          mma_f16(d, wa8 & 0x000F000Fu, wb8 & 0x000F000Fu, wa8 & 0x00F000F0u, wb8 & 0x00F000F0u, xv.z, xv.w);
+          const float s0 = c ? sum[s].z : sum[s].x, s1 = c ? sum[s].w : sum[s].y;
+          blk[s][0] = fmaf(fa, fmaf(za, s0, d[0]), blk[s][0]), blk[s][1] = fmaf(fa, fmaf(za, s1, d[1]), blk[s][1]);
+          blk[s][2] = fmaf(fb, fmaf(zb, s0, d[2]), blk[s][2]), blk[s][3] = fmaf(fb, fmaf(zb, s1, d[3]), blk[s][3]);
         }
       }
 #pragma unroll
-      for (int s = 0; s < S; ++s) x[s] += span;
+      for (int s = 0; s < S; ++s) x[s] += span, sx[s] += sspan;
     }
   }
+}
+
+// One row's 512 k of a block into the tile, by one warp (16 k a lane): f16 times 2^E, the groups' sums times 2^(E - 24), and
+// 2^(12 - E).  xt: the row's line in the block's first span; sx: its first group's sum; odd: the row's place among the lines.
+DSGX_DEV void stage_row(const __nv_bfloat16* row, int k0, int K, bool vec, uint8_t* xt, uint32_t span, bool odd, float* sx, uint32_t sspan,
+                        float* scale, int lane) {
+  const int k = k0 + 16 * lane;
+  uint32_t w[8];
+  if (vec && k + 16 <= K) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(row + k)), b = __ldg(reinterpret_cast<const uint4*>(row + k + 8));
+    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+  } else {
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t lo = k + 2 * i < K ? p[k + 2 * i] : 0u, hi = k + 2 * i + 1 < K ? p[k + 2 * i + 1] : 0u;
+      w[i] = lo | hi << 16;
+    }
+  }
+  uint32_t top = 0;  // the largest finite magnitude's bits
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t lo = w[i] & 0x7FFFu, hi = w[i] >> 16 & 0x7FFFu;
+    top = max(top, max(lo < 0x7F80u ? lo : 0u, hi < 0x7F80u ? hi : 0u));
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  const int E = top >= 0x80u ? min(14 + 127 - (int)(top >> 7), 126) : 126;  // (subnormal or zero: as small as it gets)
+  const float even = __uint_as_float((uint32_t)(E + 127) << 23), off = __uint_as_float((uint32_t)(E - 4 + 127) << 23);
+  uint32_t h[8];
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const __half lo = __float2half_rn(bf16_bits_to_f(w[i] & 0xffffu) * even), hi = __float2half_rn(bf16_bits_to_f(w[i] >> 16) * off);
+    sum = __fadd_rn(__fadd_rn(sum, __half2float(lo)), __half2float(hi) * 16.f);
+    h[i] = (uint32_t)__half_as_ushort(lo) | (uint32_t)__half_as_ushort(hi) << 16;
+  }
+  sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, 1));
+  uint4 o[2];  // words (v0 v1)(v2 v3)(v4 v5)(v6 v7) -> (v0 v4)(v1 v5)(v2 v6)(v3 v7)
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    uint32_t* d = &o[j].x;
+    d[0] = __byte_perm(h[4 * j], h[4 * j + 2], 0x5410), d[1] = __byte_perm(h[4 * j], h[4 * j + 2], 0x7632);
+    d[2] = __byte_perm(h[4 * j + 1], h[4 * j + 3], 0x5410), d[3] = __byte_perm(h[4 * j + 1], h[4 * j + 3], 0x7632);
+  }
+  uint4* d = reinterpret_cast<uint4*>(xt + (size_t)(lane >> 2) * span + (((lane & 3) * 32) ^ (odd ? 64 : 0)));
+  d[0] = o[0], d[1] = o[1];
+  if (!(lane & 1)) *reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(sx) + (size_t)(lane >> 2) * sspan + 8 * (lane >> 1 & 1)) = sum * 0x1p-24f;
+  if (lane == 0) *scale = __uint_as_float((uint32_t)(12 - E + 127) << 23);
 }
 
 // ---- the weights' own layout, once at load ------------------------------------------------------------------------------
@@ -146,8 +227,11 @@ DSGX_DEV void cluster_sync_all() {
 DSGX_DEV void remote_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-DSGX_DEV void st_remote(uint32_t addr, float4 v) {
-  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+// 16 bytes into another CTA's shared memory, counted by that CTA's barrier (no release that would wait for the round trip)
+DSGX_DEV void st_remote(uint32_t addr, float4 v, uint32_t bar) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(addr), "f"(v.x),
+               "f"(v.y), "f"(v.z), "f"(v.w), "r"(bar)
+               : "memory");
 }
 // bounded wait with the cluster's scope (the barrier's arrivals come from other CTAs)
 DSGX_DEV bool mbar_wait_cluster(uint64_t* bar, uint32_t parity) {
@@ -164,6 +248,11 @@ DSGX_DEV bool mbar_wait_cluster(uint64_t* bar, uint32_t parity) {
     if (ok) return true;
     if (clock64() - t0 > kWaitCycles) return false;
   }
+}
+DSGX_DEV float2 lds_f2(uint32_t a) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a));
+  return v;
 }
 DSGX_DEV float4 add4(float4 a, float4 b) {
   return make_float4(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y), __fadd_rn(a.z, b.z), __fadd_rn(a.w, b.w));
@@ -193,7 +282,10 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
   uint8_t* part = ring + (size_t)W * NST * kUnitBlk;                   // [P][S][32][4] f32
   uint8_t* recv = part + (size_t)P * kPart;                            // [kSlotsOwned][C][S][32][4] f32
   uint8_t* xt = recv + (C > 1 ? (size_t)kSlotsOwned * C * kPart : 0);  // [spans][M rows][128 B]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(xt + (size_t)p.xblocks * p.M * 1024);
+  const int Me = V::even(p.M);
+  float* xsum = reinterpret_cast<float*>(xt + (size_t)p.xblocks * p.M * 1024);  // [spans][row pairs][2 groups][2 rows]
+  float* xscale = xsum + (size_t)p.xblocks * Me * 16;                           // [blocks][rows]: 2^(12 - E)
+  uint64_t* bars = reinterpret_cast<uint64_t*>(xscale + (size_t)p.xblocks * Me);
   uint64_t* rfull = bars + W * NST;                                    // [kSlotsOwned] every rank's sums are in my buffer
   uint64_t* rfree = rfull + kSlotsOwned;                               // [owner][kSlotsOwned] that owner's buffer may be written
   int* cnt = reinterpret_cast<int*>(rfree + kMaxCluster * kSlotsOwned);  // [P] block pairs summed of a unit in flight
@@ -203,7 +295,7 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
   if (warp < W && lane == 0)
     for (int s = 0; s < NST; ++s) mbar_init(bars + warp * NST + s, 1);
   if (threadIdx.x == W * 32) {
-    for (int s = 0; s < kSlotsOwned; ++s) mbar_init(rfull + s, 32 * C);
+    for (int s = 0; s < kSlotsOwned; ++s) mbar_init(rfull + s, 1), mbar_expect_tx(rfull + s, C * kPart);
     for (int s = 0; s < kMaxCluster * kSlotsOwned; ++s) mbar_init(rfree + s, 1);
     *done = 0, *fail = 0;
   }
@@ -247,30 +339,27 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
 
   // ---- this rank's activations ------------------------------------------------------------------------------------------
   pdl_wait();
-  {
-    // tile: [span of 64 k][row][the span's 8 pieces of 8 bf16], a piece = the k a lane's word covers, in the words' nibble
-    // order; odd rows with the span's two groups exchanged, so that two rows' reads of one group do not meet in the banks
-    const bool vec = p.x_vec != 0;
-    const int n = nbk * 32;  // groups of 16 a row
-    for (int i = threadIdx.x; i < n * p.M; i += V::kThreads) {
-      const int r = i / n, kg = i - r * n;
-      uint4 o[2];
-      tile_group(o, p.x + (size_t)r * p.ldx, b0 * 512 + 16 * kg, p.K, vec);
-      uint4* d = reinterpret_cast<uint4*>(xt + (size_t)((kg >> 2) * p.M + r) * 128 + (((kg & 3) * 32) ^ ((r & 1) * 64)));
-      d[0] = o[0], d[1] = o[1];
-    }
+  // tile: [span of 64 k][row][the span's 8 pieces of 8 f16], a piece = the k a lane's word covers, in the words' nibble order;
+  // odd rows with the span's two groups exchanged, so that two rows' reads of one group do not meet in the banks
+  const uint32_t span = p.M * 128, sspan = Me * 8;
+  for (int i = warp; i < nbk * p.M; i += W + 1) {
+    const int b = i / p.M, r = i - b * p.M;
+    stage_row(p.x + (size_t)r * p.ldx, (b0 + b) * 512, p.K, p.x_vec != 0, xt + (size_t)b * 8 * span + r * 128, span, r & 1,
+              xsum + (size_t)b * 16 * Me + (r >> 1) * 4 + (r & 1), sspan, xscale + b * Me + r, lane);
   }
   __syncthreads();
 
   if (warp < W) {
     // ---- stream warps ---------------------------------------------------------------------------------------------------
     const int g = lane >> 2, t = lane & 3;
-    const uint32_t span = p.M * 128, ring_at = smem_u32(myring);
-    uint32_t xl[S];  // row 8 s + g of the tile (columns without a row: the last row, their sums are not used)
+    const uint32_t ring_at = smem_u32(myring);
+    uint32_t xl[S], sl[S], fl[S];  // row 8 s + g of the tile (columns without a row: the last row, their sums are not used)
 #pragma unroll
     for (int s = 0; s < S; ++s) {
       const int r = min(8 * s + g, p.M - 1);
+      const int pr = min(4 * s + t, Me / 2 - 1);  // the pair of rows whose sums the lane holds
       xl[s] = smem_u32(xt) + r * 128 + ((t * 16) ^ ((r & 1) * 64));
+      sl[s] = smem_u32(xsum) + pr * 16, fl[s] = smem_u32(xscale) + pr * 8;
     }
     uint32_t consumed = 0;
     bool ok = true;
@@ -278,9 +367,6 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
       const int rt = r0 + (j & (Q - 1)) * RPT;
       float acc[S][4], lv[3][S][4];  // the run's sums; the subtrees that wait for their right halves
       int b = p.nb * rt / kRuns, r = 0;
-      uint32_t xb[S];
-#pragma unroll
-      for (int s = 0; s < S; ++s) xb[s] = xl[s] + (b - b0) * 8 * span;
       for (; r < RPT; ++r) {
         const int e = p.nb * (rt + r + 1) / kRuns;
 #pragma unroll
@@ -291,9 +377,18 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
             ok = false;
             break;
           }
-          unit_block<S>(acc, ring_at + si * kUnitBlk, xb, span, lane);
+          uint32_t xb[S], sb[S];
+          float blk[S][4];
+          const int lb = b - b0;
 #pragma unroll
-          for (int s = 0; s < S; ++s) xb[s] += 8 * span;
+          for (int s = 0; s < S; ++s) xb[s] = xl[s] + lb * 8 * span, sb[s] = sl[s] + lb * 8 * sspan;
+          unit_block<S>(blk, ring_at + si * kUnitBlk, xb, span, sb, sspan, lane);
+#pragma unroll
+          for (int s = 0; s < S; ++s) {  // times 2^(24 - E), in two steps that cannot leave f32's range by themselves
+            const float2 f = lds_f2(fl[s] + lb * Me * 4);
+            acc[s][0] = fmaf(blk[s][0] * 4096.f, f.x, acc[s][0]), acc[s][1] = fmaf(blk[s][1] * 4096.f, f.y, acc[s][1]);
+            acc[s][2] = fmaf(blk[s][2] * 4096.f, f.x, acc[s][2]), acc[s][3] = fmaf(blk[s][3] * 4096.f, f.y, acc[s][3]);
+          }
           ++consumed;
           __syncwarp();
           if (lane == 0 && open_task()) issue();
@@ -410,10 +505,10 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
             ok = false;
             break;
           }
+          const uint32_t bar = map_rank(smem_u32(rfull + slot), owner);
           const uint32_t to = map_rank(smem_u32(recv) + (uint32_t)((slot * C + (int)rank) * kPart + lane * 16), owner);
 #pragma unroll
-          for (int s = 0; s < S; ++s) st_remote(to + 512 * s, a[s]);
-          remote_arrive(map_rank(smem_u32(rfull + slot), owner));
+          for (int s = 0; s < S; ++s) st_remote(to + 512 * s, a[s], bar);
         }
       }
       const int o = i - lag;
@@ -424,6 +519,7 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
           break;
         }
         join(reinterpret_cast<const float4*>(recv + (size_t)slot * C * kPart) + lane, C);
+        if (lane == 0) mbar_expect_tx(rfull + slot, C * kPart);  // (for the unit that takes the buffer next)
         __syncwarp();
         if (lane < C) remote_arrive(map_rank(smem_u32(rfree + rank * kSlotsOwned + slot), lane));
         write(u0 + o);
@@ -493,11 +589,11 @@ cudaError_t launch(LinearParams p, cudaStream_t st, bool* fits) {
   if (!best) return cudaSuccess;
   p.cluster = best, p.xblocks = (p.nb + best - 1) / best;
   p.lc = best == 8 ? 3 : best == 4 ? 2 : best == 2 ? 1 : 0;
-  // Tasks a unit: as few as leave every stream warp of a CTA eight tasks (the last task of a launch is idle time of the
+  // Tasks a unit: as few as leave every stream warp of a CTA three tasks (the last task of a launch is idle time of the
   // others), at most one a block or a run.
   const int per_cta = (p.units + clusters - 1) / clusters;
   p.lq = 0;
-  while ((2 << p.lq) <= kRuns / best && (2 << p.lq) <= p.xblocks && (per_cta << p.lq) < 8 * V::W) ++p.lq;
+  while ((2 << p.lq) <= kRuns / best && (2 << p.lq) <= p.xblocks && (per_cta << p.lq) < 3 * V::W) ++p.lq;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((p.units < clusters ? p.units : clusters) * best), cfg.blockDim = dim3(V::kThreads);
   cfg.dynamicSmemBytes = V::smem(p.M, p.xblocks, best), cfg.stream = st;
@@ -515,7 +611,7 @@ cudaError_t launch(LinearParams p, cudaStream_t st, bool* fits) {
 // One launch for M rows, or *fits = false where their activations do not fit shared memory.
 cudaError_t launch_linear_int4(const LinearParams& p, cudaStream_t st, bool* fits) {
   if (p.M <= 8) return launch<LinVar<1, 15, 2, 32>>(p, st, fits);
-  return launch<LinVar<2, 15, 2, 16>>(p, st, fits);
+  return launch<LinVar<2, 11, 2, 16>>(p, st, fits);
 }
 
 size_t linear_bytes(int N, int K, bool glu) {
