@@ -55,6 +55,10 @@ class LayerStep(C.Structure):
                 ("norm_w", C.c_void_p), ("xn_out", C.c_void_p), ("norm_eps", C.c_float), ("norm_mode", C.c_int32)]
 
 
+class MoeBlock(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("wr", "bias", "idx", "w", "ws", "reserved")]
+
+
 class LinearW(C.Structure):
     _fields_ = [("w", C.c_void_p), ("N", C.c_int32), ("K", C.c_int32), ("fmt", C.c_uint32), ("glu", C.c_int32)]
 
@@ -83,6 +87,8 @@ SYMBOLS = {
     "dsgx_finalize": (_I, [_V, _V, _I, _I, _V, _I, _V]),
     "dsgx_moe_layer_decode": (_I, [C.POINTER(MoeShape), C.POINTER(LayerW), _V, _I, C.POINTER(LayerStep), _I, _V]),
     "dsgx_moe_layer_decode_host": (_I, [C.POINTER(MoeShape), C.POINTER(LayerW), _V, _I, C.POINTER(LayerStep), _V, _V]),
+    "dsgx_moe_block_ws_bytes": (_Z, [C.POINTER(MoeShape)]),
+    "dsgx_moe_block_decode": (_I, [C.POINTER(MoeShape), C.POINTER(LayerW), _V, _I, C.POINTER(MoeBlock), _V, _V, _V]),
     "dsgx_linear_bytes": (_Z, [_I, _I, _I]),
     "dsgx_linear_prepare": (_I, [_V, _V, C.c_uint32, _I, _I, _V, _V]),
     "dsgx_linear_decode": (_I, [C.POINTER(LinearW), _V, C.c_int64, _I, _V, C.c_int64, _V, C.c_int64, _I, _V, _V]),

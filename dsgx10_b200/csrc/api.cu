@@ -407,6 +407,47 @@ int dsgx_moe_layer_decode_host(const dsgx_moe_shape* s, const dsgx_layer_w* L, c
   return e == cudaSuccess ? DSGX_OK : cuda_fail(e);
 }
 
+static int check_block_shape(const dsgx_moe_shape* s) {
+  const int rc = check_shape(s);
+  if (rc) return rc;
+  if (s->fmt != DSGX_FMT_INT4 && s->fmt != DSGX_FMT_BF16) return DSGX_ERR_FORMAT;
+  if (s->e_lo != 0 || s->e_hi != s->E) return DSGX_ERR_UNSUPPORTED;  // (one GPU holds the whole layer)
+  return block_rows(s->H, s->I, 1) ? DSGX_OK : DSGX_ERR_SHAPE;
+}
+
+size_t dsgx_moe_block_ws_bytes(const dsgx_moe_shape* s) { return check_block_shape(s) ? 0 : block_ws_bytes(s->H, s->I); }
+
+int dsgx_moe_block_decode(const dsgx_moe_shape* s, const dsgx_layer_w* L, const void* x, int M, const dsgx_moe_block* b, const void* res,
+                          void* out, void* stream) {
+  const int rc = check_block_shape(s);
+  if (rc) return rc;
+  if (!L || !x || !b || !out || !b->wr || !b->idx || !b->w || !b->ws || !L->pool || !L->desc) return DSGX_ERR_ARG;
+  if (M < 1 || M > DSGX_MAX_STEP_ROWS) return DSGX_ERR_ARG;
+  if (L->fmt != s->fmt || L->sh.g || L->sh.u || L->sh.d) return DSGX_ERR_FORMAT;  // (the shared expert is bf16)
+  const bool shb = L->sh.bg != nullptr || L->sh.bgu != nullptr;
+  if (shb ? (!L->sh.bd || (L->sh.bgu ? (L->sh.bg || L->sh.bu) : !L->sh.bu)) : (L->sh.bu || L->sh.bd)) return DSGX_ERR_ARG;
+  if (((uintptr_t)L->pool | (uintptr_t)b->ws) & 255) return DSGX_ERR_ARG;
+  if (((uintptr_t)x | (uintptr_t)b->wr | (uintptr_t)L->desc | (uintptr_t)L->sh.bg | (uintptr_t)L->sh.bu | (uintptr_t)L->sh.bd | (uintptr_t)L->sh.bgu) & 15)
+    return DSGX_ERR_ARG;
+  if ((((uintptr_t)res | (uintptr_t)out) & 7) || (((uintptr_t)b->bias | (uintptr_t)b->idx | (uintptr_t)b->w) & 3)) return DSGX_ERR_ARG;
+  BlockParams p{};
+  p.H = s->H, p.I = s->I, p.E = s->E, p.topk = s->topk, p.b16 = s->fmt == DSGX_FMT_BF16, p.fmt = s->fmt;
+  p.pool = L->pool, p.desc = L->desc, p.sh_g = L->sh.bg, p.sh_u = L->sh.bu, p.sh_d = L->sh.bd, p.sh_bgu = L->sh.bgu;
+  p.rp = RouteParams{s->E, s->topk, s->n_group, s->topk_group, s->score_fn, s->norm_topk, s->route_scale};
+  p.wr = b->wr, p.bias = b->bias;
+  const int per = block_rows(s->H, s->I, M);
+  for (int r = 0; r < M; r += per) {  // (more rows than one launch takes: in stream order on the same workspace)
+    p.M = M - r < per ? M - r : per;
+    p.x = reinterpret_cast<const __nv_bfloat16*>(x) + (size_t)r * s->H;
+    p.res = res ? reinterpret_cast<const __nv_bfloat16*>(res) + (size_t)r * s->H : nullptr;
+    p.out = reinterpret_cast<__nv_bfloat16*>(out) + (size_t)r * s->H;
+    p.idx = b->idx + (size_t)r * s->topk, p.w = b->w + (size_t)r * s->topk;
+    cudaError_t e = launch_block_int4(p, b->ws, (cudaStream_t)stream);
+    if (e != cudaSuccess) return cuda_fail(e);
+  }
+  return DSGX_OK;
+}
+
 static bool linear_shape_ok(int N, int K) {
   return N >= 1 && K >= 1 && N <= (1 << 30) && K <= (1 << 30) && (((size_t)N + 7) / 8) * (((size_t)K + 511) / 512) < ((size_t)1 << 31);
 }

@@ -1,0 +1,699 @@
+// A whole INT4-g32 (or BF16) MoE layer for 1..8 rows in one launch: router logits, routing, the picked experts' gate / up with
+// SwiGLU, down, the bf16 shared expert, the weighted sum in ascending expert id, the residual, the rounding.
+//
+// Bound: the weights of the distinct picked experts are read once, so HBM.  One CTA a SM, launched cooperatively (all resident
+// together, so CTAs may wait for one another; every wait is bounded and a run-out is recorded in the workspace).  Twelve
+// warps compute: eleven stream weights through private rings of bulk copies, one joins their sums; four prepare activations.
+//
+//   front    every CTA but the last M: the router's logit slices (route.cuh's order).  The last M CTAs route a row each; the
+//            last of them builds the step's table: the picked experts in ascending id with the rows that picked them.
+//   shared   meanwhile the other CTAs stream the shared expert's gate and up matrices, which need no routing.
+//   up       a CTA owns a run of (expert, 8 channels) units, shorter where it has streamed more of the shared expert.
+//   down     the shared expert's tiles first (its h is ready early), then a run of (expert, 16 channels) units as soon as the
+//            expert's h is complete; their weights are already in the rings.
+//   combine  after a grid-wide count: every element adds its row's picks, the shared expert and the residual.
+//
+// Work items.  A unit (16 weight rows) is cut along K in tasks of about two 512-k blocks, dealt to the stream warps in turn
+// across units and phases; a task's sums go to shared memory and the joining warp adds a unit's tasks in ascending k.  The cut
+// depends on H and I alone, so a row's bits do not depend on the other rows.
+//
+// An INT4 block is used as the experts' format has it (decode_int4.cu).  Its lanes mix two groups of 32 in every MMA (lane 4 g +
+// t holds k = 64 q + 16 t + 0..15 of row g: lanes t = 0, 1 one group, t = 2, 3 the next), so the eight columns of B are (row of
+// x, half) pairs: column 2 r + h holds row r's values in the lanes of half h and zeros in the others, lane (g, t) ends with
+// both groups' sums of row t and two packed multiply-adds finish 64 k (scale, zero point: int4_mma.cuh).  Four rows of x a
+// set of MMAs; an expert that more rows picked takes two sets.  Only the rows that picked an expert are computed for it.
+//
+// The expert's input rows and h are f16 with a power of two a 512-k block; gate, up and the down sums stay f32; h is rounded to
+// bf16 once, because it is an MMA operand (2^-9 of its value; a second half would double the down products' MMAs).
+#include <atomic>
+#include <type_traits>
+
+#include "common.cuh"
+#include "decode_common.cuh"
+#include "int4_mma.cuh"
+#include "kernels.h"
+#include "route.cuh"
+
+namespace dsgx {
+
+constexpr int kMaxEnt = kMaxRows * kMaxTopK;
+
+// A picked expert: its matrices, the rows that picked it (n of them, ascending, a byte each).
+struct alignas(16) BlockEnt {
+  const uint8_t *g, *u, *d;
+  unsigned long long rows;
+  int n;
+  int pad[3];
+};
+struct alignas(16) BlockTab {
+  int nslots, bad, npick, pad;
+  BlockEnt ent[kMaxEnt];
+  int pick[kMaxRows][kMaxTopK];   // a row's picks in ascending expert id: slot | its place among the slot's rows << 8
+  float w[kMaxRows][kMaxTopK];
+};
+static_assert(sizeof(BlockEnt) == 48 && sizeof(BlockTab) % 16 == 0, "copied in 16-byte pieces");
+
+struct BlockSync {
+  int cnt_lp, cnt_rt, tab_ready, cnt_done, cnt_exit, pad[3];
+  int cnt_h[kMaxEnt + 1];  // gate/up units of a slot that are in memory
+};
+
+namespace {
+
+constexpr int kStreamW = 11, kStageW0 = kStreamW + 1, kWarps = 16, kStagers = kWarps - kStageW0, kThreads = kWarps * 32;
+constexpr int kStage = 2 * kQBlk;        // a ring stage: an INT4 block pair (a pair of bf16 blocks, 4096 B, fits)
+constexpr int kP = 16;                   // tasks' sums in flight
+constexpr int kPart = 512;               // bytes of a task's sums: [2 sets][32 lanes][2] f32
+constexpr int kShared = kMaxEnt;         // the shared expert's place among the h, y and counters
+constexpr int kMaxSegs = kMaxEnt + 4;
+constexpr size_t kSmemMax = 227 * 1024;
+
+// A CTA's run of units of one phase.
+struct Seg {
+  int down, b16, slot, rows;  // slot: of a down run (an up run covers several); rows: of the activation tile
+  int u0, n;                  // units; an up run's unit u: slot u / (I / 8)
+  int tasks, base;            // tasks of the run; tasks before it
+};
+
+DSGX_DEV int tasks_of(int nb) { return nb <= 1 ? 1 : nb / 2 < 8 ? nb / 2 : 8; }  // tasks a unit
+
+// ---- the tile of activations: [nb x 8 spans][rows][128 B], then group sums [spans][rows][2], then scales [nb][rows]
+__host__ __device__ inline size_t tile_bytes(int K, int rows) { return (size_t)K / 512 * rows * (1024 + 64 + 4) + 16; }
+struct Tile {
+  uint8_t* x;
+  float *sum, *scale;
+  DSGX_DEV Tile(uint8_t* base, int nb, int rows) : x(base), sum(reinterpret_cast<float*>(base + (size_t)nb * rows * 1024)), scale(sum + (size_t)nb * rows * 16) {}
+};
+
+// One INT4 block pair: acc[s][strip] += (.x, .y: the two halves of the groups) row g of strip a / b times the lane's row t of set s,
+// times 2^(E - 24).
+template <int S>
+DSGX_DEV void pair_int4(float2 (&acc)[S][2], uint32_t st, const uint32_t (&x_at)[S], const uint32_t (&step)[S], const uint32_t (&sum_at)[S],
+                        uint32_t sstep, int lane) {
+  const int g = lane >> 2;
+  const uint2 za = lds_v2(st + 2304 + 8 * g), zb = lds_v2(st + kQBlk + 2304 + 8 * g);  // the halves' eight zero points each
+  const uint4 sa0 = lds_v4(st + 2048 + 32 * g), sa1 = lds_v4(st + 2048 + 32 * g + 16);
+  const uint4 sb0 = lds_v4(st + kQBlk + 2048 + 32 * g), sb1 = lds_v4(st + kQBlk + 2048 + 32 * g + 16);
+  const uint32_t *a0 = &sa0.x, *a1 = &sa1.x, *b0 = &sb0.x, *b1 = &sb1.x;
+  uint32_t x[S], sm[S];
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    x[s] = x_at[s], sm[s] = sum_at[s];
+    acc[s][0] = acc[s][1] = make_float2(0.f, 0.f);
+  }
+#pragma unroll
+  for (int jj = 0; jj < 4; ++jj) {
+    const uint4 va = lds_v4(st + 512 * jj + 16 * lane), vb = lds_v4(st + kQBlk + 512 * jj + 16 * lane);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const uint32_t al = q ? va.z : va.x, ah = q ? va.w : va.y, bl = q ? vb.z : vb.x, bh = q ? vb.w : vb.y;
+      const uint32_t al8 = al >> 8, ah8 = ah >> 8, bl8 = bl >> 8, bh8 = bh >> 8;
+      const float2 mza = make_float2(minus_zero(q ? za.x >> 4 & 0x0F0F0F0Fu : za.x & 0x0F0F0F0Fu, jj), minus_zero(q ? za.y >> 4 & 0x0F0F0F0Fu : za.y & 0x0F0F0F0Fu, jj));
+      const float2 mzb = make_float2(minus_zero(q ? zb.x >> 4 & 0x0F0F0F0Fu : zb.x & 0x0F0F0F0Fu, jj), minus_zero(q ? zb.y >> 4 & 0x0F0F0F0Fu : zb.y & 0x0F0F0F0Fu, jj));
+      const float2 fa = q ? make_float2(scale_hi(a0[jj]), scale_hi(a1[jj])) : make_float2(scale_lo(a0[jj]), scale_lo(a1[jj]));
+      const float2 fb = q ? make_float2(scale_hi(b0[jj]), scale_hi(b1[jj])) : make_float2(scale_lo(b0[jj]), scale_lo(b1[jj]));
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        const uint4 x0 = lds_v4(x[s]), x1 = lds_v4(x[s] + 16);
+        const float2 sum = lds_f2(sm[s]);
+        x[s] += step[s], sm[s] += sstep;
+        float d[4];
+        mma_f16_zero(d, al & kNib0, bl & kNib0, al & kNib1, bl & kNib1, x0.x, x0.y);
+        mma_f16(d, al8 & kNib0, bl8 & kNib0, al8 & kNib1, bl8 & kNib1, x0.z, x0.w);
+        mma_f16(d, ah & kNib0, bh & kNib0, ah & kNib1, bh & kNib1, x1.x, x1.y);
+        mma_f16(d, ah8 & kNib0, bh8 & kNib0, ah8 & kNib1, bh8 & kNib1, x1.z, x1.w);
+        acc[s][0] = fma2(fa, fma2(mza, sum, make_float2(d[0], d[1])), acc[s][0]);
+        acc[s][1] = fma2(fb, fma2(mzb, sum, make_float2(d[2], d[3])), acc[s][1]);
+      }
+    }
+  }
+}
+
+// One bf16 block pair (128 k) on a bf16 tile: all eight columns are rows of x (column n: row n / 2 + 4 (n & 1), so that a lane
+// ends with rows t and t + 4).
+DSGX_DEV void pair_b16(float (&d)[4], uint32_t st, uint32_t x, uint32_t span, int lane) {
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const uint32_t a = st + 1024 * q + 16 * lane;
+    const uint4 a0 = lds_v4(a), a1 = lds_v4(a + 512), b0 = lds_v4(a + kQBlk), b1 = lds_v4(a + kQBlk + 512);
+    const uint4 x0 = lds_v4(x), x1 = lds_v4(x + 16);
+    x += span;
+    mma_bf16(d, __byte_perm(a0.x, a0.z, 0x5410), __byte_perm(b0.x, b0.z, 0x5410), __byte_perm(a0.x, a0.z, 0x7632), __byte_perm(b0.x, b0.z, 0x7632), x0.x, x0.y);
+    mma_bf16(d, __byte_perm(a0.y, a0.w, 0x5410), __byte_perm(b0.y, b0.w, 0x5410), __byte_perm(a0.y, a0.w, 0x7632), __byte_perm(b0.y, b0.w, 0x7632), x0.z, x0.w);
+    mma_bf16(d, __byte_perm(a1.x, a1.z, 0x5410), __byte_perm(b1.x, b1.z, 0x5410), __byte_perm(a1.x, a1.z, 0x7632), __byte_perm(b1.x, b1.z, 0x7632), x1.x, x1.y);
+    mma_bf16(d, __byte_perm(a1.y, a1.w, 0x5410), __byte_perm(b1.y, b1.w, 0x5410), __byte_perm(a1.y, a1.w, 0x7632), __byte_perm(b1.y, b1.w, 0x7632), x1.z, x1.w);
+  }
+}
+
+// ---- the division of a phase's units over the CTAs.  n shared units of cost cs over the first Gs CTAs, N routed ones of cost c so
+// that every CTA's total is alike: where CTA i's routed run begins.
+DSGX_DEV int shared_begin(int i, int n, int Gs) { return (int)((long long)n * min(i, Gs) / Gs); }
+DSGX_DEV int routed_begin(int i, int N, long long c, int n, long long cs, int Gs, int G) {
+  if (i <= 0) return 0;
+  if (i >= G) return N;
+  const long long total = N * c + n * cs;
+  if (total / G < cs * ((n + Gs - 1) / Gs + 1)) return (int)((long long)N * i / G);  // (few routed units: an even deal)
+  const long long before = total * i / G - cs * shared_begin(i, n, Gs);
+  return (int)min((long long)N, max(0ll, before / c));
+}
+
+// ---- the table, by one whole CTA; scratch: 16 + 2 x kMaxEnt words of shared memory --------------------------------------------
+DSGX_DEV void build_block_tab(BlockTab& tab, uint32_t* scratch, const int* idx, const float* w, const BlockParams& p) {
+  uint32_t *bm = scratch, *mask = scratch + 16;
+  int* id = reinterpret_cast<int*>(mask + kMaxEnt);
+  const int tid = threadIdx.x, np = p.M * p.topk;
+  if (tid < 16) bm[tid] = 0;
+  if (tid < kMaxEnt) mask[tid] = 0;
+  if (tid == 0) tab.bad = 0;
+  __syncthreads();
+  auto known = [&](int e) { return e >= 0 && e < p.E; };
+  auto rank_of = [&](int e) {
+    int r = __popc(bm[e >> 5] & ((1u << (e & 31)) - 1u));
+    for (int k = 0; k < (e >> 5); ++k) r += __popc(bm[k]);
+    return r;
+  };
+  if (tid < np && known(idx[tid])) atomicOr(&bm[idx[tid] >> 5], 1u << (idx[tid] & 31));
+  if (tid < np && !known(idx[tid])) tab.bad = DSGX_ERR_ARG;
+  __syncthreads();
+  int slot = 0;
+  if (tid < np && known(idx[tid])) {
+    slot = rank_of(idx[tid]);
+    atomicOr(&mask[slot], 1u << (tid / p.topk));
+    id[slot] = idx[tid];
+  }
+  __syncthreads();
+  int n = 0;
+  for (int k = 0; k < 16; ++k) n += __popc(bm[k]);
+  if (tid < n) {
+    const dsgx_mat_desc* d = p.desc + (size_t)id[tid] * 3;
+    BlockEnt& e = tab.ent[tid];
+    if (d[0].fmt != p.fmt || d[1].fmt != p.fmt || d[2].fmt != p.fmt) tab.bad = DSGX_ERR_FORMAT;
+    e.g = p.pool + d[0].off, e.u = p.pool + d[1].off, e.d = p.pool + d[2].off;
+    unsigned long long rows = 0;
+    int c = 0;
+    for (int r = 0; r < kMaxRows; ++r)
+      if (mask[tid] >> r & 1) rows |= (unsigned long long)r << (8 * c++);
+    e.rows = rows, e.n = c;
+  }
+  if (tid < np && known(idx[tid])) {
+    const int m = tid / p.topk;
+    int place = 0;  // among the row's picks, ascending expert id
+    for (int j = 0; j < p.topk; ++j) place += idx[m * p.topk + j] < idx[tid];
+    tab.pick[m][place] = slot | __popc(mask[slot] & ((1u << m) - 1u)) << 8;
+    tab.w[m][place] = w[tid];
+  }
+  __syncthreads();
+  if (tid == 0) tab.nslots = tab.bad ? 0 : n, tab.npick = tab.bad ? 0 : p.topk;
+  __syncthreads();
+}
+
+template <int NST>
+__global__ void __launch_bounds__(kThreads, 1) k_block(const BlockParams p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int G = gridDim.x, cta = blockIdx.x;
+  const int nbH = p.H / 512, nbI = p.I / 512, upp = p.I / 8, NT = p.H / 16, QH = tasks_of(nbH), QI = tasks_of(nbI);
+  uint8_t* ring = smem;
+  uint8_t* part = ring + (size_t)kStreamW * NST * kStage;
+  BlockTab& tab = *reinterpret_cast<BlockTab*>(part + kP * kPart);
+  uint8_t* tiles = reinterpret_cast<uint8_t*>(&tab + 1);  // [nbuf] activation tiles
+  uint8_t* zero = tiles + (size_t)p.nbuf * p.tile + 16;   // 32 bytes, off the banks that the tile's lines use
+  uint64_t* bars = reinterpret_cast<uint64_t*>(zero + 48);
+  uint64_t* tile_full = bars + kStreamW * NST;            // [kMaxSegs] the segment's activations are in their tile
+  uint64_t* tile_free = tile_full + kMaxSegs;             // [kMaxSegs] no stream warp reads them any more
+  uint64_t* tabbar = tile_free + kMaxSegs;                // the table and all segments are known
+  Seg* segs = reinterpret_cast<Seg*>(tabbar + 2);
+  int* cnt = reinterpret_cast<int*>(segs + kMaxSegs);     // [kP] tasks summed of a unit in flight
+  int* done = cnt + kP;                                   // tasks whose unit has been joined
+  int* s_nseg = done + 1;
+  int* s_fail = done + 2;
+  int* s_tick = done + 3;
+  BlockSync* sy = p.sync;
+
+  if (warp < kStreamW && lane == 0)
+    for (int s = 0; s < NST; ++s) mbar_init(bars + warp * NST + s, 1);
+  for (int i = threadIdx.x; i < kMaxSegs; i += kThreads) mbar_init(tile_full + i, kStagers), mbar_init(tile_free + i, kStreamW);
+  if (threadIdx.x < kP) cnt[threadIdx.x] = 0;
+  if (threadIdx.x < 8) reinterpret_cast<uint32_t*>(zero)[threadIdx.x] = 0;
+
+  const bool has_sh = p.sh_d != nullptr;
+  const int Gs = G - p.M;  // the CTAs that do not route
+  const bool router = cta >= Gs;
+  // the run that needs no routing: the shared expert's gate and up
+  const int a0 = has_sh && !router ? shared_begin(cta, upp, Gs) : 0, a1 = has_sh && !router ? shared_begin(cta + 1, upp, Gs) : 0;
+  if (threadIdx.x == 0) {
+    mbar_init(tabbar, 1);
+    *done = 0, *s_nseg = 0, *s_fail = 0;
+    segs[0] = Seg{0, 1, kShared, p.M, a0, a1 - a0, (a1 - a0) * QH, 0};
+  }
+  mbar_fence_init();
+  __syncthreads();
+
+  if (router) {
+    // ---- a row each; the last one to be routed builds the table -------------------------------------------------------------
+    RouteSmem& rs = *reinterpret_cast<RouteSmem*>(tiles);
+    int* s_idx = reinterpret_cast<int*>(part);
+    float* s_w = reinterpret_cast<float*>(s_idx + kMaxEnt);
+    uint32_t* scratch = reinterpret_cast<uint32_t*>(s_w + kMaxEnt);
+    const int row = cta - Gs, KS = (p.H + 1023) / 1024;
+    if (threadIdx.x == 0) *s_tick = poll_ge(&sy->cnt_lp, Gs) ? 1 : 0;
+    __syncthreads();
+    bool ok = *s_tick != 0;
+    __syncthreads();
+    if (ok) {
+      route_row_cta(p.rp, p.lpart + (size_t)row * p.E, KS, (size_t)kMaxRows * p.E, p.bias, rs, nullptr, p.idx + row * p.topk, p.w + row * p.topk);
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) *s_tick = atomicAdd(&sy->cnt_rt, 1);
+      __syncthreads();
+      if (*s_tick == p.M - 1) {
+        __threadfence();
+        if ((int)threadIdx.x < p.M * p.topk) s_idx[threadIdx.x] = __ldcg(p.idx + threadIdx.x), s_w[threadIdx.x] = __ldcg(p.w + threadIdx.x);
+        __syncthreads();
+        build_block_tab(tab, scratch, s_idx, s_w, p);
+        if (threadIdx.x == 0 && tab.bad) atomicCAS(p.status, 0, tab.bad);
+        const uint4* s4 = reinterpret_cast<const uint4*>(&tab);
+        for (int i = threadIdx.x; i < (int)(sizeof(BlockTab) / 16); i += kThreads) reinterpret_cast<uint4*>(p.tab)[i] = s4[i];
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) atomicExch(&sy->tab_ready, 1);
+      }
+    } else if (threadIdx.x == 0) {
+      *s_fail = 1;
+    }
+    __syncthreads();
+  } else if (warp < kStageW0) {
+    // ---- the router's logit slices, one warp a (expert, 1024 k); a CTA reports when all of its are in memory ------------------
+    const int KS = (p.H + 1023) / 1024, ntask = p.E * KS;
+    for (int i = warp * Gs + cta; i < ntask; i += kStageW0 * Gs) logit_slice_task(p.x, p.wr, p.M, p.H, p.E, i / KS, i % KS, p.lpart, lane);
+    __threadfence();
+    asm volatile("bar.sync 1, %0;" ::"n"(kStageW0 * 32) : "memory");
+    if (threadIdx.x == 0) {
+      __threadfence();
+      atomicAdd(&sy->cnt_lp, 1);
+    }
+  }
+
+  const int nb_first = a1 > a0 ? 1 : 0;  // segments known without the table
+  if (warp < kStreamW) {
+    // ---- stream warps --------------------------------------------------------------------------------------------------------
+    uint8_t* myring = ring + (size_t)warp * NST * kStage;
+    uint64_t* mybar = bars + warp * NST;
+    const uint32_t ring_at = smem_u32(myring);
+    const uint64_t pol = policy_evict_first();
+    uint32_t issued = 0, consumed = 0;
+    bool ok = true;
+    auto first_task = [&](const Seg& s) { return (int)((unsigned)(warp + kStreamW - s.base % kStreamW) % kStreamW); };
+    // producer (lane 0): segment, task, block, quarter of a bf16 block
+    int nknown = nb_first, ps = 0, pt = -1, pb = 0, pe = 0, pc = 0;
+    bool all_known = false;
+    const uint8_t *pa = nullptr, *pz = nullptr;
+    auto open_task = [&]() {
+      while (pb == pe) {
+        if (ps >= nknown) {
+          if (!all_known && mbar_test_wait(tabbar, 0)) all_known = true, nknown = *s_nseg;
+          if (ps >= nknown) return false;
+        }
+        const Seg& s = segs[ps];
+        if (pt < 0) pt = first_task(s);
+        if (pt >= s.tasks) {
+          ++ps, pt = -1;
+          continue;
+        }
+        const int Q = s.down ? QI : QH, nb = s.down ? nbI : nbH;
+        int u = s.u0 + pt / Q;
+        const int q = pt % Q;
+        pb = nb * q / Q, pe = nb * (q + 1) / Q, pc = 0, pt += kStreamW;
+        const size_t blk = s.b16 ? 4 * kHBlk : kQBlk;  // bytes of 8 rows x 512 k
+        if (s.down) {
+          const uint8_t* d = s.slot == kShared ? p.sh_d : tab.ent[s.slot].d;
+          pa = d + (size_t)(2 * u) * nb * blk, pz = pa + nb * blk;
+        } else if (s.slot == kShared) {
+          if (p.sh_bgu) pa = p.sh_bgu + (size_t)(2 * u) * nb * blk, pz = pa + nb * blk;
+          else pa = p.sh_g + (size_t)u * nb * blk, pz = p.sh_u + (size_t)u * nb * blk;
+        } else {
+          const BlockEnt& e = tab.ent[u / upp];
+          u %= upp;
+          pa = e.g + (size_t)u * nb * blk, pz = e.u + (size_t)u * nb * blk;
+        }
+        pa += pb * blk, pz += pb * blk;
+      }
+      return true;
+    };
+    int pseg_b16 = 0;
+    auto issue = [&]() {
+      pseg_b16 = segs[ps].b16;
+      const uint32_t slot = issued % NST, bytes = pseg_b16 ? kHBlk : kQBlk;
+      uint8_t* st = myring + slot * kStage;
+      mbar_expect_tx(mybar + slot, 2 * bytes);
+      bulk_g2s_hint(st, pa, bytes, mybar + slot, pol);
+      bulk_g2s_hint(st + kQBlk, pz, bytes, mybar + slot, pol);
+      ++issued, pa += bytes, pz += bytes;
+      if (!pseg_b16 || ++pc == 4) ++pb, pc = 0;
+    };
+    auto fill = [&]() {
+      while (issued - consumed < (uint32_t)NST && open_task()) issue();
+    };
+    if (lane == 0) fill();
+    auto stage_ready = [&]() {
+      const uint32_t si = consumed % NST;
+      if (!mbar_wait(mybar + si, (consumed / NST) & 1)) ok = false;
+      return ring_at + si * kStage;
+    };
+    auto stage_used = [&]() {
+      ++consumed;
+      __syncwarp();
+      if (lane == 0) fill();
+    };
+
+    for (int k = 0; ok; ++k) {
+      if (k >= nb_first) {  // (the table is needed from here on)
+        if (k == nb_first && !mbar_wait(tabbar, 0, 64)) ok = false;
+        if (!ok || *s_fail || k >= *s_nseg) break;
+        if (lane == 0) fill();
+      }
+      const Seg s = segs[k];
+      if (!mbar_wait(tile_full + k, 0, 20)) {
+        ok = false;
+        break;
+      }
+      const int Q = s.down ? QI : QH, nb = s.down ? nbI : nbH;
+      const Tile tile(tiles + (size_t)(k % p.nbuf) * p.tile, nb, s.rows);
+      const uint32_t span = s.rows * 128, x0 = smem_u32(tile.x), z0 = smem_u32(zero);
+      for (int i = first_task(s); i < s.tasks && ok; i += kStreamW) {
+        const int u = s.u0 + i / Q, q = i % Q, b0 = nb * q / Q, b1 = nb * (q + 1) / Q;
+        // the rows of this unit: the place in the tile of the j-th
+        unsigned long long rows = 0x0706050403020100ull;
+        int n = s.rows;
+        if (!s.down && s.slot != kShared) rows = tab.ent[u / upp].rows, n = tab.ent[u / upp].n;
+        auto row = [&](int j) { return (int)(rows >> (8 * min(j, n - 1)) & 0xff); };
+        float acc[2][2] = {{0.f, 0.f}, {0.f, 0.f}};  // [rows t, t + 4][strip]
+        if (s.b16) {
+          const uint32_t xr = x0 + row((g >> 1) + 4 * (g & 1)) * 128 + t * 32;
+          for (int b = b0; b < b1 && ok; ++b) {
+            float d[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int c = 0; c < 4; ++c) {
+              const uint32_t st = stage_ready();
+              if (!ok) break;
+              pair_b16(d, st, xr + (8 * b + 2 * c) * span, span, lane);
+              stage_used();
+            }
+            acc[0][0] = __fadd_rn(acc[0][0], d[0]), acc[1][0] = __fadd_rn(acc[1][0], d[1]);
+            acc[0][1] = __fadd_rn(acc[0][1], d[2]), acc[1][1] = __fadd_rn(acc[1][1], d[3]);
+          }
+        } else {
+          const bool mine = (t >> 1) == (g & 1);
+          auto run = [&](auto sets) {
+            constexpr int S = decltype(sets)::value;
+            uint32_t xr[S], step[S], sr[S], fr[S];
+#pragma unroll
+            for (int e = 0; e < S; ++e) {
+              const int col = 4 * e + (g >> 1), me = row(4 * e + t);
+              const bool on = mine && col < n;
+              xr[e] = on ? x0 + b0 * 8 * span + row(col) * 128 + t * 32 : z0, step[e] = on ? span : 0u;
+              sr[e] = smem_u32(tile.sum) + (b0 * 8 * s.rows + me) * 8, fr[e] = smem_u32(tile.scale) + (b0 * s.rows + me) * 4;
+            }
+            for (int b = b0; b < b1; ++b) {
+              const uint32_t st = stage_ready();
+              if (!ok) break;
+              float2 blk[S][2];
+              pair_int4<S>(blk, st, xr, step, sr, s.rows * 8, lane);
+#pragma unroll
+              for (int e = 0; e < S; ++e) {  // times 2^(24 - E), in two steps that cannot leave f32's range by themselves
+                const float f = lds_f(fr[e]);
+                acc[e][0] = fmaf(__fadd_rn(blk[e][0].x, blk[e][0].y) * 4096.f, f, acc[e][0]);
+                acc[e][1] = fmaf(__fadd_rn(blk[e][1].x, blk[e][1].y) * 4096.f, f, acc[e][1]);
+                xr[e] += 8 * step[e], sr[e] += s.rows * 64, fr[e] += s.rows * 4;
+              }
+              stage_used();
+            }
+          };
+          if (n > 4) run(std::integral_constant<int, 2>());
+          else run(std::integral_constant<int, 1>());
+        }
+        if (!ok) break;
+        const int j = s.base + i;
+        if (!(ok = wait_shared_ge(done, j - kP + 1, 100))) break;
+        float2* d = reinterpret_cast<float2*>(part + (j % kP) * kPart) + lane;
+        d[0] = make_float2(acc[0][0], acc[0][1]), d[32] = make_float2(acc[1][0], acc[1][1]);
+        __threadfence_block();
+        __syncwarp();
+        if (lane == 0) atomicAdd(cnt + (j - q) % kP, 1);
+      }
+      if (ok && lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(tile_free + k)) : "memory");
+    }
+    if (!ok) *s_fail = 1;
+    if (lane == 0)  // (only after a wait that ran out: no copy is left in flight)
+      for (; consumed < issued; ++consumed) mbar_wait(mybar + consumed % NST, (consumed / NST) & 1);
+  } else if (warp == kStreamW) {
+    // ---- the joining warp: a unit's tasks in ascending k, then SwiGLU or the picks' outputs -----------------------------------
+    bool ok = true;
+    for (int k = 0; ok; ++k) {
+      if (k >= nb_first) {
+        if (k == nb_first && !mbar_wait(tabbar, 0, 64)) ok = false;
+        if (!ok || *s_fail || k >= *s_nseg) break;
+      }
+      const Seg s = segs[k];
+      const int Q = s.down ? QI : QH;
+      int reported = 0;
+      for (int i = 0; i < s.n && ok; ++i) {
+        const int j = s.base + i * Q;
+        int* c = cnt + j % kP;
+        if (!(ok = wait_shared_ge(c, Q, 40))) break;
+        float2 v[2];
+        for (int q = 0; q < Q; ++q) {
+          const float2* d = reinterpret_cast<const float2*>(part + ((j + q) % kP) * kPart) + lane;
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            v[e] = q == 0 ? d[32 * e] : make_float2(__fadd_rn(v[e].x, d[32 * e].x), __fadd_rn(v[e].y, d[32 * e].y));
+        }
+        __syncwarp();
+        if (lane == 0) {
+          *c = 0;
+          st_shared_release(done, j + Q);
+        }
+        const int u = s.u0 + i;
+        if (s.down) {
+          const int n = s.slot == kShared ? p.M : tab.ent[s.slot].n;
+          float* y = p.y + ((size_t)s.slot * kMaxRows + t) * p.H + 16 * u + g;
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (4 * e + t < n) y[(size_t)4 * e * p.H] = v[e].x, y[(size_t)4 * e * p.H + 8] = v[e].y;
+          continue;
+        }
+        const int slot = s.slot == kShared ? kShared : u / upp, ch = (s.slot == kShared ? u : u % upp) * 8;
+        const int n = slot == kShared ? p.M : tab.ent[slot].n;
+        __nv_bfloat16* h = p.h + ((size_t)slot * kMaxRows + t) * p.I + ch;
+        if (slot == kShared && p.sh_bgu) {
+          // interleaved rows: strip rows 2 i and 2 i + 1 are gate and up of a channel (first strip: channels 0-3, second: 4-7)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float ua = __shfl_down_sync(0xffffffffu, v[e].x, 4), ub = __shfl_down_sync(0xffffffffu, v[e].y, 4);
+            if (!(g & 1) && 4 * e + t < n) {
+              h[(size_t)4 * e * p.I + (g >> 1)] = __float2bfloat16_rn(__fmul_rn(silu(v[e].x), ua));
+              h[(size_t)4 * e * p.I + 4 + (g >> 1)] = __float2bfloat16_rn(__fmul_rn(silu(v[e].y), ub));
+            }
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (4 * e + t < n) h[(size_t)4 * e * p.I + g] = __float2bfloat16_rn(__fmul_rn(silu(v[e].x), v[e].y));
+        }
+        // the run's units of a slot are reported together: h is read when all of the slot's are there
+        if (i + 1 == s.n || (s.slot != kShared && (u + 1) / upp != slot)) {
+          __threadfence();
+          __syncwarp();
+          if (lane == 0) atomicAdd(&sy->cnt_h[slot], i + 1 - reported);
+          reported = i + 1;
+        }
+      }
+    }
+    if (ok && !*s_fail) {
+      __threadfence();
+      __syncwarp();
+      if (lane == 0) atomicAdd(&sy->cnt_done, 1);
+    } else {
+      *s_fail = 1;
+    }
+  } else {
+    // ---- the staging warps: the table, then every segment's activations ---------------------------------------------------------
+    const int sw = warp - kStageW0;
+    bool ok = true;
+    for (int k = 0; ok; ++k) {
+      if (k == nb_first) {
+        if (sw == 0) {  // the table, and from it this CTA's segments
+          int got = 0;
+          if (lane == 0) got = !*s_fail && poll_ge(&sy->tab_ready, 1);
+          got = __shfl_sync(0xffffffffu, got, 0);
+          if (got) {
+            for (int i = lane; i < (int)(sizeof(BlockTab) / 16); i += 32)
+              reinterpret_cast<uint4*>(&tab)[i] = __ldcg(reinterpret_cast<const uint4*>(p.tab) + i);
+            __syncwarp();
+            if (lane == 0) {
+              const long long cI = p.b16 ? 4 * kHBlk : kQBlk, cS = 4 * kHBlk;  // (costs of 8 rows x 512 k)
+              int nseg = nb_first, base = (a1 - a0) * QH;
+              const int NU = tab.nslots * upp, nsh = has_sh ? upp : 0;
+              const int u0 = routed_begin(cta, NU, cI, nsh, cS, Gs, G), u1 = routed_begin(cta + 1, NU, cI, nsh, cS, Gs, G);
+              if (u1 > u0) segs[nseg++] = Seg{0, p.b16, 0, p.M, u0, u1 - u0, (u1 - u0) * QH, base}, base += (u1 - u0) * QH;
+              const int nd = has_sh ? NT : 0, s0 = shared_begin(cta, nd, G), s1 = shared_begin(cta + 1, nd, G);
+              if (s1 > s0) segs[nseg++] = Seg{1, 1, kShared, p.M, s0, s1 - s0, (s1 - s0) * QI, base}, base += (s1 - s0) * QI;
+              const int ND = tab.nslots * NT, d0 = routed_begin(cta, ND, cI, nd, cS, G, G), d1 = routed_begin(cta + 1, ND, cI, nd, cS, G, G);
+              for (int d = d0; d < d1;) {
+                const int slot = d / NT, e = min(d1, (slot + 1) * NT);
+                segs[nseg++] = Seg{1, p.b16, slot, tab.ent[slot].n, d - slot * NT, e - d, (e - d) * QI, base}, base += (e - d) * QI;
+                d = e;
+              }
+              *s_nseg = nseg;
+            }
+            __threadfence_block();
+            __syncwarp();
+          } else {
+            *s_fail = 1;
+          }
+          __syncwarp();
+          if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(tabbar)) : "memory");
+        } else if (!mbar_wait(tabbar, 0, 64)) {
+          ok = false;
+        }
+      }
+      if (!ok || *s_fail || (k >= nb_first && k >= *s_nseg)) break;
+      const Seg s = segs[k];
+      if (k >= p.nbuf && !mbar_wait(tile_free + k - p.nbuf, 0, 20)) {
+        ok = false;
+        break;
+      }
+      const int nb = s.down ? nbI : nbH, K = s.down ? p.I : p.H;
+      if (s.down) {  // the slot's h, once all of its units are in memory
+        int got = 0;
+        if (lane == 0) got = poll_ge(&sy->cnt_h[s.slot], upp);
+        if (!(ok = __shfl_sync(0xffffffffu, got, 0) != 0)) break;
+      }
+      const Tile tile(tiles + (size_t)(k % p.nbuf) * p.tile, nb, s.rows);
+      const __nv_bfloat16* src = s.down ? p.h + (size_t)s.slot * kMaxRows * p.I : p.x;
+      const uint32_t span = s.rows * 128;
+      for (int i = sw; i < nb * s.rows; i += kStagers) {
+        const int b = i / s.rows, r = i - b * s.rows;
+        uint8_t* xt = tile.x + (size_t)b * 8 * span + r * 128;
+        if (s.b16) {
+          uint32_t w[8];
+          uint4 o[2];
+          load_16<true>(w, src + (size_t)r * K, b * 512 + 16 * lane, K, true);
+          nibble_order(o, w);
+          uint4* d = reinterpret_cast<uint4*>(xt + (size_t)(lane >> 2) * span + (lane & 3) * 32);
+          d[0] = o[0], d[1] = o[1];
+        } else {
+          stage_row<4, true>(src + (size_t)r * K, b * 512, K, true, xt, span, false, tile.sum + (size_t)b * 16 * s.rows + 2 * r, s.rows * 8,
+                             tile.scale + b * s.rows + r, lane);
+        }
+      }
+      __threadfence_block();
+      __syncwarp();
+      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(tile_full + k)) : "memory");
+    }
+    if (!ok) *s_fail = 1;
+  }
+
+  // ---- every CTA's outputs are in memory: a row's picks in ascending expert id, the shared expert, the residual, one rounding
+  __syncthreads();
+  if (threadIdx.x == 0 && !*s_fail && !poll_ge(&sy->cnt_done, G)) *s_fail = 1;
+  __syncthreads();
+  if (!*s_fail) {
+    const int H4 = p.H / 4, items = p.M * H4;
+    const int i0 = (int)((long long)items * cta / G), i1 = (int)((long long)items * (cta + 1) / G);
+    for (int i = i0 + threadIdx.x; i < i1; i += kThreads) {
+      const int m = i / H4, c = 4 * (i - m * H4);
+      float4 v[kMaxTopK], sh = make_float4(0.f, 0.f, 0.f, 0.f);
+      uint2 r = make_uint2(0u, 0u);
+#pragma unroll
+      for (int j = 0; j < kMaxTopK; ++j)
+        if (j < tab.npick) {
+          const int at = tab.pick[m][j];
+          v[j] = __ldcg(reinterpret_cast<const float4*>(p.y + ((size_t)(at & 0xff) * kMaxRows + (at >> 8)) * p.H + c));
+        }
+      if (has_sh) sh = __ldcg(reinterpret_cast<const float4*>(p.y + ((size_t)kShared * kMaxRows + m) * p.H + c));
+      if (p.res) r = *reinterpret_cast<const uint2*>(p.res + (size_t)m * p.H + c);
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int j = 0; j < kMaxTopK; ++j)
+        if (j < tab.npick) {
+          const float w = tab.w[m][j];
+          a.x = fmaf(w, v[j].x, a.x), a.y = fmaf(w, v[j].y, a.y), a.z = fmaf(w, v[j].z, a.z), a.w = fmaf(w, v[j].w, a.w);
+        }
+      a.x = __fadd_rn(__fadd_rn(a.x, sh.x), bf16_bits_to_f(r.x & 0xffffu)), a.y = __fadd_rn(__fadd_rn(a.y, sh.y), bf16_bits_to_f(r.x >> 16));
+      a.z = __fadd_rn(__fadd_rn(a.z, sh.z), bf16_bits_to_f(r.y & 0xffffu)), a.w = __fadd_rn(__fadd_rn(a.w, sh.w), bf16_bits_to_f(r.y >> 16));
+      *reinterpret_cast<uint2*>(p.out + (size_t)m * p.H + c) = pack_bf16x4(a.x, a.y, a.z, a.w);
+    }
+  }
+  if (threadIdx.x == 0 && *s_fail) atomicCAS(p.status, 0, (int)DSGX_ERR_DEVICE_WAIT);
+  // ---- the last CTA to leave resets the counters ------------------------------------------------------------------------------
+  __syncthreads();
+  if (threadIdx.x == 0) *s_tick = atomicAdd(&sy->cnt_exit, 1);
+  __syncthreads();
+  if (*s_tick == G - 1) {
+    for (int i = threadIdx.x; i < kMaxEnt + 1; i += kThreads) sy->cnt_h[i] = 0;
+    if (threadIdx.x == 0) sy->cnt_lp = 0, sy->cnt_rt = 0, sy->tab_ready = 0, sy->cnt_done = 0, sy->cnt_exit = 0;
+  }
+}
+
+template <int NST>
+size_t block_smem(size_t tile, int nbuf) {
+  return (size_t)kStreamW * NST * kStage + kP * kPart + sizeof(BlockTab) + nbuf * tile + 64 + (kStreamW * NST + 2 * kMaxSegs + 2) * 8 +
+         kMaxSegs * sizeof(Seg) + (kP + 4) * 4 + 16;
+}
+size_t block_tile(int H, int I, int M) {
+  size_t t = tile_bytes(H, M) > tile_bytes(I, M) ? tile_bytes(H, M) : tile_bytes(I, M);
+  t = t > sizeof(RouteSmem) ? t : sizeof(RouteSmem);  // (the routing's scratch before the first tile)
+  return (t + 127) & ~(size_t)127;
+}
+
+template <int NST>
+cudaError_t launch(const BlockParams& p, cudaStream_t st) {
+  static std::atomic<bool> done[64];  // (per device; two host threads may both set the attribute: harmless)
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!done[dev & 63].load(std::memory_order_acquire)) {
+    cudaError_t e = cudaFuncSetAttribute(k_block<NST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMax);
+    if (e != cudaSuccess) return e;
+    done[dev & 63].store(true, std::memory_order_release);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(sm_count()), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = block_smem<NST>(p.tile, p.nbuf), cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeCooperative, at[0].val.cooperative = 1;
+  cfg.attrs = at, cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, k_block<NST>, p);
+}
+
+size_t al256(size_t v) { return (v + 255) & ~(size_t)255; }
+
+}  // namespace
+
+size_t block_ws_bytes(int H, int I) {
+  return 256 + al256(sizeof(BlockSync)) + al256(sizeof(BlockTab)) + al256((size_t)((H + 1023) / 1024) * kMaxRows * 512 * 4) +
+         al256((size_t)(kMaxEnt + 1) * kMaxRows * I * 2) + al256((size_t)(kMaxEnt + 1) * kMaxRows * H * 4);
+}
+
+// The rows of one launch: as many of M as the activations' shared memory holds (every row's weights are streamed once a launch).
+int block_rows(int H, int I, int M) {
+  int r = M < kMaxRows ? M : kMaxRows;
+  while (r > 1 && block_smem<2>(block_tile(H, I, r), 1) > kSmemMax) r = (r + 1) / 2;
+  return block_smem<2>(block_tile(H, I, r), 1) > kSmemMax || sm_count() < 2 * kMaxRows ? 0 : r;
+}
+
+cudaError_t launch_block_int4(BlockParams p, void* ws, cudaStream_t st) {
+  char* w = reinterpret_cast<char*>(ws);
+  p.status = reinterpret_cast<int*>(w), w += 256;
+  p.sync = reinterpret_cast<BlockSync*>(w), w += al256(sizeof(BlockSync));
+  p.tab = reinterpret_cast<BlockTab*>(w), w += al256(sizeof(BlockTab));
+  p.lpart = reinterpret_cast<float*>(w), w += al256((size_t)((p.H + 1023) / 1024) * kMaxRows * 512 * 4);
+  p.h = reinterpret_cast<__nv_bfloat16*>(w), w += al256((size_t)(kMaxEnt + 1) * kMaxRows * p.I * 2);
+  p.y = reinterpret_cast<float*>(w);
+  p.tile = block_tile(p.H, p.I, p.M);
+  // two tiles (the next segment's activations are prepared while the present ones are in use) and three ring stages where
+  // they fit, in this order
+  p.nbuf = block_smem<2>(p.tile, 2) <= kSmemMax ? 2 : 1;
+  if (p.nbuf == 2 && block_smem<3>(p.tile, 2) <= kSmemMax) return launch<3>(p, st);
+  return launch<2>(p, st);
+}
+
+}  // namespace dsgx

@@ -164,6 +164,35 @@ size_t linear_bytes(int N, int K, bool glu);
 cudaError_t launch_linear_prepare(const uint8_t* w, const uint8_t* w_up, int N, int K, uint8_t* out, cudaStream_t st);
 cudaError_t launch_linear_int4(const LinearParams& p, cudaStream_t st, bool* fits);
 
+// ---- a whole INT4 or BF16 layer in one launch (block_int4.cu) -------------------------------------------------------------
+struct BlockSync;
+struct BlockTab;
+struct BlockParams {
+  int H, I, E, topk, M, b16;
+  uint32_t fmt;
+  const uint8_t* pool;
+  const dsgx_mat_desc* desc;
+  const uint8_t *sh_g, *sh_u, *sh_d, *sh_bgu;  // the bf16 shared expert (sh_d null: none; sh_bgu: gate and up interleaved)
+  RouteParams rp;
+  const float *wr, *bias;
+  const __nv_bfloat16 *x, *res;
+  __nv_bfloat16* out;
+  int* idx;
+  float* w;
+  // filled in by the launch
+  int* status;
+  BlockSync* sync;
+  BlockTab* tab;
+  float* lpart;        // [H / 1024 slices][8][E] partial router logits
+  __nv_bfloat16* h;    // [64 + 1 slots][8][I]
+  float* y;            // [64 + 1 slots][8][H]
+  size_t tile;         // bytes of an activation tile in shared memory
+  int nbuf;
+};
+size_t block_ws_bytes(int H, int I);
+int block_rows(int H, int I, int M);  // rows one launch takes (0: the shape does not fit)
+cudaError_t launch_block_int4(BlockParams p, void* ws, cudaStream_t st);
+
 // ---- prefill (FP8) ----------------------------------------------------------------------------------------------------
 struct PrefillWeights {  // K-major row-major copies of the layer's matrices, [E + 1 experts] each (index E: shared)
   uint8_t *g, *u, *d;

@@ -2,27 +2,19 @@
 // residual added, or with a second matrix silu(x W^T) * (x W_up^T).
 //
 // Bound: the weights are read once (0.578 bytes a weight), so HBM; the conversion of the nibbles in registers is the next
-// limit.  Work is cut in units of 16 output rows (SwiGLU: 8 gate + 8 up), a unit along K in 1, 2, 4 or 8 tasks, a task in
+// limit (int4_mma.cuh).  Work is cut in units of 16 output rows (SwiGLU: 8 gate + 8 up), a unit along K in 1, 2, 4 or 8 tasks, a task in
 // blocks of 16 rows x 512 k.  A CTA owns a run of units and its stream warps take the run's tasks in turn, each through a
 // private ring of bulk copies (one a block), so that every SM streams one contiguous run and the launch ends within a
 // task on every SM.  A task's sums go to shared memory; one more warp joins the tasks of a unit and writes the outputs,
 // so that the stream never waits for a reduction.
-//
-// The conversion that is left: a nibble n in the low byte of a half-word is, as it stands, the f16 subnormal n 2^-24 (bits 0-3)
-// or n 2^-20 (bits 4-7), and the MMA takes subnormals exactly, so a word of eight weights costs four ANDs and one shift and no
-// arithmetic at all.  x goes to f16 for that: per row and block of 512 k a power of two 2^E brings the largest magnitude into
-// [2^14, 2^15), where bf16's eight bits are exact down to 2^-32 of it (smaller values round at 2^-40 of the largest, far below
-// an f32 sum's last bit); values that meet a nibble in bits 4-7 are taken times 2^-4.  The zero point leaves the sum in f32:
-// sum (n - z) x = sum n x - z sum x, the second sum of a group once a row.  Whatever is infinite or NaN in a row makes the
-// whole row NaN.
 //
 // Weight layout (k_linear_prepare makes it from the experts' 8-row blocks): the blocks of a unit one after the other, 4736
 // bytes each, [8 spans of 64 k][32 lanes][four words: row g of the first strip and of the second in the span's first group of
 // 32, then both in its second], a word = the 8 nibbles k = 32 group + 8 t + 0..7 of lane 4 g + t (nibbles i and i + 4 meet in one f16 pair); [4 x 128 k][8 g][eight bf16
 // scales: (strip, group) by (first span, second span)]; [8 g][4 x 128 k][the eight zero points' nibbles in that order].
 // In the experts' blocks a lane's 16 bytes mix two groups in every MMA, so their scales have to go onto the weights (and
-// round them) or the MMAs' columns be halved (int4_pair.cuh: twice the MMAs and activation loads from five rows on); here
-// an MMA stays inside one group, its f32 sums take the scale, and all eight columns are rows of x.
+// round them) or the MMAs' columns be halved (block_int4.cu: twice the MMAs and activation loads from five rows on; 131072 x
+// 4096 and eight rows took 87 us that way, 71 this way); here an MMA stays inside one group, its f32 sums take the scale, and all eight columns are rows of x.
 //
 // K over a cluster: with C > 1 (2, 4 or 8 CTAs) the ranks of a cluster take consecutive parts of K of the same units.  The
 // activations of M rows are held in shared memory for a rank's own part only, and a matrix with few units still occupies
@@ -33,11 +25,9 @@
 // is summed in ascending order from zero, and the runs are joined as a binary tree, ((r0 + r1) + (r2 + r3)) + ((r4 + r5) + (r6 +
 // r7)), of which a task and a rank hold whole subtrees.  So a row's bits do not depend on the rows beside it or their number.
 #include <atomic>
-#include <cuda_fp16.h>
 
 #include "common.cuh"
-#include "decode_common.cuh"
-#include "int4_pair.cuh"
+#include "int4_mma.cuh"
 #include "kernels.h"
 
 namespace dsgx {
@@ -63,19 +53,6 @@ struct LinVar {
   }
   __host__ __device__ static int even(int M) { return (M + 1) & ~1; }
 };
-
-DSGX_DEV void mma_f16_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
-}
-DSGX_DEV void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 
 // The products of one block, times 2^(E - 24): blk[s] = a lane's four sums (first strip's row g with rows 8 s + 2 t and + 1 of x,
 // then the second strip's).  st: the stage; x[s], sx[s]: this lane's activations and group sums at the block's first span;
@@ -109,17 +86,14 @@ DSGX_DEV void unit_block(float (&blk)[S][4], uint32_t st, const uint32_t (&x_at)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {  // the span's two groups
         const uint32_t wa = c ? w.z : w.x, wb = c ? w.w : w.y, wa8 = wa >> 8, wb8 = wb >> 8;
-        // -z as a float: 0x4B0000zz is 2^23 + z
-        const float za = 8388608.f - __uint_as_float(__byte_perm(q ? zo : ze, 0x4B000000u, 0x7440u + 2 * c));
-        const float zb = 8388608.f - __uint_as_float(__byte_perm(q ? zo : ze, 0x4B000000u, 0x7440u + 2 * c + 1));
-        const float fa = __uint_as_float(q ? sw[2 * c] & 0xffff0000u : sw[2 * c] << 16);
-        const float fb = __uint_as_float(q ? sw[2 * c + 1] & 0xffff0000u : sw[2 * c + 1] << 16);
+        const float za = minus_zero(q ? zo : ze, 2 * c), zb = minus_zero(q ? zo : ze, 2 * c + 1);
+        const float fa = q ? scale_hi(sw[2 * c]) : scale_lo(sw[2 * c]), fb = q ? scale_hi(sw[2 * c + 1]) : scale_lo(sw[2 * c + 1]);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
           const uint4 xv = lds_v4(x[s] ^ (c ? 64u : 0u));
           float d[4];
-          mma_f16_zero(d, wa & 0x000F000Fu, wb & 0x000F000Fu, wa & 0x00F000F0u, wb & 0x00F000F0u, xv.x, xv.y);
-          mma_f16(d, wa8 & 0x000F000Fu, wb8 & 0x000F000Fu, wa8 & 0x00F000F0u, wb8 & 0x00F000F0u, xv.z, xv.w);
+          mma_f16_zero(d, wa & kNib0, wb & kNib0, wa & kNib1, wb & kNib1, xv.x, xv.y);
+          mma_f16(d, wa8 & kNib0, wb8 & kNib0, wa8 & kNib1, wb8 & kNib1, xv.z, xv.w);
           const float s0 = c ? sum[s].z : sum[s].x, s1 = c ? sum[s].w : sum[s].y;
           blk[s][0] = fmaf(fa, fmaf(za, s0, d[0]), blk[s][0]), blk[s][1] = fmaf(fa, fmaf(za, s1, d[1]), blk[s][1]);
           blk[s][2] = fmaf(fb, fmaf(zb, s0, d[2]), blk[s][2]), blk[s][3] = fmaf(fb, fmaf(zb, s1, d[3]), blk[s][3]);
@@ -129,54 +103,6 @@ DSGX_DEV void unit_block(float (&blk)[S][4], uint32_t st, const uint32_t (&x_at)
       for (int s = 0; s < S; ++s) x[s] += span, sx[s] += sspan;
     }
   }
-}
-
-// One row's 512 k of a block into the tile, by one warp (16 k a lane): f16 times 2^E, the groups' sums times 2^(E - 24), and
-// 2^(12 - E).  xt: the row's line in the block's first span; sx: its first group's sum; odd: the row's place among the lines.
-DSGX_DEV void stage_row(const __nv_bfloat16* row, int k0, int K, bool vec, uint8_t* xt, uint32_t span, bool odd, float* sx, uint32_t sspan,
-                        float* scale, int lane) {
-  const int k = k0 + 16 * lane;
-  uint32_t w[8];
-  if (vec && k + 16 <= K) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(row + k)), b = __ldg(reinterpret_cast<const uint4*>(row + k + 8));
-    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
-  } else {
-    const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t lo = k + 2 * i < K ? p[k + 2 * i] : 0u, hi = k + 2 * i + 1 < K ? p[k + 2 * i + 1] : 0u;
-      w[i] = lo | hi << 16;
-    }
-  }
-  uint32_t top = 0;  // the largest finite magnitude's bits
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t lo = w[i] & 0x7FFFu, hi = w[i] >> 16 & 0x7FFFu;
-    top = max(top, max(lo < 0x7F80u ? lo : 0u, hi < 0x7F80u ? hi : 0u));
-  }
-  top = __reduce_max_sync(0xffffffffu, top);
-  const int E = top >= 0x80u ? min(14 + 127 - (int)(top >> 7), 126) : 126;  // (subnormal or zero: as small as it gets)
-  const float even = __uint_as_float((uint32_t)(E + 127) << 23), off = __uint_as_float((uint32_t)(E - 4 + 127) << 23);
-  uint32_t h[8];
-  float sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const __half lo = __float2half_rn(bf16_bits_to_f(w[i] & 0xffffu) * even), hi = __float2half_rn(bf16_bits_to_f(w[i] >> 16) * off);
-    sum = __fadd_rn(__fadd_rn(sum, __half2float(lo)), __half2float(hi) * 16.f);
-    h[i] = (uint32_t)__half_as_ushort(lo) | (uint32_t)__half_as_ushort(hi) << 16;
-  }
-  sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, 1));
-  uint4 o[2];  // words (v0 v1)(v2 v3)(v4 v5)(v6 v7) -> (v0 v4)(v1 v5)(v2 v6)(v3 v7)
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    uint32_t* d = &o[j].x;
-    d[0] = __byte_perm(h[4 * j], h[4 * j + 2], 0x5410), d[1] = __byte_perm(h[4 * j], h[4 * j + 2], 0x7632);
-    d[2] = __byte_perm(h[4 * j + 1], h[4 * j + 3], 0x5410), d[3] = __byte_perm(h[4 * j + 1], h[4 * j + 3], 0x7632);
-  }
-  uint4* d = reinterpret_cast<uint4*>(xt + (size_t)(lane >> 2) * span + (((lane & 3) * 32) ^ (odd ? 64 : 0)));
-  d[0] = o[0], d[1] = o[1];
-  if (!(lane & 1)) *reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(sx) + (size_t)(lane >> 2) * sspan + 8 * (lane >> 1 & 1)) = sum * 0x1p-24f;
-  if (lane == 0) *scale = __uint_as_float((uint32_t)(12 - E + 127) << 23);
 }
 
 // ---- the weights' own layout, once at load ------------------------------------------------------------------------------
@@ -249,23 +175,9 @@ DSGX_DEV bool mbar_wait_cluster(uint64_t* bar, uint32_t parity) {
     if (clock64() - t0 > kWaitCycles) return false;
   }
 }
-DSGX_DEV float2 lds_f2(uint32_t a) {
-  float2 v;
-  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a));
-  return v;
-}
 DSGX_DEV float4 add4(float4 a, float4 b) {
   return make_float4(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y), __fadd_rn(a.z, b.z), __fadd_rn(a.w, b.w));
 }
-DSGX_DEV int ld_shared_acquire(const int* p) {
-  int v;
-  asm volatile("ld.acquire.cta.shared::cta.s32 %0, [%1];" : "=r"(v) : "r"(smem_u32(p)) : "memory");
-  return v;
-}
-DSGX_DEV void st_shared_release(int* p, int v) {
-  asm volatile("st.release.cta.shared::cta.s32 [%0], %1;" ::"r"(smem_u32(p)), "r"(v) : "memory");
-}
-
 template <class V>
 __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearParams p) {
   constexpr int S = V::S, W = V::W, NST = V::NST, P = V::P, kPart = V::kPart;
@@ -344,7 +256,7 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
   const uint32_t span = p.M * 128, sspan = Me * 8;
   for (int i = warp; i < nbk * p.M; i += W + 1) {
     const int b = i / p.M, r = i - b * p.M;
-    stage_row(p.x + (size_t)r * p.ldx, (b0 + b) * 512, p.K, p.x_vec != 0, xt + (size_t)b * 8 * span + r * 128, span, r & 1,
+    stage_row<8, false>(p.x + (size_t)r * p.ldx, (b0 + b) * 512, p.K, p.x_vec != 0, xt + (size_t)b * 8 * span + r * 128, span, r & 1,
               xsum + (size_t)b * 16 * Me + (r >> 1) * 4 + (r & 1), sspan, xscale + b * Me + r, lane);
   }
   __syncthreads();
@@ -421,13 +333,7 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
         }
       }
       // the sums into the partial buffer, once the unit that had the place has been added up
-      if (ok && j >= ld_shared_acquire(done) + P) {
-        const long long t0 = clock64();
-        while (ok && j >= ld_shared_acquire(done) + P) {
-          __nanosleep(100);
-          ok = clock64() - t0 < kWaitCycles;
-        }
-      }
+      if (ok) ok = wait_shared_ge(done, j - P + 1, 100);
       if (!ok) break;
       float4* d = reinterpret_cast<float4*>(part + (size_t)(j & (P - 1)) * kPart) + lane;
 #pragma unroll
@@ -483,14 +389,7 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
     for (int i = 0; i < n + lag && ok; ++i) {
       if (i < n) {
         int* c = cnt + (i & (P - 1));
-        if (ld_shared_acquire(c) < Q) {
-          const long long t0 = clock64();
-          while (ok && ld_shared_acquire(c) < Q) {
-            __nanosleep(40);
-            ok = clock64() - t0 < kWaitCycles;
-          }
-          if (!ok) break;
-        }
+        if (!(ok = wait_shared_ge(c, Q, 40))) break;
         join(reinterpret_cast<const float4*>(part + (size_t)((i << lq) & (P - 1)) * kPart) + lane, Q);
         __syncwarp();
         if (lane == 0) {

@@ -178,6 +178,38 @@ class LayerStep:
         return out_host
 
 
+class MoeBlock:
+    """A whole INT4 or BF16 layer for 1..16 rows in one launch (dsgx_moe_block_decode): out = res + MoE(x)."""
+
+    def __init__(self, shp, wr, bias=None, device="cuda"):
+        n = lib().dsgx_moe_block_ws_bytes(C.byref(shp))
+        if n == 0:
+            raise _lib.DsgxError(_lib.ERR_SHAPE, "dsgx_moe_block_ws_bytes")
+        self.shp, self.wr, self.bias = shp, wr, bias
+        self.device = torch.device(device, torch.cuda.current_device()) if torch.device(device).index is None else torch.device(device)
+        for t, shape, what in ((wr, (shp.E, shp.H), "wr"), (bias, (shp.E,), "bias")):
+            if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != self.device):
+                raise ValueError(f"MoeBlock: {what} must be contiguous f32 {shape} on {self.device}")
+        self.idx = torch.empty(_lib.MAX_STEP_ROWS, shp.topk, dtype=torch.int32, device=self.device)
+        self.w = torch.empty(_lib.MAX_STEP_ROWS, shp.topk, dtype=torch.float32, device=self.device)
+        self.ws = torch.zeros(n, dtype=torch.uint8, device=self.device)
+        self.c = _lib.MoeBlock(_ptr(wr), _ptr(bias), _ptr(self.idx), _ptr(self.w), _ptr(self.ws), None)
+
+    def run(self, layer_w, x, res=None, out=None):
+        """x, res: contiguous bf16 [M][H] -> (out bf16 [M][H], idx int32 [M][topk], w f32 [M][topk]); idx and w are this
+        object's buffers, overwritten by the next run.  out may be x or res."""
+        M = x.shape[0]
+        if out is None:
+            out = torch.empty_like(x)
+        for t, what in ((x, "x"), (res, "res"), (out, "out")):
+            if t is not None and (t.dtype != torch.bfloat16 or tuple(t.shape) != (M, self.shp.H) or not t.is_contiguous() or t.device != self.device):
+                raise ValueError(f"MoeBlock: {what} must be contiguous bf16 [M][{self.shp.H}] on {self.device}")
+        with torch.cuda.device(self.device):
+            check(lib().dsgx_moe_block_decode(C.byref(self.shp), C.byref(layer_w), _ptr(x), M, C.byref(self.c), _ptr(res), _ptr(out),
+                                              torch.cuda.current_stream(self.device).cuda_stream), "dsgx_moe_block_decode")
+        return out, self.idx[:M], self.w[:M]
+
+
 def prefill_view(shp, ws, T):
     v = _lib.PrefillView()
     check(lib().dsgx_prefill_view_of(C.byref(shp), _ptr(ws), T, C.byref(v)), "dsgx_prefill_view_of")

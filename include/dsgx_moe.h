@@ -309,6 +309,35 @@ int dsgx_moe_layer_decode(const dsgx_moe_shape* shape, const dsgx_layer_w* L, co
 int dsgx_moe_layer_decode_host(const dsgx_moe_shape* shape, const dsgx_layer_w* L, const void* x_host, int M,
                                const dsgx_layer_step* step, void* out_host, void* stream);
 
+/* ---- a whole INT4 layer in one launch (1..DSGX_MAX_STEP_ROWS rows) -----------------------------------------------------
+ * out = bf16(res + MoE(x)) of an INT4-g32 or BF16 layer (DSGX_FMT_INT4, DSGX_FMT_BF16; the bf16 shared expert in either form of
+ * dsgx_shared_w, or none): router logits, selection, the picked experts, the weighted sum, the residual, in ONE kernel.
+ * dsgx_moe_layer_decode runs the same layer as four launches with f32 partial sums for other GPUs; this call is the whole
+ * layer on one GPU (e_lo = 0, e_hi = E; otherwise DSGX_ERR_UNSUPPORTED).
+ *   idx, w: the picks, bit for bit dsgx_route's of dsgx_router_logits.
+ *   The experts: W = (u - z) s unrounded, gate, up and the down sums in f32, h = bf16(silu(g) u), out_r = sum of w_e y_e in
+ *   ascending expert id, then the shared expert, then the residual, one rounding.  (The four launches round W, g and u to bf16 as
+ *   altar-1 does, so the two agree within those roundings, not bit for bit.)
+ * A row's bits depend neither on the other rows nor on their number, and are the same run after run.  Only the rows that
+ * picked an expert are computed for it.  Up to eight rows are one launch (fewer where H or I is so large that their
+ * activations do not fit shared memory: 8192 and eight rows take two), more follow in stream order.
+ * x, res (may be null), out: bf16 [M][H]; out may be x or res.  ws: dsgx_moe_block_ws_bytes(shape) bytes, zeroed once; the
+ * kernel leaves its counters at zero.  Its first word is the status (dsgx_ws_status): a descriptor of another format gives
+ * DSGX_ERR_FORMAT and leaves the routed experts out; a bounded wait that ran out gives DSGX_ERR_DEVICE_WAIT and no output.
+ * The CTAs (one a SM) wait for one another, so the launch is cooperative: it starts when all of them fit, and it can be
+ * captured into a graph.  Calls that share a workspace must not overlap. */
+typedef struct dsgx_moe_block {
+  const float* wr;   /* router weights f32 [E][H] */
+  const float* bias; /* selection bias f32 [E] or null */
+  int32_t* idx;      /* out: [M][topk] */
+  float* w;          /* out: [M][topk] */
+  void* ws;
+  void* reserved;
+} dsgx_moe_block;
+size_t dsgx_moe_block_ws_bytes(const dsgx_moe_shape* shape);
+int dsgx_moe_block_decode(const dsgx_moe_shape* shape, const dsgx_layer_w* L, const void* x_bf16, int M, const dsgx_moe_block* block,
+                          const void* res_bf16, void* out_bf16, void* stream);
+
 /* ---- dense products with 4-bit weights (1..DSGX_MAX_STEP_ROWS rows) ---------------------------------------------------
  * out[m][n] = sum_k x[m][k] W[n][k], W[n][k] = (u - z) s of an INT4-g32 matrix: the projections, dense FFN layers and heads of
  * a model whose experts this library runs; stands in for the engines' weight-streaming GEMV over INT4 weights (altar1

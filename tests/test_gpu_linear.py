@@ -1,10 +1,12 @@
 """The dense INT4 products (dsgx_linear_decode) against the formula in 64 bits.
 
-Tolerance, by arithmetic.  A product x (u - z) has at most 8 + 4 significant bits: exact in f32.  A group's sum is two MMAs of 16
-products, each adding with at most one truncation (2^-23 of the running magnitude) a product and one for its accumulator: 34;
-a fused multiply-add a group (16 in a block of 512, 2 nb in a run's nb / 8 blocks) and the runs' three levels round by 2^-24
-each.  So |y - exact| <= GAMMA A with A = sum |x| |W| and GAMMA = (34 + 8 + nb + 2) 2^-23 < (80 + nb) 2^-23; the one
-rounding of the output adds 2^-8 |y| (bf16) or 2^-24 |y| (f32)."""
+Tolerance, by arithmetic.  The kernel forms sum u x and z sum x of every group of 32 apart and subtracts.  A product u x has at
+most 4 + 8 significant bits: exact.  sum u x is two MMAs of 16 products, each adding with at most one truncation (2^-23 of
+the running magnitude) a product and one for its accumulator: 34; sum x is 32 adds of 2^-24, times z and into the difference
+by one fused multiply-add: 17 x 2^-23; the scale by another one; 16 groups a block and at most nb / 8 + 1 blocks a run in
+sequence, the runs' three levels, each 2^-24.  So |y - exact| <= GAMMA A with A = sum |x| (u + z) s and
+GAMMA = (34 + 17 + 8 + nb / 16 + 3) 2^-23 < (80 + nb) 2^-23; the one rounding of the output adds 2^-8 |y| (bf16) or 2^-24 |y| (f32).
+(x in f16 with its block's power of two is exact for these inputs: none is below 2^-32 of its block's largest.)"""
 import numpy as np
 import pytest
 
@@ -15,8 +17,8 @@ pytestmark = pytest.mark.gpu
 def _make(N, K, seed, zeros=True):
     from dsgx10_b200 import weights
     from tests.linear_util import random_int4
-    wp, s, zp, w = random_int4(N, K, seed, zeros)
-    return torch.from_numpy(weights.pack_linear_int4(wp, s, zp, K=K)).cuda(), torch.from_numpy(w)
+    wp, s, zp, w, bound = random_int4(N, K, seed, zeros)
+    return torch.from_numpy(weights.pack_linear_int4(wp, s, zp, K=K)).cuda(), torch.from_numpy(w), torch.from_numpy(bound)
 
 
 def _x(M, K, seed):
@@ -42,12 +44,12 @@ SHAPES = [(1, 1, 1), (1, 8, 512), (2, 9, 513), (3, 17, 31), (4, 16, 32), (1, 33,
 @pytest.mark.parametrize("f32", [False, True])
 def test_product(M, N, K, f32):
     from dsgx10_b200 import linear
-    blocks, w = _make(N, K, 11 * N + K)
+    blocks, w, wb = _make(N, K, 11 * N + K)
     x = _x(M, K, M + K)
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
     got = linear.linear_decode(linear.LinearW(N, K, blocks), x.cuda(), out_dtype=torch.float32 if f32 else torch.bfloat16, status=status)
     assert int(status) == 0
-    _check(got, x.double() @ w.T, x.double().abs() @ w.abs().T, K)
+    _check(got, x.double() @ w.T, x.double().abs() @ wb.T, K)
 
 
 @pytest.mark.parametrize("M,N,K", [(1, 7, 40), (4, 1000, 1024), (6, 129, 3000), (16, 520, 5120), (1, 9000, 2048)])
@@ -55,11 +57,11 @@ def test_swiglu(M, N, K):
     """h = silu(g) u: an error dg moves silu by at most 1.1 dg (its slope is below 1.1); expf, the division and the product
     are within 8 x 2^-24 of the value."""
     from dsgx10_b200 import linear
-    (bg, wg), (bu, wu) = _make(N, K, 5), _make(N, K, 6, zeros=False)
+    (bg, wg, bwg), (bu, wu, bwu) = _make(N, K, 5), _make(N, K, 6, zeros=False)
     x = _x(M, K, 3)
     got = linear.linear_decode(linear.LinearW(N, K, bg, up=bu), x.cuda())
     g, u = x.double() @ wg.T, x.double() @ wu.T
-    dg, du = (_gamma(K) * (x.double().abs() @ w.abs().T) for w in (wg, wu))
+    dg, du = (_gamma(K) * (x.double().abs() @ w.T) for w in (bwg, bwu))
     act = g * torch.sigmoid(g)
     h = act * u
     _check(got, h, 0 * h, K, extra=1.1 * dg * (u.abs() + du) + act.abs() * du + h.abs() * 8 * 2.0 ** -24)
@@ -70,12 +72,12 @@ def test_residual_and_in_place(f32):
     """One rounding after the residual's add (which rounds once more in f32: 2^-24 of the sum)."""
     from dsgx10_b200 import linear
     M, N, K = 5, 333, 1500
-    blocks, w = _make(N, K, 21)
+    blocks, w, wb = _make(N, K, 21)
     x, res = _x(M, K, 22), _x(M, N, 23)
     lw = linear.LinearW(N, K, blocks)
     y = x.double() @ w.T + res.double()
     got = linear.linear_decode(lw, x.cuda(), res=res.cuda(), out_dtype=torch.float32 if f32 else torch.bfloat16)
-    _check(got, y, x.double().abs() @ w.abs().T, K, extra=2.0 ** -24 * y.abs())
+    _check(got, y, x.double().abs() @ wb.T, K, extra=2.0 ** -24 * y.abs())
     if not f32:
         r = res.cuda()
         assert linear.linear_decode(lw, x.cuda(), res=r, out=r) is r and torch.equal(r, got)
@@ -85,7 +87,7 @@ def test_rows_do_not_depend_on_each_other():
     """A row alone, among four, eight or sixteen (another kernel, another split of K): the same bits; twice: the same bits."""
     from dsgx10_b200 import linear
     for N, K in ((500, 6144), (2000, 1111), (16, 9000)):
-        blocks, _ = _make(N, K, N)
+        blocks, _, _ = _make(N, K, N)
         lw = linear.LinearW(N, K, blocks)
         x = _x(16, K, K).cuda()
         all16 = linear.linear_decode(lw, x, out_dtype=torch.float32)
@@ -97,7 +99,7 @@ def test_rows_do_not_depend_on_each_other():
 def test_inf_and_nan_stay_in_their_row():
     from dsgx10_b200 import linear
     N, K = 200, 1030
-    blocks, _ = _make(N, K, 41)
+    blocks, _, _ = _make(N, K, 41)
     lw = linear.LinearW(N, K, blocks)
     for M in (2, 7, 12):
         x = _x(M, K, 42).cuda()
@@ -114,7 +116,7 @@ def test_strided_and_unaligned_rows():
     outside the rows is written."""
     from dsgx10_b200 import linear
     M, N, K = 6, 77, 1001
-    blocks, _ = _make(N, K, 51)
+    blocks, _, _ = _make(N, K, 51)
     lw = linear.LinearW(N, K, blocks)
     x, res = _x(M, K, 52).cuda(), _x(M, N, 53).cuda()
     want = linear.linear_decode(lw, x, res=res)
@@ -165,7 +167,7 @@ def test_streams_and_graph():
 def test_python_refusals():
     from dsgx10_b200 import linear
     N, K = 64, 700
-    blocks, _ = _make(N, K, 81)
+    blocks, _, _ = _make(N, K, 81)
     lw = linear.LinearW(N, K, blocks)
     x = _x(2, K, 82).cuda()
     for bad in (x.float(), x[:, :-1], x.cpu(), x[0], _x(17, K, 1).cuda(), torch.empty(K, 2, dtype=torch.bfloat16, device="cuda").T,
