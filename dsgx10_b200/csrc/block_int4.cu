@@ -26,6 +26,7 @@
 // The expert's input rows and h are f16 with a power of two a 512-k block; gate, up and the down sums stay f32; h is rounded to
 // bf16 once, because it is an MMA operand (2^-9 of its value; a second half would double the down products' MMAs).
 #include <atomic>
+#include <cstddef>
 #include <type_traits>
 
 #include "common.cuh"
@@ -47,9 +48,9 @@ struct alignas(16) BlockEnt {
 };
 struct alignas(16) BlockTab {
   int nslots, bad, npick, pad;
-  BlockEnt ent[kMaxEnt];
   int pick[kMaxRows][kMaxTopK];   // a row's picks in ascending expert id: slot | its place among the slot's rows << 8
   float w[kMaxRows][kMaxTopK];
+  BlockEnt ent[kMaxEnt];          // (last: only as many as the step can have picked are read)
 };
 static_assert(sizeof(BlockEnt) == 48 && sizeof(BlockTab) % 16 == 0, "copied in 16-byte pieces");
 
@@ -67,6 +68,17 @@ constexpr int kPart = 512;               // bytes of a task's sums: [2 sets][32 
 constexpr int kShared = kMaxEnt;         // the shared expert's place among the h, y and counters
 constexpr int kMaxSegs = kMaxEnt + 4;
 constexpr size_t kSmemMax = 227 * 1024;
+
+// bounded poll until *p >= target (decode_common.cuh's poll_ge with a shorter sleep: these waits are on the critical path)
+DSGX_DEV bool poll_near(const int* p, int target) {
+  if (ld_acquire(p) >= target) return true;
+  const long long t0 = clock64();
+  while (ld_acquire(p) < target) {
+    __nanosleep(32);
+    if (clock64() - t0 > kWaitCycles) return false;
+  }
+  return true;
+}
 
 // A CTA's run of units of one phase.
 struct Seg {
@@ -146,65 +158,77 @@ DSGX_DEV void pair_b16(float (&d)[4], uint32_t st, uint32_t x, uint32_t span, in
 }
 
 // ---- the division of a phase's units over the CTAs.  n shared units of cost cs over the first Gs CTAs, N routed ones of cost c so
-// that every CTA's total is alike: where CTA i's routed run begins.
-DSGX_DEV int shared_begin(int i, int n, int Gs) { return (int)((long long)n * min(i, Gs) / Gs); }
-DSGX_DEV int routed_begin(int i, int N, long long c, int n, long long cs, int Gs, int G) {
+// that every CTA's total is alike (a CTA behind Gs routes meanwhile: it counts like the others' average): where CTA i's
+// routed run begins.
+DSGX_DEV int shared_begin(int i, int n, int Gs) { return (int)((unsigned)(n * min(i, Gs)) / (unsigned)Gs); }
+DSGX_DEV int routed_begin(int i, int N, int c, int n, int cs, int Gs, int G) {
   if (i <= 0) return 0;
   if (i >= G) return N;
-  const long long total = N * c + n * cs;
-  if (total / G < cs * ((n + Gs - 1) / Gs + 1)) return (int)((long long)N * i / G);  // (few routed units: an even deal)
-  const long long before = total * i / G - cs * shared_begin(i, n, Gs);
+  const long long avg = (long long)n * cs / Gs, total = (long long)N * c + (long long)n * cs + (G - Gs) * avg;
+  if (total < (long long)G * cs * ((n + Gs - 1) / Gs + 1)) return (int)((long long)N * i / G);  // (few routed units: an even deal)
+  const long long before = total * i / G - (long long)cs * shared_begin(i, n, Gs) - max(0, i - Gs) * avg;
   return (int)min((long long)N, max(0ll, before / c));
 }
 
-// ---- the table, by one whole CTA; scratch: 16 + 2 x kMaxEnt words of shared memory --------------------------------------------
-DSGX_DEV void build_block_tab(BlockTab& tab, uint32_t* scratch, const int* idx, const float* w, const BlockParams& p) {
-  uint32_t *bm = scratch, *mask = scratch + 16;
-  int* id = reinterpret_cast<int*>(mask + kMaxEnt);
-  const int tid = threadIdx.x, np = p.M * p.topk;
-  if (tid < 16) bm[tid] = 0;
-  if (tid < kMaxEnt) mask[tid] = 0;
-  if (tid == 0) tab.bad = 0;
-  __syncthreads();
-  auto known = [&](int e) { return e >= 0 && e < p.E; };
-  auto rank_of = [&](int e) {
-    int r = __popc(bm[e >> 5] & ((1u << (e & 31)) - 1u));
-    for (int k = 0; k < (e >> 5); ++k) r += __popc(bm[k]);
-    return r;
-  };
-  if (tid < np && known(idx[tid])) atomicOr(&bm[idx[tid] >> 5], 1u << (idx[tid] & 31));
-  if (tid < np && !known(idx[tid])) tab.bad = DSGX_ERR_ARG;
-  __syncthreads();
-  int slot = 0;
-  if (tid < np && known(idx[tid])) {
-    slot = rank_of(idx[tid]);
-    atomicOr(&mask[slot], 1u << (tid / p.topk));
-    id[slot] = idx[tid];
+// ---- the table, by the first 64 threads of a CTA, a thread a pick, written straight to global memory.  s_idx, s_first: kMaxEnt
+// words of shared memory each.
+DSGX_DEV void build_block_tab(BlockTab* out, int* s_idx, int* s_first, const BlockParams& p) {
+  constexpr int kNone = 0x7fffffff;
+  const int i = threadIdx.x, np = p.M * p.topk;
+  const bool in = i < np;
+  int e = in ? __ldcg(p.idx + i) : kNone;
+  const float w = in ? __ldcg(p.w + i) : 0.f;
+  const bool bad_id = in && (e < 0 || e >= p.E);
+  if (bad_id) e = kNone;
+  uint4 d[3];  // off, s2, fmt of the expert's three descriptors
+  if (e != kNone)
+#pragma unroll
+    for (int m = 0; m < 3; ++m) d[m] = __ldg(reinterpret_cast<const uint4*>(p.desc + (size_t)e * 3 + m));
+  s_idx[i] = e;
+  asm volatile("bar.sync 3, 64;" ::: "memory");
+  bool first = e != kNone;
+  uint32_t mask = 0;  // the rows that picked the expert
+  const int row = i / p.topk;
+  int place = 0, r = 0, c = 0;  // the pick's place in its row's ascending order
+  for (int j = 0; j < np; ++j) {
+    const int o = s_idx[j];
+    if (o == e) mask |= 1u << r, first = first && j >= i;
+    if (r == row) place += o < e;
+    if (++c == p.topk) c = 0, ++r;
   }
-  __syncthreads();
-  int n = 0;
-  for (int k = 0; k < 16; ++k) n += __popc(bm[k]);
-  if (tid < n) {
-    const dsgx_mat_desc* d = p.desc + (size_t)id[tid] * 3;
-    BlockEnt& e = tab.ent[tid];
-    if (d[0].fmt != p.fmt || d[1].fmt != p.fmt || d[2].fmt != p.fmt) tab.bad = DSGX_ERR_FORMAT;
-    e.g = p.pool + d[0].off, e.u = p.pool + d[1].off, e.d = p.pool + d[2].off;
-    unsigned long long rows = 0;
-    int c = 0;
-    for (int r = 0; r < kMaxRows; ++r)
-      if (mask[tid] >> r & 1) rows |= (unsigned long long)r << (8 * c++);
-    e.rows = rows, e.n = c;
+  s_first[i] = first ? e : kNone;
+  asm volatile("bar.sync 3, 64;" ::: "memory");
+  int slot = 0, n = 0;
+  for (int j = 0; j < np; ++j) {
+    const int o = s_first[j];
+    slot += o < e, n += o != kNone;
   }
-  if (tid < np && known(idx[tid])) {
-    const int m = tid / p.topk;
-    int place = 0;  // among the row's picks, ascending expert id
-    for (int j = 0; j < p.topk; ++j) place += idx[m * p.topk + j] < idx[tid];
-    tab.pick[m][place] = slot | __popc(mask[slot] & ((1u << m) - 1u)) << 8;
-    tab.w[m][place] = w[tid];
+  int bad = bad_id ? DSGX_ERR_ARG : 0;
+  if (first) {
+    if (d[0].w != p.fmt || d[1].w != p.fmt || d[2].w != p.fmt) bad = DSGX_ERR_FORMAT;
+    BlockEnt en;
+    en.g = p.pool + ((uint64_t)d[0].x | (uint64_t)d[0].y << 32), en.u = p.pool + ((uint64_t)d[1].x | (uint64_t)d[1].y << 32);
+    en.d = p.pool + ((uint64_t)d[2].x | (uint64_t)d[2].y << 32);
+    en.rows = 0, en.n = 0, en.pad[0] = en.pad[1] = en.pad[2] = 0;
+#pragma unroll
+    for (int q = 0; q < kMaxRows; ++q)
+      if (mask >> q & 1) en.rows |= (unsigned long long)q << (8 * en.n++);
+    out->ent[slot] = en;
   }
-  __syncthreads();
-  if (tid == 0) tab.nslots = tab.bad ? 0 : n, tab.npick = tab.bad ? 0 : p.topk;
-  __syncthreads();
+  if (in) {
+    out->pick[row][place] = slot | __popc(mask & ((1u << row) - 1u)) << 8;
+    out->w[row][place] = w;
+  }
+  s_idx[i] = bad;  // (read as picks only before the barrier above)
+  __threadfence();
+  asm volatile("bar.sync 3, 64;" ::: "memory");
+  if (i == 0) {
+    for (int j = 0; j < np; ++j) bad = bad ? bad : s_idx[j];
+    if (bad) atomicCAS(p.status, 0, bad);
+    out->nslots = bad ? 0 : n, out->npick = bad ? 0 : p.topk;
+    __threadfence();
+    atomicExch(&p.sync->tab_ready, 1);
+  }
 }
 
 template <int NST>
@@ -249,43 +273,101 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const BlockParams p) {
   mbar_fence_init();
   __syncthreads();
 
+  // ---- stream warps: the producer's state (lane 0): segment, task, block, quarter of a bf16 block
+  const int nb_first = a1 > a0 ? 1 : 0;  // segments whose units are known without the table
+  uint8_t* myring = ring + (size_t)warp * NST * kStage;
+  uint64_t* mybar = bars + warp * NST;
+  const uint64_t pol = policy_evict_first();
+  uint32_t issued = 0, consumed = 0;
+  int nknown = nb_first, ps = 0, pt = -1, pb = 0, pe = 0, pc = 0;
+  bool all_known = false;
+  const uint8_t *pa = nullptr, *pz = nullptr;
+  auto first_task = [&](const Seg& s) { return (int)((unsigned)(warp + kStreamW - s.base % kStreamW) % kStreamW); };
+  auto open_task = [&]() {
+    while (pb == pe) {
+      if (ps >= nknown) {
+        if (!all_known && mbar_test_wait(tabbar, 0)) all_known = true, nknown = *s_nseg;
+        if (ps >= nknown) return false;
+      }
+      const Seg& s = segs[ps];
+      if (pt < 0) pt = first_task(s);
+      if (pt >= s.tasks) {
+        ++ps, pt = -1;
+        continue;
+      }
+      const int Q = s.down ? QI : QH, nb = s.down ? nbI : nbH;
+      int u = s.u0 + pt / Q;
+      const int q = pt % Q;
+      pb = nb * q / Q, pe = nb * (q + 1) / Q, pc = 0, pt += kStreamW;
+      const size_t blk = s.b16 ? 4 * kHBlk : kQBlk;  // bytes of 8 rows x 512 k
+      if (s.down) {
+        const uint8_t* d = s.slot == kShared ? p.sh_d : tab.ent[s.slot].d;
+        pa = d + (size_t)(2 * u) * nb * blk, pz = pa + nb * blk;
+      } else if (s.slot == kShared) {
+        if (p.sh_bgu) pa = p.sh_bgu + (size_t)(2 * u) * nb * blk, pz = pa + nb * blk;
+        else pa = p.sh_g + (size_t)u * nb * blk, pz = p.sh_u + (size_t)u * nb * blk;
+      } else {
+        const BlockEnt& e = tab.ent[u / upp];
+        u %= upp;
+        pa = e.g + (size_t)u * nb * blk, pz = e.u + (size_t)u * nb * blk;
+      }
+      pa += pb * blk, pz += pb * blk;
+    }
+    return true;
+  };
+  auto issue = [&]() {
+    const int b16 = segs[ps].b16;
+    const uint32_t slot = issued % NST, bytes = b16 ? kHBlk : kQBlk;
+    uint8_t* st = myring + slot * kStage;
+    mbar_expect_tx(mybar + slot, 2 * bytes);
+    bulk_g2s_hint(st, pa, bytes, mybar + slot, pol);
+    bulk_g2s_hint(st + kQBlk, pz, bytes, mybar + slot, pol);
+    ++issued, pa += bytes, pz += bytes;
+    if (!b16 || ++pc == 4) ++pb, pc = 0;
+  };
+  auto fill = [&]() {
+    while (issued - consumed < (uint32_t)NST && open_task()) issue();
+  };
+
   if (router) {
     // ---- a row each; the last one to be routed builds the table -------------------------------------------------------------
     RouteSmem& rs = *reinterpret_cast<RouteSmem*>(tiles);
     int* s_idx = reinterpret_cast<int*>(part);
-    float* s_w = reinterpret_cast<float*>(s_idx + kMaxEnt);
-    uint32_t* scratch = reinterpret_cast<uint32_t*>(s_w + kMaxEnt);
-    const int row = cta - Gs, KS = (p.H + 1023) / 1024;
-    if (threadIdx.x == 0) *s_tick = poll_ge(&sy->cnt_lp, Gs) ? 1 : 0;
+    const int row = cta - Gs, KS = (p.H + 1023) / 1024, nt = (p.E + 31) & ~31;
+    for (int i = threadIdx.x; i < p.E * 3; i += kThreads) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.desc + i));
+    if (threadIdx.x == 0) *s_tick = poll_near(&sy->cnt_lp, Gs) ? 1 : 0;
     __syncthreads();
-    bool ok = *s_tick != 0;
+    const bool ok = *s_tick != 0;
     __syncthreads();
     if (ok) {
-      route_row_cta(p.rp, p.lpart + (size_t)row * p.E, KS, (size_t)kMaxRows * p.E, p.bias, rs, nullptr, p.idx + row * p.topk, p.w + row * p.topk);
-      __threadfence();
-      __syncthreads();
-      if (threadIdx.x == 0) *s_tick = atomicAdd(&sy->cnt_rt, 1);
-      __syncthreads();
-      if (*s_tick == p.M - 1) {
+      if ((int)threadIdx.x < nt)
+        route_row_cta(p.rp, p.lpart + (size_t)row * p.E, KS, (size_t)kMaxRows * p.E, p.bias, rs, nullptr, p.idx + row * p.topk,
+                      p.w + row * p.topk, nullptr, nullptr, CtaPart{nt, 2});
+      if (warp == 0) {  // (warp 0 wrote the picks)
         __threadfence();
-        if ((int)threadIdx.x < p.M * p.topk) s_idx[threadIdx.x] = __ldcg(p.idx + threadIdx.x), s_w[threadIdx.x] = __ldcg(p.w + threadIdx.x);
-        __syncthreads();
-        build_block_tab(tab, scratch, s_idx, s_w, p);
-        if (threadIdx.x == 0 && tab.bad) atomicCAS(p.status, 0, tab.bad);
-        const uint4* s4 = reinterpret_cast<const uint4*>(&tab);
-        for (int i = threadIdx.x; i < (int)(sizeof(BlockTab) / 16); i += kThreads) reinterpret_cast<uint4*>(p.tab)[i] = s4[i];
+        __syncwarp();
+        if (lane == 0) *s_tick = p.M > 1 ? atomicAdd(&sy->cnt_rt, 1) : 0;
+      }
+      __syncthreads();
+      if (*s_tick == p.M - 1 && threadIdx.x < 64) {
         __threadfence();
-        __syncthreads();
-        if (threadIdx.x == 0) atomicExch(&sy->tab_ready, 1);
+        build_block_tab(p.tab, s_idx, s_idx + kMaxEnt, p);
       }
     } else if (threadIdx.x == 0) {
       *s_fail = 1;
     }
     __syncthreads();
   } else if (warp < kStageW0) {
-    // ---- the router's logit slices, one warp a (expert, 1024 k); a CTA reports when all of its are in memory ------------------
+    // ---- the router's logit slices, one warp a (expert, 1024 k); a CTA reports when all of its are in memory.  The first slice's
+    // weights are requested before the rings fill, whose weights are not needed before the logits are done. --------------------
     const int KS = (p.H + 1023) / 1024, ntask = p.E * KS;
-    for (int i = warp * Gs + cta; i < ntask; i += kStageW0 * Gs) logit_slice_task(p.x, p.wr, p.M, p.H, p.E, i / KS, i % KS, p.lpart, lane);
+    int i = warp * Gs + cta;
+    float4 wv[8];
+    if (i < ntask) logit_slice_weights(p.wr, p.H, i / KS, i % KS, lane, wv);
+    if (warp < kStreamW && lane == 0) fill();
+    __syncwarp();
+    if (i < ntask) logit_slice_rows(p.x, wv, p.M, p.H, p.E, i / KS, i % KS, p.lpart, lane);
+    for (i += kStageW0 * Gs; i < ntask; i += kStageW0 * Gs) logit_slice_task(p.x, p.wr, p.M, p.H, p.E, i / KS, i % KS, p.lpart, lane);
     __threadfence();
     asm volatile("bar.sync 1, %0;" ::"n"(kStageW0 * 32) : "memory");
     if (threadIdx.x == 0) {
@@ -294,67 +376,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const BlockParams p) {
     }
   }
 
-  const int nb_first = a1 > a0 ? 1 : 0;  // segments known without the table
   if (warp < kStreamW) {
     // ---- stream warps --------------------------------------------------------------------------------------------------------
-    uint8_t* myring = ring + (size_t)warp * NST * kStage;
-    uint64_t* mybar = bars + warp * NST;
     const uint32_t ring_at = smem_u32(myring);
-    const uint64_t pol = policy_evict_first();
-    uint32_t issued = 0, consumed = 0;
     bool ok = true;
-    auto first_task = [&](const Seg& s) { return (int)((unsigned)(warp + kStreamW - s.base % kStreamW) % kStreamW); };
-    // producer (lane 0): segment, task, block, quarter of a bf16 block
-    int nknown = nb_first, ps = 0, pt = -1, pb = 0, pe = 0, pc = 0;
-    bool all_known = false;
-    const uint8_t *pa = nullptr, *pz = nullptr;
-    auto open_task = [&]() {
-      while (pb == pe) {
-        if (ps >= nknown) {
-          if (!all_known && mbar_test_wait(tabbar, 0)) all_known = true, nknown = *s_nseg;
-          if (ps >= nknown) return false;
-        }
-        const Seg& s = segs[ps];
-        if (pt < 0) pt = first_task(s);
-        if (pt >= s.tasks) {
-          ++ps, pt = -1;
-          continue;
-        }
-        const int Q = s.down ? QI : QH, nb = s.down ? nbI : nbH;
-        int u = s.u0 + pt / Q;
-        const int q = pt % Q;
-        pb = nb * q / Q, pe = nb * (q + 1) / Q, pc = 0, pt += kStreamW;
-        const size_t blk = s.b16 ? 4 * kHBlk : kQBlk;  // bytes of 8 rows x 512 k
-        if (s.down) {
-          const uint8_t* d = s.slot == kShared ? p.sh_d : tab.ent[s.slot].d;
-          pa = d + (size_t)(2 * u) * nb * blk, pz = pa + nb * blk;
-        } else if (s.slot == kShared) {
-          if (p.sh_bgu) pa = p.sh_bgu + (size_t)(2 * u) * nb * blk, pz = pa + nb * blk;
-          else pa = p.sh_g + (size_t)u * nb * blk, pz = p.sh_u + (size_t)u * nb * blk;
-        } else {
-          const BlockEnt& e = tab.ent[u / upp];
-          u %= upp;
-          pa = e.g + (size_t)u * nb * blk, pz = e.u + (size_t)u * nb * blk;
-        }
-        pa += pb * blk, pz += pb * blk;
-      }
-      return true;
-    };
-    int pseg_b16 = 0;
-    auto issue = [&]() {
-      pseg_b16 = segs[ps].b16;
-      const uint32_t slot = issued % NST, bytes = pseg_b16 ? kHBlk : kQBlk;
-      uint8_t* st = myring + slot * kStage;
-      mbar_expect_tx(mybar + slot, 2 * bytes);
-      bulk_g2s_hint(st, pa, bytes, mybar + slot, pol);
-      bulk_g2s_hint(st + kQBlk, pz, bytes, mybar + slot, pol);
-      ++issued, pa += bytes, pz += bytes;
-      if (!pseg_b16 || ++pc == 4) ++pb, pc = 0;
-    };
-    auto fill = [&]() {
-      while (issued - consumed < (uint32_t)NST && open_task()) issue();
-    };
-    if (lane == 0) fill();
     auto stage_ready = [&]() {
       const uint32_t si = consumed % NST;
       if (!mbar_wait(mybar + si, (consumed / NST) & 1)) ok = false;
@@ -368,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const BlockParams p) {
 
     for (int k = 0; ok; ++k) {
       if (k >= nb_first) {  // (the table is needed from here on)
-        if (k == nb_first && !mbar_wait(tabbar, 0, 64)) ok = false;
+        if (k == nb_first && !mbar_wait(tabbar, 0, 20)) ok = false;
         if (!ok || *s_fail || k >= *s_nseg) break;
         if (lane == 0) fill();
       }
@@ -450,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const BlockParams p) {
     bool ok = true;
     for (int k = 0; ok; ++k) {
       if (k >= nb_first) {
-        if (k == nb_first && !mbar_wait(tabbar, 0, 64)) ok = false;
+        if (k == nb_first && !mbar_wait(tabbar, 0, 20)) ok = false;
         if (!ok || *s_fail || k >= *s_nseg) break;
       }
       const Seg s = segs[k];
@@ -518,63 +543,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const BlockParams p) {
   } else {
     // ---- the staging warps: the table, then every segment's activations ---------------------------------------------------------
     const int sw = warp - kStageW0;
-    bool ok = true;
-    for (int k = 0; ok; ++k) {
-      if (k == nb_first) {
-        if (sw == 0) {  // the table, and from it this CTA's segments
-          int got = 0;
-          if (lane == 0) got = !*s_fail && poll_ge(&sy->tab_ready, 1);
-          got = __shfl_sync(0xffffffffu, got, 0);
-          if (got) {
-            for (int i = lane; i < (int)(sizeof(BlockTab) / 16); i += 32)
-              reinterpret_cast<uint4*>(&tab)[i] = __ldcg(reinterpret_cast<const uint4*>(p.tab) + i);
-            __syncwarp();
-            if (lane == 0) {
-              const long long cI = p.b16 ? 4 * kHBlk : kQBlk, cS = 4 * kHBlk;  // (costs of 8 rows x 512 k)
-              int nseg = nb_first, base = (a1 - a0) * QH;
-              const int NU = tab.nslots * upp, nsh = has_sh ? upp : 0;
-              const int u0 = routed_begin(cta, NU, cI, nsh, cS, Gs, G), u1 = routed_begin(cta + 1, NU, cI, nsh, cS, Gs, G);
-              if (u1 > u0) segs[nseg++] = Seg{0, p.b16, 0, p.M, u0, u1 - u0, (u1 - u0) * QH, base}, base += (u1 - u0) * QH;
-              const int nd = has_sh ? NT : 0, s0 = shared_begin(cta, nd, G), s1 = shared_begin(cta + 1, nd, G);
-              if (s1 > s0) segs[nseg++] = Seg{1, 1, kShared, p.M, s0, s1 - s0, (s1 - s0) * QI, base}, base += (s1 - s0) * QI;
-              const int ND = tab.nslots * NT, d0 = routed_begin(cta, ND, cI, nd, cS, G, G), d1 = routed_begin(cta + 1, ND, cI, nd, cS, G, G);
-              for (int d = d0; d < d1;) {
-                const int slot = d / NT, e = min(d1, (slot + 1) * NT);
-                segs[nseg++] = Seg{1, p.b16, slot, tab.ent[slot].n, d - slot * NT, e - d, (e - d) * QI, base}, base += (e - d) * QI;
-                d = e;
-              }
-              *s_nseg = nseg;
-            }
-            __threadfence_block();
-            __syncwarp();
-          } else {
-            *s_fail = 1;
-          }
-          __syncwarp();
-          if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(tabbar)) : "memory");
-        } else if (!mbar_wait(tabbar, 0, 64)) {
-          ok = false;
-        }
-      }
-      if (!ok || *s_fail || (k >= nb_first && k >= *s_nseg)) break;
-      const Seg s = segs[k];
-      if (k >= p.nbuf && !mbar_wait(tile_free + k - p.nbuf, 0, 20)) {
-        ok = false;
-        break;
-      }
-      const int nb = s.down ? nbI : nbH, K = s.down ? p.I : p.H;
-      if (s.down) {  // the slot's h, once all of its units are in memory
-        int got = 0;
-        if (lane == 0) got = poll_ge(&sy->cnt_h[s.slot], upp);
-        if (!(ok = __shfl_sync(0xffffffffu, got, 0) != 0)) break;
-      }
-      const Tile tile(tiles + (size_t)(k % p.nbuf) * p.tile, nb, s.rows);
-      const __nv_bfloat16* src = s.down ? p.h + (size_t)s.slot * kMaxRows * p.I : p.x;
-      const uint32_t span = s.rows * 128;
-      for (int i = sw; i < nb * s.rows; i += kStagers) {
-        const int b = i / s.rows, r = i - b * s.rows;
+    auto stage = [&](int k, bool b16, int rows, int nb, const __nv_bfloat16* src, int K) {
+      const Tile tile(tiles + (size_t)(k % p.nbuf) * p.tile, nb, rows);
+      const uint32_t span = rows * 128;
+      for (int i = sw; i < nb * rows; i += kStagers) {
+        const int b = i / rows, r = i - b * rows;
         uint8_t* xt = tile.x + (size_t)b * 8 * span + r * 128;
-        if (s.b16) {
+        if (b16) {
           uint32_t w[8];
           uint4 o[2];
           load_16<true>(w, src + (size_t)r * K, b * 512 + 16 * lane, K, true);
@@ -582,20 +557,73 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const BlockParams p) {
           uint4* d = reinterpret_cast<uint4*>(xt + (size_t)(lane >> 2) * span + (lane & 3) * 32);
           d[0] = o[0], d[1] = o[1];
         } else {
-          stage_row<4, true>(src + (size_t)r * K, b * 512, K, true, xt, span, false, tile.sum + (size_t)b * 16 * s.rows + 2 * r, s.rows * 8,
-                             tile.scale + b * s.rows + r, lane);
+          stage_row<4, true>(src + (size_t)r * K, b * 512, K, true, xt, span, false, tile.sum + (size_t)b * 16 * rows + 2 * r, rows * 8,
+                             tile.scale + b * rows + r, lane);
         }
       }
       __threadfence_block();
       __syncwarp();
       if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(tile_full + k)) : "memory");
+    };
+    bool ok = true;
+    // x: for the shared expert in bf16, for the routed ones as their format wants it
+    for (int k = 0; k <= nb_first && ok; ++k) {
+      if (k >= p.nbuf) ok = mbar_wait(tile_free + k - p.nbuf, 0, 20);
+      if (ok) stage(k, k < nb_first || p.b16, p.M, nbH, p.x, p.H);
+    }
+    // the table, and from it this CTA's segments
+    int got = 0;
+    if (lane == 0) got = ok && !*s_fail && poll_near(&sy->tab_ready, 1);
+    got = __shfl_sync(0xffffffffu, got, 0);
+    if (got) {
+      const int n16 = (int)(offsetof(BlockTab, ent) + min(p.M * p.topk, kMaxEnt) * sizeof(BlockEnt)) / 16;
+      for (int i = sw * 32 + lane; i < n16; i += kStagers * 32) reinterpret_cast<uint4*>(&tab)[i] = __ldcg(reinterpret_cast<const uint4*>(p.tab) + i);
+      __threadfence_block();
+    } else {
+      ok = false;
+      *s_fail = 1;
+    }
+    asm volatile("bar.sync 4, %0;" ::"n"(kStagers * 32) : "memory");
+    if (sw == 0) {
+      if (!*s_fail) {
+        // costs of 8 rows x 512 k in 64 bytes; lanes 0 and 1: this CTA's and the next one's first up unit, 2 and 3: down
+        const int cI = p.b16 ? 4 * kHBlk / 64 : kQBlk / 64, cS = 4 * kHBlk / 64, up = lane < 2;
+        const int NU = tab.nslots * upp, ND = tab.nslots * NT, nsh = has_sh ? upp : 0, nd = has_sh ? NT : 0;
+        const int at = routed_begin(cta + (lane & 1), up ? NU : ND, cI, up ? nsh : nd, cS, up ? Gs : G, G);
+        const int u0 = __shfl_sync(0xffffffffu, at, 0), u1 = __shfl_sync(0xffffffffu, at, 1);
+        const int d0 = __shfl_sync(0xffffffffu, at, 2), d1 = __shfl_sync(0xffffffffu, at, 3);
+        if (lane == 0) {
+          int nseg = nb_first, base = (a1 - a0) * QH;
+          segs[nseg++] = Seg{0, p.b16, 0, p.M, u0, u1 - u0, (u1 - u0) * QH, base}, base += (u1 - u0) * QH;
+          const int s0 = shared_begin(cta, nd, G), s1 = shared_begin(cta + 1, nd, G);
+          if (s1 > s0) segs[nseg++] = Seg{1, 1, kShared, p.M, s0, s1 - s0, (s1 - s0) * QI, base}, base += (s1 - s0) * QI;
+          for (int d = d0; d < d1;) {
+            const int slot = d / NT, e = min(d1, (slot + 1) * NT);
+            segs[nseg++] = Seg{1, p.b16, slot, tab.ent[slot].n, d - slot * NT, e - d, (e - d) * QI, base}, base += (e - d) * QI;
+            d = e;
+          }
+          *s_nseg = nseg;
+        }
+      }
+      __threadfence_block();
+      __syncwarp();
+      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(tabbar)) : "memory");
+    }
+    if (ok) ok = mbar_wait(tabbar, 0, 20);
+    for (int k = nb_first + 1; ok && !*s_fail && k < *s_nseg; ++k) {
+      const Seg s = segs[k];
+      if (k >= p.nbuf) ok = mbar_wait(tile_free + k - p.nbuf, 0, 20);
+      int there = 0;  // the slot's h, once all of its units are in memory
+      if (lane == 0) there = ok && poll_near(&sy->cnt_h[s.slot], upp);
+      if (!(ok = __shfl_sync(0xffffffffu, there, 0) != 0)) break;
+      stage(k, s.b16, s.rows, nbI, p.h + (size_t)s.slot * kMaxRows * p.I, p.I);
     }
     if (!ok) *s_fail = 1;
   }
 
   // ---- every CTA's outputs are in memory: a row's picks in ascending expert id, the shared expert, the residual, one rounding
   __syncthreads();
-  if (threadIdx.x == 0 && !*s_fail && !poll_ge(&sy->cnt_done, G)) *s_fail = 1;
+  if (threadIdx.x == 0 && !*s_fail && !poll_near(&sy->cnt_done, G)) *s_fail = 1;
   __syncthreads();
   if (!*s_fail) {
     const int H4 = p.H / 4, items = p.M * H4;
