@@ -63,6 +63,7 @@ namespace {
 
 constexpr int kStreamW = 11, kStageW0 = kStreamW + 1, kWarps = 16, kStagers = kWarps - kStageW0, kThreads = kWarps * 32;
 constexpr int kStage = 2 * kQBlk;        // a ring stage: an INT4 block pair (a pair of bf16 blocks, 4096 B, fits)
+constexpr int kFront = 300 * 1024;       // bytes an SM streams from the end of the logits until the table is known (7 us)
 constexpr int kP = 16;                   // tasks' sums in flight
 constexpr int kPart = 512;               // bytes of a task's sums: [2 sets][32 lanes][2] f32
 constexpr int kShared = kMaxEnt;         // the shared expert's place among the h, y and counters
@@ -157,17 +158,19 @@ DSGX_DEV void pair_b16(float (&d)[4], uint32_t st, uint32_t x, uint32_t span, in
   }
 }
 
-// ---- the division of a phase's units over the CTAs.  n shared units of cost cs over the first Gs CTAs, N routed ones of cost c so
-// that every CTA's total is alike (a CTA behind Gs routes meanwhile: it counts like the others' average): where CTA i's
-// routed run begins.
+// ---- the division of a phase's units over the CTAs.  n shared units of cost cs over the first Gs CTAs, then N routed ones of cost c
+// so that all CTAs end alike; none begins its routed units before a time worth `front` has passed.  Where CTA i's routed run
+// begins.
 DSGX_DEV int shared_begin(int i, int n, int Gs) { return (int)((unsigned)(n * min(i, Gs)) / (unsigned)Gs); }
-DSGX_DEV int routed_begin(int i, int N, int c, int n, int cs, int Gs, int G) {
+DSGX_DEV int routed_begin(int i, int N, int c, int n, int cs, int Gs, int G, int front) {
   if (i <= 0) return 0;
   if (i >= G) return N;
-  const long long avg = (long long)n * cs / Gs, total = (long long)N * c + (long long)n * cs + (G - Gs) * avg;
-  if (total < (long long)G * cs * ((n + Gs - 1) / Gs + 1)) return (int)((long long)N * i / G);  // (few routed units: an even deal)
-  const long long before = total * i / G - (long long)cs * shared_begin(i, n, Gs) - max(0, i - Gs) * avg;
-  return (int)min((long long)N, max(0ll, before / c));
+  const int a = n / Gs, few = max(cs * a, front), many = max(cs * (a + 1), front);  // a CTA has a or a + 1 shared units
+  const int extra = shared_begin(i, n, Gs) - a * min(i, Gs), all_extra = n - a * Gs;
+  const long long used = (long long)few * (i - extra) + (long long)many * extra - (i > Gs ? (long long)(few - front) * (i - Gs) : 0);
+  const long long total = (long long)N * c + (long long)few * (G - all_extra) + (long long)many * all_extra - (long long)(few - front) * (G - Gs);
+  if (total < (long long)G * 2 * many) return (int)((long long)N * i / G);  // (few routed units: an even deal)
+  return (int)min((long long)N, max(0ll, (total * i / G - used) / c));
 }
 
 // ---- the table, by the first 64 threads of a CTA, a thread a pick, written straight to global memory.  s_idx, s_first: kMaxEnt
@@ -358,16 +361,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const BlockParams p) {
     }
     __syncthreads();
   } else if (warp < kStageW0) {
-    // ---- the router's logit slices, one warp a (expert, 1024 k); a CTA reports when all of its are in memory.  The first slice's
-    // weights are requested before the rings fill, whose weights are not needed before the logits are done. --------------------
+    // ---- the router's logit slices, one warp a (expert, 1024 k); a CTA reports when all of its are in memory.  (The rings
+    // filled first: 2.4 us later logits and not a microsecond gained on the shared expert.) ------------------------------------
     const int KS = (p.H + 1023) / 1024, ntask = p.E * KS;
     int i = warp * Gs + cta;
-    float4 wv[8];
-    if (i < ntask) logit_slice_weights(p.wr, p.H, i / KS, i % KS, lane, wv);
-    if (warp < kStreamW && lane == 0) fill();
-    __syncwarp();
-    if (i < ntask) logit_slice_rows(p.x, wv, p.M, p.H, p.E, i / KS, i % KS, p.lpart, lane);
-    for (i += kStageW0 * Gs; i < ntask; i += kStageW0 * Gs) logit_slice_task(p.x, p.wr, p.M, p.H, p.E, i / KS, i % KS, p.lpart, lane);
+    for (; i < ntask; i += kStageW0 * Gs) logit_slice_task(p.x, p.wr, p.M, p.H, p.E, i / KS, i % KS, p.lpart, lane);
     __threadfence();
     asm volatile("bar.sync 1, %0;" ::"n"(kStageW0 * 32) : "memory");
     if (threadIdx.x == 0) {
@@ -380,6 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const BlockParams p) {
     // ---- stream warps --------------------------------------------------------------------------------------------------------
     const uint32_t ring_at = smem_u32(myring);
     bool ok = true;
+    if (lane == 0) fill();
     auto stage_ready = [&]() {
       const uint32_t si = consumed % NST;
       if (!mbar_wait(mybar + si, (consumed / NST) & 1)) ok = false;
@@ -589,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const BlockParams p) {
         // costs of 8 rows x 512 k in 64 bytes; lanes 0 and 1: this CTA's and the next one's first up unit, 2 and 3: down
         const int cI = p.b16 ? 4 * kHBlk / 64 : kQBlk / 64, cS = 4 * kHBlk / 64, up = lane < 2;
         const int NU = tab.nslots * upp, ND = tab.nslots * NT, nsh = has_sh ? upp : 0, nd = has_sh ? NT : 0;
-        const int at = routed_begin(cta + (lane & 1), up ? NU : ND, cI, up ? nsh : nd, cS, up ? Gs : G, G);
+        const int at = routed_begin(cta + (lane & 1), up ? NU : ND, cI, up ? nsh : nd, cS, up ? Gs : G, G, up ? kFront / (64 * nbH) : 0);
         const int u0 = __shfl_sync(0xffffffffu, at, 0), u1 = __shfl_sync(0xffffffffu, at, 1);
         const int d0 = __shfl_sync(0xffffffffu, at, 2), d1 = __shfl_sync(0xffffffffu, at, 3);
         if (lane == 0) {

@@ -83,6 +83,14 @@ DSGX_DEV float2 fma2(float2 a, float2 b, float2 c) {
   return d;
 }
 
+DSGX_DEV float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
 constexpr uint32_t kNib0 = 0x000F000Fu, kNib1 = 0x00F000F0u;  // nibbles 0 and 4 of a word; 1 and 5 (2, 6 and 3, 7 after a shift by 8)
 // minus the zero point in byte b of a word of them: 0x4B0000zz is 2^23 + z
 DSGX_DEV float minus_zero(uint32_t zeros, int b) { return 8388608.f - __uint_as_float(__byte_perm(zeros, 0x4B000000u, 0x7440u + b)); }
