@@ -41,24 +41,25 @@ constexpr size_t kSmemMax = 227 * 1024;
 
 constexpr int kUnitBlk = 4736;    // 16 rows x 512 k
 
-// S sets of eight rows; W stream warps with NST ring stages each, P tasks' sums in flight (a power of two)
-template <int S_, int W_, int NST_, int P_>
+// S sets of eight rows (kCol: four rows at most, see unit_block4); W stream warps with NST ring stages each, P tasks' sums in flight (a power of two)
+template <int S_, int W_, int NST_, int P_, bool kCol_ = false>
 struct LinVar {
   static constexpr int S = S_, W = W_, NST = NST_, P = P_;
+  static constexpr bool kCol = kCol_;
   static constexpr int kThreads = (W + 1) * 32;
   static constexpr int kPart = 512 * S;  // bytes of a task's (or a rank's) sums: [S][32 lanes][4] f32
   static size_t smem(int M, int kblocks, int C) {
     return (size_t)W * NST * kUnitBlk + (size_t)P * kPart + (C > 1 ? (size_t)kSlotsOwned * C * kPart : 0) +
-           (size_t)kblocks * (M * 1024 + even(M) * 68) + (W * NST + kSlotsOwned * (1 + kMaxCluster)) * 8 + P * 4 + 16 + 128;
+           (size_t)kblocks * (M * 1024 + even(M) * 68) + (kCol ? 256 : 0) + (W * NST + kSlotsOwned * (1 + kMaxCluster)) * 8 + P * 4 + 16 + 128;
   }
   __host__ __device__ static int even(int M) { return (M + 1) & ~1; }
 };
 
 // The products of one block, times 2^(E - 24): blk[s] = a lane's four sums (first strip's row g with rows 8 s + 2 t and + 1 of x,
-// then the second strip's).  st: the stage; x[s], sx[s]: this lane's activations and group sums at the block's first span;
+// then the second strip's), the spans' first and second groups apart.  st: the stage; x[s], sx[s]: this lane's activations and group sums at the block's first span;
 // span, sspan: bytes from one span to the next.
 template <int S>
-DSGX_DEV void unit_block(float (&blk)[S][4], uint32_t st, const uint32_t (&x_at)[S], uint32_t span, const uint32_t (&sx_at)[S], uint32_t sspan,
+DSGX_DEV void unit_block(float (&blk)[S][4][2], uint32_t st, const uint32_t (&x_at)[S], uint32_t span, const uint32_t (&sx_at)[S], uint32_t sspan,
                          int lane) {
   const int g = lane >> 2;
   const uint4 zq = lds_v4(st + 4608 + 16 * g);
@@ -67,7 +68,8 @@ DSGX_DEV void unit_block(float (&blk)[S][4], uint32_t st, const uint32_t (&x_at)
 #pragma unroll
   for (int s = 0; s < S; ++s) {
     x[s] = x_at[s], sx[s] = sx_at[s];
-    blk[s][0] = blk[s][1] = blk[s][2] = blk[s][3] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) blk[s][i][0] = blk[s][i][1] = 0.f;
   }
 #pragma unroll
   for (int jj = 0; jj < 4; ++jj) {
@@ -95,12 +97,45 @@ DSGX_DEV void unit_block(float (&blk)[S][4], uint32_t st, const uint32_t (&x_at)
           mma_f16_zero(d, wa & kNib0, wb & kNib0, wa & kNib1, wb & kNib1, xv.x, xv.y);
           mma_f16(d, wa8 & kNib0, wb8 & kNib0, wa8 & kNib1, wb8 & kNib1, xv.z, xv.w);
           const float s0 = c ? sum[s].z : sum[s].x, s1 = c ? sum[s].w : sum[s].y;
-          blk[s][0] = fmaf(fa, fmaf(za, s0, d[0]), blk[s][0]), blk[s][1] = fmaf(fa, fmaf(za, s1, d[1]), blk[s][1]);
-          blk[s][2] = fmaf(fb, fmaf(zb, s0, d[2]), blk[s][2]), blk[s][3] = fmaf(fb, fmaf(zb, s1, d[3]), blk[s][3]);
+          blk[s][0][c] = fmaf(fa, fmaf(za, s0, d[0]), blk[s][0][c]), blk[s][1][c] = fmaf(fa, fmaf(za, s1, d[1]), blk[s][1][c]);
+          blk[s][2][c] = fmaf(fb, fmaf(zb, s0, d[2]), blk[s][2][c]), blk[s][3][c] = fmaf(fb, fmaf(zb, s1, d[3]), blk[s][3][c]);
         }
       }
 #pragma unroll
       for (int s = 0; s < S; ++s) x[s] += span, sx[s] += sspan;
+    }
+  }
+}
+
+// The same for up to four rows, with the same bits: column 2 r + c of B is row r in the MMAs of a span's group c and zeros in the
+// other group's, so a lane ends with row t's two group sums side by side and packed operations finish them: 46 instructions
+// 64 k instead of 60.  x0, x1: where the lane finds group 0's and group 1's activations (zeros: step 0); sx: row t's sums.
+DSGX_DEV void unit_block4(float2 (&blk)[2], uint32_t st, uint32_t x0, uint32_t x1, uint32_t step0, uint32_t step1, uint32_t sx, uint32_t sspan,
+                          int lane) {
+  const int g = lane >> 2;
+  const uint4 zq = lds_v4(st + 4608 + 16 * g);
+  const uint32_t* zw = &zq.x;
+  blk[0] = blk[1] = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int jj = 0; jj < 4; ++jj) {
+    const uint4 sc = lds_v4(st + 4096 + 128 * jj + 16 * g);
+    const uint32_t ze = zw[jj] & 0x0F0F0F0Fu, zo = (zw[jj] >> 4) & 0x0F0F0F0Fu;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const uint4 w = lds_v4(st + 512 * (2 * jj + q) + 16 * lane), xa = lds_v4(x0), xb = lds_v4(x1);
+      const float2 sum = lds_f2(sx);
+      x0 += step0, x1 += step1, sx += sspan;
+      const uint32_t a8 = w.x >> 8, b8 = w.y >> 8, c8 = w.z >> 8, d8 = w.w >> 8, z = q ? zo : ze;
+      float d[4];
+      mma_f16_zero(d, w.x & kNib0, w.y & kNib0, w.x & kNib1, w.y & kNib1, xa.x, xa.y);
+      mma_f16(d, a8 & kNib0, b8 & kNib0, a8 & kNib1, b8 & kNib1, xa.z, xa.w);
+      mma_f16(d, w.z & kNib0, w.w & kNib0, w.z & kNib1, w.w & kNib1, xb.x, xb.y);
+      mma_f16(d, c8 & kNib0, d8 & kNib0, c8 & kNib1, d8 & kNib1, xb.z, xb.w);
+      const float2 za = make_float2(minus_zero(z, 0), minus_zero(z, 2)), zb = make_float2(minus_zero(z, 1), minus_zero(z, 3));
+      const float2 fa = q ? make_float2(scale_hi(sc.x), scale_hi(sc.z)) : make_float2(scale_lo(sc.x), scale_lo(sc.z));
+      const float2 fb = q ? make_float2(scale_hi(sc.y), scale_hi(sc.w)) : make_float2(scale_lo(sc.y), scale_lo(sc.w));
+      blk[0] = fma2(fa, fma2(za, sum, make_float2(d[0], d[1])), blk[0]);
+      blk[1] = fma2(fb, fma2(zb, sum, make_float2(d[2], d[3])), blk[1]);
     }
   }
 }
@@ -197,7 +232,8 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
   const int Me = V::even(p.M);
   float* xsum = reinterpret_cast<float*>(xt + (size_t)p.xblocks * p.M * 1024);  // [spans][row pairs][2 groups][2 rows]
   float* xscale = xsum + (size_t)p.xblocks * Me * 16;                           // [blocks][rows]: 2^(12 - E)
-  uint64_t* bars = reinterpret_cast<uint64_t*>(xscale + (size_t)p.xblocks * Me);
+  uint8_t* zero = smem + (((xscale + (size_t)p.xblocks * Me) - reinterpret_cast<float*>(smem)) * 4 + 127) / 128 * 128;  // kCol: 128 zeros
+  uint64_t* bars = reinterpret_cast<uint64_t*>(V::kCol ? zero + 128 : reinterpret_cast<uint8_t*>(xscale + (size_t)p.xblocks * Me));
   uint64_t* rfull = bars + W * NST;                                    // [kSlotsOwned] every rank's sums are in my buffer
   uint64_t* rfree = rfull + kSlotsOwned;                               // [owner][kSlotsOwned] that owner's buffer may be written
   int* cnt = reinterpret_cast<int*>(rfree + kMaxCluster * kSlotsOwned);  // [P] block pairs summed of a unit in flight
@@ -212,6 +248,7 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
     *done = 0, *fail = 0;
   }
   for (int i = threadIdx.x; i < P; i += V::kThreads) cnt[i] = 0;
+  if (V::kCol && threadIdx.x < 32) reinterpret_cast<uint32_t*>(zero)[threadIdx.x] = 0;
   mbar_fence_init();
   __syncwarp();
   if (C > 1) cluster_sync_all();
@@ -252,12 +289,14 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
   // ---- this rank's activations ------------------------------------------------------------------------------------------
   pdl_wait();
   // tile: [span of 64 k][row][the span's 8 pieces of 8 f16], a piece = the k a lane's word covers, in the words' nibble order;
-  // odd rows with the span's two groups exchanged, so that two rows' reads of one group do not meet in the banks
+  // eight columns: odd rows with the span's two groups exchanged, so that two rows' reads of one group do not meet in the
+  // banks.  The groups' sums: a row's two side by side (kCol), or two rows' of a group.
   const uint32_t span = p.M * 128, sspan = Me * 8;
   for (int i = warp; i < nbk * p.M; i += W + 1) {
     const int b = i / p.M, r = i - b * p.M;
-    stage_row<8, false>(p.x + (size_t)r * p.ldx, (b0 + b) * 512, p.K, p.x_vec != 0, xt + (size_t)b * 8 * span + r * 128, span, r & 1,
-              xsum + (size_t)b * 16 * Me + (r >> 1) * 4 + (r & 1), sspan, xscale + b * Me + r, lane);
+    stage_row<V::kCol ? 4 : 8, false>(p.x + (size_t)r * p.ldx, (b0 + b) * 512, p.K, p.x_vec != 0, xt + (size_t)b * 8 * span + r * 128, span,
+                                      !V::kCol && (r & 1), xsum + (size_t)b * 16 * Me + (V::kCol ? 2 * r : (r >> 1) * 4 + (r & 1)), sspan,
+                                      xscale + b * Me + r, lane);
   }
   __syncthreads();
 
@@ -266,12 +305,19 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
     const int g = lane >> 2, t = lane & 3;
     const uint32_t ring_at = smem_u32(myring);
     uint32_t xl[S], sl[S], fl[S];  // row 8 s + g of the tile (columns without a row: the last row, their sums are not used)
+    uint32_t xz = 0;               // kCol: where the lane reads zeros for the other group
+    const int half = g & 1;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      const int r = min(8 * s + g, p.M - 1);
-      const int pr = min(4 * s + t, Me / 2 - 1);  // the pair of rows whose sums the lane holds
-      xl[s] = smem_u32(xt) + r * 128 + ((t * 16) ^ ((r & 1) * 64));
-      sl[s] = smem_u32(xsum) + pr * 16, fl[s] = smem_u32(xscale) + pr * 8;
+      if (V::kCol) {
+        const int r = min(g >> 1, p.M - 1), me = min(t, p.M - 1);
+        xl[s] = smem_u32(xt) + r * 128 + 64 * half + t * 16, xz = smem_u32(zero) + 64 * half + t * 16;
+        sl[s] = smem_u32(xsum) + me * 8, fl[s] = smem_u32(xscale) + me * 4;
+      } else {
+        const int r = min(8 * s + g, p.M - 1), pr = min(4 * s + t, Me / 2 - 1);  // (pr: the pair of rows whose sums the lane holds)
+        xl[s] = smem_u32(xt) + r * 128 + ((t * 16) ^ ((r & 1) * 64));
+        sl[s] = smem_u32(xsum) + pr * 16, fl[s] = smem_u32(xscale) + pr * 8;
+      }
     }
     uint32_t consumed = 0;
     bool ok = true;
@@ -289,17 +335,28 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
             ok = false;
             break;
           }
-          uint32_t xb[S], sb[S];
-          float blk[S][4];
           const int lb = b - b0;
+          const uint32_t st = ring_at + si * kUnitBlk;
+          // the block's sums times 2^(24 - E), in two steps that cannot leave f32's range by themselves
+          if constexpr (V::kCol) {
+            float2 blk[2];
+            const uint32_t xb = xl[0] + lb * 8 * span;
+            unit_block4(blk, st, half ? xz : xb, half ? xb : xz, half ? 0 : span, half ? span : 0, sl[0] + lb * 8 * sspan, sspan, lane);
+            const float f = lds_f(fl[0] + lb * Me * 4);
+            acc[0][0] = fmaf(__fadd_rn(blk[0].x, blk[0].y) * 4096.f, f, acc[0][0]);
+            acc[0][2] = fmaf(__fadd_rn(blk[1].x, blk[1].y) * 4096.f, f, acc[0][2]);
+          } else {
+            uint32_t xb[S], sb[S];
+            float blk[S][4][2];
 #pragma unroll
-          for (int s = 0; s < S; ++s) xb[s] = xl[s] + lb * 8 * span, sb[s] = sl[s] + lb * 8 * sspan;
-          unit_block<S>(blk, ring_at + si * kUnitBlk, xb, span, sb, sspan, lane);
+            for (int s = 0; s < S; ++s) xb[s] = xl[s] + lb * 8 * span, sb[s] = sl[s] + lb * 8 * sspan;
+            unit_block<S>(blk, st, xb, span, sb, sspan, lane);
 #pragma unroll
-          for (int s = 0; s < S; ++s) {  // times 2^(24 - E), in two steps that cannot leave f32's range by themselves
-            const float2 f = lds_f2(fl[s] + lb * Me * 4);
-            acc[s][0] = fmaf(blk[s][0] * 4096.f, f.x, acc[s][0]), acc[s][1] = fmaf(blk[s][1] * 4096.f, f.y, acc[s][1]);
-            acc[s][2] = fmaf(blk[s][2] * 4096.f, f.x, acc[s][2]), acc[s][3] = fmaf(blk[s][3] * 4096.f, f.y, acc[s][3]);
+            for (int s = 0; s < S; ++s) {
+              const float2 f = lds_f2(fl[s] + lb * Me * 4);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) acc[s][i] = fmaf(__fadd_rn(blk[s][i][0], blk[s][i][1]) * 4096.f, i & 1 ? f.y : f.x, acc[s][i]);
+            }
           }
           ++consumed;
           __syncwarp();
@@ -369,8 +426,8 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
       for (int s = 0; s < S; ++s) {
         const float v[4] = {a[s].x, a[s].y, a[s].z, a[s].w};
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int m = 8 * s + 2 * t + e;
+        for (int e = 0; e < (V::kCol ? 1 : 2); ++e) {
+          const int m = V::kCol ? t : 8 * s + 2 * t + e;
           if (m >= p.M) continue;
           if (glu) {
             const int c = 8 * unit + g;
@@ -509,6 +566,7 @@ cudaError_t launch(LinearParams p, cudaStream_t st, bool* fits) {
 
 // One launch for M rows, or *fits = false where their activations do not fit shared memory.
 cudaError_t launch_linear_int4(const LinearParams& p, cudaStream_t st, bool* fits) {
+  if (p.M <= 4) return launch<LinVar<1, 15, 2, 32, true>>(p, st, fits);
   if (p.M <= 8) return launch<LinVar<1, 15, 2, 32>>(p, st, fits);
   return launch<LinVar<2, 11, 2, 16>>(p, st, fits);
 }
