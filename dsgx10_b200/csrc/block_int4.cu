@@ -545,19 +545,27 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const BlockParams p) {
     auto stage = [&](int k, bool b16, int rows, int nb, const __nv_bfloat16* src, int K) {
       const Tile tile(tiles + (size_t)(k % p.nbuf) * p.tile, nb, rows);
       const uint32_t span = rows * 128;
-      for (int i = sw; i < nb * rows; i += kStagers) {
-        const int b = i / rows, r = i - b * rows;
-        uint8_t* xt = tile.x + (size_t)b * 8 * span + r * 128;
-        if (b16) {
-          uint32_t w[8];
-          uint4 o[2];
-          load_16<true>(w, src + (size_t)r * K, b * 512 + 16 * lane, K, true);
-          nibble_order(o, w);
-          uint4* d = reinterpret_cast<uint4*>(xt + (size_t)(lane >> 2) * span + (lane & 3) * 32);
-          d[0] = o[0], d[1] = o[1];
-        } else {
-          stage_row<4, true>(src + (size_t)r * K, b * 512, K, true, xt, span, false, tile.sum + (size_t)b * 16 * rows + 2 * r, rows * 8,
-                             tile.scale + b * rows + r, lane);
+      constexpr int kAhead = 3;  // rows whose loads a warp has in flight
+      for (int i0 = sw; i0 < nb * rows; i0 += kAhead * kStagers) {
+        uint32_t w[kAhead][8];
+#pragma unroll
+        for (int c = 0; c < kAhead; ++c) {
+          const int i = i0 + c * kStagers, b = i / rows, r = i - b * rows;
+          if (i < nb * rows) load_16<true>(w[c], src + (size_t)r * K, b * 512 + 16 * lane, K, true);
+        }
+#pragma unroll
+        for (int c = 0; c < kAhead; ++c) {
+          const int i = i0 + c * kStagers, b = i / rows, r = i - b * rows;
+          if (i >= nb * rows) break;
+          uint8_t* xt = tile.x + (size_t)b * 8 * span + r * 128;
+          if (b16) {
+            uint4 o[2];
+            nibble_order(o, w[c]);
+            uint4* d = reinterpret_cast<uint4*>(xt + (size_t)(lane >> 2) * span + (lane & 3) * 32);
+            d[0] = o[0], d[1] = o[1];
+          } else {
+            stage_row<4>(w[c], xt, span, false, tile.sum + (size_t)b * 16 * rows + 2 * r, rows * 8, tile.scale + b * rows + r, lane);
+          }
         }
       }
       __threadfence_block();

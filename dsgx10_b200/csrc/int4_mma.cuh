@@ -123,14 +123,11 @@ DSGX_DEV void nibble_order(uint4 (&o)[2], const uint32_t (&w)[8]) {
   }
 }
 
-// One row's 512 k of a block into the activation tile, by one warp (16 k a lane): f16 times 2^E; the groups' sums times
+// One row's 512 k of a block into the activation tile, by one warp (w: a lane's 16 k): f16 times 2^E; the groups' sums times
 // 2^(E - 24); 2^(12 - E).  xt: the row's 128-byte line in the block's first span of 64 k, the next span's `span` bytes on; flip:
 // the line's two groups exchanged; sx: the row's first group sum, GB bytes to the span's second, `sspan` to the next span.
-template <int GB, bool kCg>
-DSGX_DEV void stage_row(const __nv_bfloat16* row, int k0, int K, bool vec, uint8_t* xt, uint32_t span, bool flip, float* sx, uint32_t sspan,
-                        float* scale, int lane) {
-  uint32_t w[8];
-  load_16<kCg>(w, row, k0 + 16 * lane, K, vec);
+template <int GB>
+DSGX_DEV void stage_row(const uint32_t (&w)[8], uint8_t* xt, uint32_t span, bool flip, float* sx, uint32_t sspan, float* scale, int lane) {
   uint32_t top = 0;  // the largest finite magnitude's bits
 #pragma unroll
   for (int i = 0; i < 8; ++i) {

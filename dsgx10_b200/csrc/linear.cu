@@ -39,15 +39,15 @@ constexpr int kMaxCluster = 8;
 constexpr int kRuns = 8;         // the parts of K whose sums are joined as a tree
 constexpr size_t kSmemMax = 227 * 1024;
 
-constexpr int kUnitBlk = 4736;    // 16 rows x 512 k
+constexpr int kUnitBlk = 4736;   // 16 rows x 512 k
 
-// S sets of eight rows (kCol: four rows at most, see unit_block4); W stream warps with NST ring stages each, P tasks' sums in flight (a power of two)
-template <int S_, int W_, int NST_, int P_, bool kCol_ = false>
+// W stream warps with NST ring stages each, P tasks' sums in flight (a power of two); kCol: four rows at most (unit_block4)
+template <bool kCol_, int W_, int NST_, int P_>
 struct LinVar {
-  static constexpr int S = S_, W = W_, NST = NST_, P = P_;
+  static constexpr int W = W_, NST = NST_, P = P_;
   static constexpr bool kCol = kCol_;
   static constexpr int kThreads = (W + 1) * 32;
-  static constexpr int kPart = 512 * S;  // bytes of a task's (or a rank's) sums: [S][32 lanes][4] f32
+  static constexpr int kPart = 512;  // bytes of a task's (or a rank's) sums: [32 lanes][4] f32
   static size_t smem(int M, int kblocks, int C) {
     return (size_t)W * NST * kUnitBlk + (size_t)P * kPart + (C > 1 ? (size_t)kSlotsOwned * C * kPart : 0) +
            (size_t)kblocks * (M * 1024 + even(M) * 68) + (kCol ? 256 : 0) + (W * NST + kSlotsOwned * (1 + kMaxCluster)) * 8 + P * 4 + 16 + 128;
@@ -55,22 +55,15 @@ struct LinVar {
   __host__ __device__ static int even(int M) { return (M + 1) & ~1; }
 };
 
-// The products of one block, times 2^(E - 24): blk[s] = a lane's four sums (first strip's row g with rows 8 s + 2 t and + 1 of x,
-// then the second strip's), the spans' first and second groups apart.  st: the stage; x[s], sx[s]: this lane's activations and group sums at the block's first span;
-// span, sspan: bytes from one span to the next.
-template <int S>
-DSGX_DEV void unit_block(float (&blk)[S][4][2], uint32_t st, const uint32_t (&x_at)[S], uint32_t span, const uint32_t (&sx_at)[S], uint32_t sspan,
-                         int lane) {
+// The products of one block, times 2^(E - 24): blk = a lane's four sums (first strip's row g with rows 2 t and 2 t + 1 of x, then
+// the second strip's), the spans' first and second groups apart.  st: the stage; x, sx: this lane's activations and group
+// sums at the block's first span; span, sspan: bytes from one span to the next.
+DSGX_DEV void unit_block8(float (&blk)[4][2], uint32_t st, uint32_t x, uint32_t span, uint32_t sx, uint32_t sspan, int lane) {
   const int g = lane >> 2;
   const uint4 zq = lds_v4(st + 4608 + 16 * g);
   const uint32_t* zw = &zq.x;
-  uint32_t x[S], sx[S];
 #pragma unroll
-  for (int s = 0; s < S; ++s) {
-    x[s] = x_at[s], sx[s] = sx_at[s];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) blk[s][i][0] = blk[s][i][1] = 0.f;
-  }
+  for (int i = 0; i < 4; ++i) blk[i][0] = blk[i][1] = 0.f;
 #pragma unroll
   for (int jj = 0; jj < 4; ++jj) {
     const uint4 sc = lds_v4(st + 4096 + 128 * jj + 16 * g);
@@ -78,31 +71,21 @@ DSGX_DEV void unit_block(float (&blk)[S][4][2], uint32_t st, const uint32_t (&x_
     const uint32_t ze = zw[jj] & 0x0F0F0F0Fu, zo = (zw[jj] >> 4) & 0x0F0F0F0Fu;  // first span's four, second span's four
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      const uint4 w = lds_v4(st + 512 * (2 * jj + q) + 16 * lane);
-      float4 sum[S];  // of the two groups, the lane's two rows each
-#pragma unroll
-      for (int s = 0; s < S; ++s) {
-        const uint4 v = lds_v4(sx[s]);
-        sum[s] = make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
-      }
+      const uint4 w = lds_v4(st + 512 * (2 * jj + q) + 16 * lane), sm = lds_v4(sx);  // (sums: of both groups, the lane's two rows each)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {  // the span's two groups
         const uint32_t wa = c ? w.z : w.x, wb = c ? w.w : w.y, wa8 = wa >> 8, wb8 = wb >> 8;
         const float za = minus_zero(q ? zo : ze, 2 * c), zb = minus_zero(q ? zo : ze, 2 * c + 1);
         const float fa = q ? scale_hi(sw[2 * c]) : scale_lo(sw[2 * c]), fb = q ? scale_hi(sw[2 * c + 1]) : scale_lo(sw[2 * c + 1]);
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-          const uint4 xv = lds_v4(x[s] ^ (c ? 64u : 0u));
-          float d[4];
-          mma_f16_zero(d, wa & kNib0, wb & kNib0, wa & kNib1, wb & kNib1, xv.x, xv.y);
-          mma_f16(d, wa8 & kNib0, wb8 & kNib0, wa8 & kNib1, wb8 & kNib1, xv.z, xv.w);
-          const float s0 = c ? sum[s].z : sum[s].x, s1 = c ? sum[s].w : sum[s].y;
-          blk[s][0][c] = fmaf(fa, fmaf(za, s0, d[0]), blk[s][0][c]), blk[s][1][c] = fmaf(fa, fmaf(za, s1, d[1]), blk[s][1][c]);
-          blk[s][2][c] = fmaf(fb, fmaf(zb, s0, d[2]), blk[s][2][c]), blk[s][3][c] = fmaf(fb, fmaf(zb, s1, d[3]), blk[s][3][c]);
-        }
+        const uint4 xv = lds_v4(x ^ (c ? 64u : 0u));
+        float d[4];
+        mma_f16_zero(d, wa & kNib0, wb & kNib0, wa & kNib1, wb & kNib1, xv.x, xv.y);
+        mma_f16(d, wa8 & kNib0, wb8 & kNib0, wa8 & kNib1, wb8 & kNib1, xv.z, xv.w);
+        const float s0 = __uint_as_float(c ? sm.z : sm.x), s1 = __uint_as_float(c ? sm.w : sm.y);
+        blk[0][c] = fmaf(fa, fmaf(za, s0, d[0]), blk[0][c]), blk[1][c] = fmaf(fa, fmaf(za, s1, d[1]), blk[1][c]);
+        blk[2][c] = fmaf(fb, fmaf(zb, s0, d[2]), blk[2][c]), blk[3][c] = fmaf(fb, fmaf(zb, s1, d[3]), blk[3][c]);
       }
-#pragma unroll
-      for (int s = 0; s < S; ++s) x[s] += span, sx[s] += sspan;
+      x += span, sx += sspan;
     }
   }
 }
@@ -215,22 +198,24 @@ DSGX_DEV float4 add4(float4 a, float4 b) {
 }
 template <class V>
 __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearParams p) {
-  constexpr int S = V::S, W = V::W, NST = V::NST, P = V::P, kPart = V::kPart;
+  constexpr int W = V::W, NST = V::NST, P = V::P, kPart = V::kPart;
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int C = p.cluster;
   const uint32_t rank = C > 1 ? cluster_rank() : 0;
-  const int cl = blockIdx.x / C, ncl = gridDim.x / C;
-  // this cluster's units and this rank's blocks of K
+  // this cluster's rows (more than eight: the clusters of a pair take eight and the rest, over the same units), its units and
+  // this rank's blocks of K
+  const int part_m = p.M > 8 ? (int)(blockIdx.x / C) & 1 : 0, m0 = 8 * part_m, M = p.M > 8 ? (part_m ? p.M - 8 : 8) : p.M;
+  const int cl = blockIdx.x / C >> (p.M > 8), ncl = gridDim.x / C >> (p.M > 8);
   const int u0 = (int)((long long)p.units * cl / ncl), u1 = (int)((long long)p.units * (cl + 1) / ncl);
   const int b0 = p.nb * (int)rank / C, nbk = p.nb * ((int)rank + 1) / C - b0;
 
   uint8_t* ring = smem;
-  uint8_t* part = ring + (size_t)W * NST * kUnitBlk;                   // [P][S][32][4] f32
-  uint8_t* recv = part + (size_t)P * kPart;                            // [kSlotsOwned][C][S][32][4] f32
+  uint8_t* part = ring + (size_t)W * NST * kUnitBlk;                   // [P][32][4] f32
+  uint8_t* recv = part + (size_t)P * kPart;                            // [kSlotsOwned][C][32][4] f32
   uint8_t* xt = recv + (C > 1 ? (size_t)kSlotsOwned * C * kPart : 0);  // [spans][M rows][128 B]
-  const int Me = V::even(p.M);
-  float* xsum = reinterpret_cast<float*>(xt + (size_t)p.xblocks * p.M * 1024);  // [spans][row pairs][2 groups][2 rows]
+  const int Me = V::even(M);
+  float* xsum = reinterpret_cast<float*>(xt + (size_t)p.xblocks * M * 1024);  // [spans][row pairs][2 groups][2 rows]
   float* xscale = xsum + (size_t)p.xblocks * Me * 16;                           // [blocks][rows]: 2^(12 - E)
   uint8_t* zero = smem + (((xscale + (size_t)p.xblocks * Me) - reinterpret_cast<float*>(smem)) * 4 + 127) / 128 * 128;  // kCol: 128 zeros
   uint64_t* bars = reinterpret_cast<uint64_t*>(V::kCol ? zero + 128 : reinterpret_cast<uint8_t*>(xscale + (size_t)p.xblocks * Me));
@@ -291,12 +276,13 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
   // tile: [span of 64 k][row][the span's 8 pieces of 8 f16], a piece = the k a lane's word covers, in the words' nibble order;
   // eight columns: odd rows with the span's two groups exchanged, so that two rows' reads of one group do not meet in the
   // banks.  The groups' sums: a row's two side by side (kCol), or two rows' of a group.
-  const uint32_t span = p.M * 128, sspan = Me * 8;
-  for (int i = warp; i < nbk * p.M; i += W + 1) {
-    const int b = i / p.M, r = i - b * p.M;
-    stage_row<V::kCol ? 4 : 8, false>(p.x + (size_t)r * p.ldx, (b0 + b) * 512, p.K, p.x_vec != 0, xt + (size_t)b * 8 * span + r * 128, span,
-                                      !V::kCol && (r & 1), xsum + (size_t)b * 16 * Me + (V::kCol ? 2 * r : (r >> 1) * 4 + (r & 1)), sspan,
-                                      xscale + b * Me + r, lane);
+  const uint32_t span = M * 128, sspan = Me * 8;
+  for (int i = warp; i < nbk * M; i += W + 1) {
+    const int b = i / M, r = i - b * M;
+    uint32_t w[8];
+    load_16<false>(w, p.x + (size_t)(m0 + r) * p.ldx, (b0 + b) * 512 + 16 * lane, p.K, p.x_vec != 0);
+    stage_row<V::kCol ? 4 : 8>(w, xt + (size_t)b * 8 * span + r * 128, span, !V::kCol && (r & 1),
+                               xsum + (size_t)b * 16 * Me + (V::kCol ? 2 * r : (r >> 1) * 4 + (r & 1)), sspan, xscale + b * Me + r, lane);
   }
   __syncthreads();
 
@@ -304,31 +290,20 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
     // ---- stream warps ---------------------------------------------------------------------------------------------------
     const int g = lane >> 2, t = lane & 3;
     const uint32_t ring_at = smem_u32(myring);
-    uint32_t xl[S], sl[S], fl[S];  // row 8 s + g of the tile (columns without a row: the last row, their sums are not used)
-    uint32_t xz = 0;               // kCol: where the lane reads zeros for the other group
-    const int half = g & 1;
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-      if (V::kCol) {
-        const int r = min(g >> 1, p.M - 1), me = min(t, p.M - 1);
-        xl[s] = smem_u32(xt) + r * 128 + 64 * half + t * 16, xz = smem_u32(zero) + 64 * half + t * 16;
-        sl[s] = smem_u32(xsum) + me * 8, fl[s] = smem_u32(xscale) + me * 4;
-      } else {
-        const int r = min(8 * s + g, p.M - 1), pr = min(4 * s + t, Me / 2 - 1);  // (pr: the pair of rows whose sums the lane holds)
-        xl[s] = smem_u32(xt) + r * 128 + ((t * 16) ^ ((r & 1) * 64));
-        sl[s] = smem_u32(xsum) + pr * 16, fl[s] = smem_u32(xscale) + pr * 8;
-      }
-    }
+    // the lane's column of B is row g of x, or (kCol) row g / 2 in group g % 2; rows past M repeat the last, their sums go unused
+    const int half = g & 1, r = min(V::kCol ? g >> 1 : g, M - 1), me = V::kCol ? min(t, M - 1) : min(t, Me / 2 - 1);
+    const uint32_t xl = smem_u32(xt) + r * 128 + (V::kCol ? 64 * half + t * 16 : (t * 16) ^ ((r & 1) * 64));
+    const uint32_t xz = V::kCol ? smem_u32(zero) + 64 * half + t * 16 : 0u;  // zeros for the other group
+    const uint32_t sl = smem_u32(xsum) + me * (V::kCol ? 8 : 16), fl = smem_u32(xscale) + me * (V::kCol ? 4 : 8);
     uint32_t consumed = 0;
     bool ok = true;
     for (int j = warp; j < total && ok; j += W) {
       const int rt = r0 + (j & (Q - 1)) * RPT;
-      float acc[S][4], lv[3][S][4];  // the run's sums; the subtrees that wait for their right halves
-      int b = p.nb * rt / kRuns, r = 0;
-      for (; r < RPT; ++r) {
+      float acc[4], lv[3][4];  // the run's sums; the subtrees that wait for their right halves
+      int b = p.nb * rt / kRuns;
+      for (int r = 0; r < RPT; ++r) {
         const int e = p.nb * (rt + r + 1) / kRuns;
-#pragma unroll
-        for (int s = 0; s < S; ++s) acc[s][0] = acc[s][1] = acc[s][2] = acc[s][3] = 0.f;
+        acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
         for (; b < e; ++b) {
           const uint32_t si = consumed % NST;
           if (!mbar_wait(mybar + si, (consumed / NST) & 1)) {
@@ -336,27 +311,19 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
             break;
           }
           const int lb = b - b0;
-          const uint32_t st = ring_at + si * kUnitBlk;
+          const uint32_t st = ring_at + si * kUnitBlk, xb = xl + lb * 8 * span, sb = sl + lb * 8 * sspan;
           // the block's sums times 2^(24 - E), in two steps that cannot leave f32's range by themselves
           if constexpr (V::kCol) {
             float2 blk[2];
-            const uint32_t xb = xl[0] + lb * 8 * span;
-            unit_block4(blk, st, half ? xz : xb, half ? xb : xz, half ? 0 : span, half ? span : 0, sl[0] + lb * 8 * sspan, sspan, lane);
-            const float f = lds_f(fl[0] + lb * Me * 4);
-            acc[0][0] = fmaf(__fadd_rn(blk[0].x, blk[0].y) * 4096.f, f, acc[0][0]);
-            acc[0][2] = fmaf(__fadd_rn(blk[1].x, blk[1].y) * 4096.f, f, acc[0][2]);
+            unit_block4(blk, st, half ? xz : xb, half ? xb : xz, half ? 0 : span, half ? span : 0, sb, sspan, lane);
+            const float f = lds_f(fl + lb * Me * 4);
+            acc[0] = fmaf(__fadd_rn(blk[0].x, blk[0].y) * 4096.f, f, acc[0]), acc[2] = fmaf(__fadd_rn(blk[1].x, blk[1].y) * 4096.f, f, acc[2]);
           } else {
-            uint32_t xb[S], sb[S];
-            float blk[S][4][2];
+            float blk[4][2];
+            unit_block8(blk, st, xb, span, sb, sspan, lane);
+            const float2 f = lds_f2(fl + lb * Me * 4);
 #pragma unroll
-            for (int s = 0; s < S; ++s) xb[s] = xl[s] + lb * 8 * span, sb[s] = sl[s] + lb * 8 * sspan;
-            unit_block<S>(blk, st, xb, span, sb, sspan, lane);
-#pragma unroll
-            for (int s = 0; s < S; ++s) {
-              const float2 f = lds_f2(fl[s] + lb * Me * 4);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) acc[s][i] = fmaf(__fadd_rn(blk[s][i][0], blk[s][i][1]) * 4096.f, i & 1 ? f.y : f.x, acc[s][i]);
-            }
+            for (int i = 0; i < 4; ++i) acc[i] = fmaf(__fadd_rn(blk[i][0], blk[i][1]) * 4096.f, i & 1 ? f.y : f.x, acc[i]);
           }
           ++consumed;
           __syncwarp();
@@ -364,37 +331,31 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
         }
         if (!ok) break;
         // run r closes as many waiting subtrees as it has trailing ones
-        auto fold = [&](float (&l)[S][4]) {
+        auto fold = [&](float (&l)[4]) {
 #pragma unroll
-          for (int s = 0; s < S; ++s)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) acc[s][c] = __fadd_rn(l[s][c], acc[s][c]);
+          for (int i = 0; i < 4; ++i) acc[i] = __fadd_rn(l[i], acc[i]);
         };
-        auto keep = [&](float (&l)[S][4]) {
+        auto keep = [&](float (&l)[4]) {
 #pragma unroll
-          for (int s = 0; s < S; ++s)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) l[s][c] = acc[s][c];
+          for (int i = 0; i < 4; ++i) l[i] = acc[i];
         };
-        if (r + 1 == RPT || (r & 1)) {
-          if (r & 1) fold(lv[0]);
-          if ((r & 3) == 3) {
+        if (!(r & 1)) {
+          keep(lv[0]);
+        } else {
+          fold(lv[0]);
+          if ((r & 3) != 3) {
+            keep(lv[1]);
+          } else {
             fold(lv[1]);
             if (r == 7) fold(lv[2]);
             else keep(lv[2]);
-          } else {
-            keep(lv[1]);
           }
-        } else {
-          keep(lv[0]);
         }
       }
       // the sums into the partial buffer, once the unit that had the place has been added up
       if (ok) ok = wait_shared_ge(done, j - P + 1, 100);
       if (!ok) break;
-      float4* d = reinterpret_cast<float4*>(part + (size_t)(j & (P - 1)) * kPart) + lane;
-#pragma unroll
-      for (int s = 0; s < S; ++s) d[32 * s] = make_float4(acc[s][0], acc[s][1], acc[s][2], acc[s][3]);
+      reinterpret_cast<float4*>(part + (size_t)(j & (P - 1)) * kPart)[lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
       __threadfence_block();
       __syncwarp();
       if (lane == 0) atomicAdd(cnt + ((j >> lq) & (P - 1)), 1);
@@ -406,38 +367,32 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
     // ---- the adding warp ------------------------------------------------------------------------------------------------
     const int g = lane >> 2, t = lane & 3, n = u1 - u0, lc = p.lc;
     const int lag = C > 1 ? C * (kSlotsOwned / 2) : 0;  // an owner joins the ranks' sums this many units later
-    float4 a[S];
+    float4 a;
     auto join = [&](const float4* d, int parts) {  // parts sums (1, 2, 4 or 8), as a tree
-      auto two = [&](int i, int s) { return add4(d[i * (kPart / 16) + 32 * s], d[(i + 1) * (kPart / 16) + 32 * s]); };
-#pragma unroll
-      for (int s = 0; s < S; ++s) {
-        if (parts == 1) a[s] = d[32 * s];
-        else if (parts == 2) a[s] = two(0, s);
-        else if (parts == 4) a[s] = add4(two(0, s), two(2, s));
-        else a[s] = add4(add4(two(0, s), two(2, s)), add4(two(4, s), two(6, s)));
-      }
+      auto two = [&](int i) { return add4(d[i * (kPart / 16)], d[(i + 1) * (kPart / 16)]); };
+      if (parts == 1) a = d[0];
+      else if (parts == 2) a = two(0);
+      else if (parts == 4) a = add4(two(0), two(2));
+      else a = add4(add4(two(0), two(2)), add4(two(4), two(6)));
     };
     auto put = [&](int m, int c, float y) {
       if (p.out_f32) reinterpret_cast<float*>(p.out)[(size_t)m * p.ldo + c] = y;
       else reinterpret_cast<__nv_bfloat16*>(p.out)[(size_t)m * p.ldo + c] = __float2bfloat16_rn(y);
     };
     auto write = [&](int unit) {
+      const float v[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-      for (int s = 0; s < S; ++s) {
-        const float v[4] = {a[s].x, a[s].y, a[s].z, a[s].w};
+      for (int e = 0; e < (V::kCol ? 1 : 2); ++e) {
+        if ((V::kCol ? t : 2 * t + e) >= M) continue;
+        const int m = m0 + (V::kCol ? t : 2 * t + e);
+        if (glu) {
+          const int c = 8 * unit + g;
+          if (c < p.N) put(m, c, __fmul_rn(silu(v[e]), v[2 + e]));
+        } else {
 #pragma unroll
-        for (int e = 0; e < (V::kCol ? 1 : 2); ++e) {
-          const int m = V::kCol ? t : 8 * s + 2 * t + e;
-          if (m >= p.M) continue;
-          if (glu) {
-            const int c = 8 * unit + g;
-            if (c < p.N) put(m, c, __fmul_rn(silu(v[e]), v[2 + e]));
-          } else {
-#pragma unroll
-            for (int hi = 0; hi < 2; ++hi) {
-              const int c = 16 * unit + 8 * hi + g;
-              if (c < p.N) put(m, c, p.res ? __fadd_rn(v[2 * hi + e], __bfloat162float(p.res[(size_t)m * p.ldr + c])) : v[2 * hi + e]);
-            }
+          for (int hi = 0; hi < 2; ++hi) {
+            const int c = 16 * unit + 8 * hi + g;
+            if (c < p.N) put(m, c, p.res ? __fadd_rn(v[2 * hi + e], __bfloat162float(p.res[(size_t)m * p.ldr + c])) : v[2 * hi + e]);
           }
         }
       }
@@ -463,8 +418,7 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
           }
           const uint32_t bar = map_rank(smem_u32(rfull + slot), owner);
           const uint32_t to = map_rank(smem_u32(recv) + (uint32_t)((slot * C + (int)rank) * kPart + lane * 16), owner);
-#pragma unroll
-          for (int s = 0; s < S; ++s) st_remote(to + 512 * s, a[s], bar);
+          st_remote(to, a, bar);
         }
       }
       const int o = i - lag;
@@ -526,49 +480,66 @@ cudaError_t resident_clusters(int C, int* n) {
   return cudaSuccess;
 }
 
-// The cluster size: the one whose busiest SM streams the fewest block pairs (ceil(units / clusters) x ceil(blocks / C)),
-// among those whose activations fit shared memory; a larger cluster has to save an eighth to be worth its exchange.
+// The division of a launch: a cluster size C (1, 2, 4, 8) and 15 or 11 stream warps (fewer leave more shared memory to the
+// activations).  What is compared is the busiest SM's block count, ceil(units / clusters) ceil(blocks / C), where eleven warps
+// stream a tenth slower and a cluster's exchange costs a quarter (12288 x 6144 pair, eight rows: 26 us with eleven warps
+// alone, 31 us with fifteen in clusters of two).
+struct Division {
+  long long cost = 0;
+  int C = 0, clusters = 0;
+};
 template <class V>
-cudaError_t launch(LinearParams p, cudaStream_t st, bool* fits) {
-  int best = 0, clusters = 1;
-  long long best_cost = 0;
+cudaError_t divide(const LinearParams& p, Division* best, bool* mine) {
+  const int rows = p.M > 8 ? 8 : p.M, pair = p.M > 8 ? 2 : 1;
   for (int C = 1; C <= kMaxCluster && C <= p.nb; C *= 2) {
     const int kb = (p.nb + C - 1) / C;
-    if (V::smem(p.M, kb, C) > kSmemMax) continue;
+    if (V::smem(rows, kb, C) > kSmemMax) continue;
     int n = 0;
     cudaError_t e = resident_clusters<V>(C, &n);
     if (e != cudaSuccess) return e;
-    const long long cost = (long long)((p.units + n - 1) / n) * kb;
-    if (!best || cost * 8 <= best_cost * 7) best = C, best_cost = cost, clusters = n;
+    n = n / pair > 0 ? n / pair : 1;
+    const long long cost = (long long)((p.units + n - 1) / n) * kb * (V::W > 11 ? 20 : 22) * (C > 1 ? 5 : 4);
+    if (!best->C || cost < best->cost) *best = Division{cost, C, n}, *mine = true;
   }
-  *fits = best != 0;
-  if (!best) return cudaSuccess;
-  p.cluster = best, p.xblocks = (p.nb + best - 1) / best;
-  p.lc = best == 8 ? 3 : best == 4 ? 2 : best == 2 ? 1 : 0;
+  return cudaSuccess;
+}
+
+template <class V>
+cudaError_t launch(LinearParams p, const Division& d, cudaStream_t st) {
+  const int C = d.C, per_cta = (p.units + d.clusters - 1) / d.clusters, rows = p.M > 8 ? 8 : p.M;
+  p.cluster = C, p.lc = C == 8 ? 3 : C == 4 ? 2 : C == 2 ? 1 : 0, p.xblocks = (p.nb + C - 1) / C, p.lq = 0;
   // Tasks a unit: as few as leave every stream warp of a CTA three tasks (the last task of a launch is idle time of the
   // others), at most one a block or a run.
-  const int per_cta = (p.units + clusters - 1) / clusters;
-  p.lq = 0;
-  while ((2 << p.lq) <= kRuns / best && (2 << p.lq) <= p.xblocks && (per_cta << p.lq) < 3 * V::W) ++p.lq;
+  while ((2 << p.lq) <= kRuns / C && (2 << p.lq) <= p.xblocks && (per_cta << p.lq) < 3 * V::W) ++p.lq;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((p.units < clusters ? p.units : clusters) * best), cfg.blockDim = dim3(V::kThreads);
-  cfg.dynamicSmemBytes = V::smem(p.M, p.xblocks, best), cfg.stream = st;
+  cfg.gridDim = dim3((p.units < d.clusters ? p.units : d.clusters) * C * (p.M > 8 ? 2 : 1)), cfg.blockDim = dim3(V::kThreads);
+  cfg.dynamicSmemBytes = V::smem(rows, p.xblocks, C), cfg.stream = st;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = best, at[1].val.clusterDim.y = 1, at[1].val.clusterDim.z = 1;
-  cfg.attrs = at, cfg.numAttrs = best > 1 ? 2 : 1;
+  at[1].val.clusterDim.x = C, at[1].val.clusterDim.y = 1, at[1].val.clusterDim.z = 1;
+  cfg.attrs = at, cfg.numAttrs = C > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, k_linear_int4<V>, p);
 }
 
 }  // namespace
 
-// One launch for M rows, or *fits = false where their activations do not fit shared memory.
+// One launch for M rows, or *fits = false where a row's activations do not fit shared memory.
+template <bool kCol>
+static cudaError_t launch_rows(const LinearParams& p, cudaStream_t st, bool* fits) {
+  using Wide = LinVar<kCol, 15, 2, 32>;
+  using Narrow = LinVar<kCol, 11, 2, 32>;
+  Division d;
+  bool wide = false, narrow = false;
+  cudaError_t e = divide<Wide>(p, &d, &wide);
+  if (e == cudaSuccess) e = divide<Narrow>(p, &d, &narrow);
+  *fits = d.C != 0;
+  if (e != cudaSuccess || !*fits) return e;
+  return narrow ? launch<Narrow>(p, d, st) : launch<Wide>(p, d, st);
+}
 cudaError_t launch_linear_int4(const LinearParams& p, cudaStream_t st, bool* fits) {
-  if (p.M <= 4) return launch<LinVar<1, 15, 2, 32, true>>(p, st, fits);
-  if (p.M <= 8) return launch<LinVar<1, 15, 2, 32>>(p, st, fits);
-  return launch<LinVar<2, 11, 2, 16>>(p, st, fits);
+  return p.M <= 4 ? launch_rows<true>(p, st, fits) : launch_rows<false>(p, st, fits);
 }
 
 size_t linear_bytes(int N, int K, bool glu) {

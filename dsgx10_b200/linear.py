@@ -35,34 +35,58 @@ class LinearW:
             check(lib().dsgx_linear_prepare(blocks.data_ptr(), up.data_ptr() if self.glu else None, _lib.FMT_INT4, N, K, self.data.data_ptr(),
                                             torch.cuda.current_stream(self.device).cuda_stream), "dsgx_linear_prepare")
         self.c = _lib.LinearW(self.data.data_ptr(), N, K, _lib.FMT_INT4, int(self.glu))
+        self.ref = C.byref(self.c)
 
 
-def _rows(t, M, width, what, dtypes, device):
-    if t.dim() != 2 or t.shape[0] != M or t.shape[1] != width or t.dtype not in dtypes or t.device != device:
-        raise ValueError(f"linear_decode: {what} {tuple(t.shape)} of {t.dtype} on {t.device}; wanted ({M}, {width}) of {dtypes} on {device}")
-    if width > 1 and t.stride(1) != 1 or M > 1 and t.stride(0) < width:
-        raise ValueError(f"linear_decode: {what} has strides {t.stride()}: the last dimension must be contiguous")
-    return t.stride(0) if M > 1 else max(t.stride(0), width)
+# (the stream's handle without building a Stream object, where torch has that call: 2 us of a 12 us host call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
+def _lead(t, M, width, what, device):
+    """The leading dimension of a [M][width] operand, checked."""
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != M or shape[1] != width or t.device != device:
+        raise ValueError(f"linear_decode: {what} {tuple(shape)} on {t.device}; wanted ({M}, {width}) on {device}")
+    s0, s1 = t.stride()
+    if (s1 != 1 and width > 1) or (s0 < width and M > 1):
+        raise ValueError(f"linear_decode: {what} has strides {(s0, s1)}: the last dimension must be contiguous, rows apart")
+    return s0 if s0 > width else width
 
 
 def linear_decode(w, x, res=None, out=None, out_dtype=torch.bfloat16, status=None):
     """x bf16 [M][K], M = 1..16 -> out [M][N] (bf16 or f32): x W^T (+ res bf16 [M][N]), or silu(x W^T) * (x Wup^T) where w has
     an `up` matrix.  x, res and out may be rows of larger tensors (last dimension contiguous); out may be res.
     status: an int32 device tensor that gets DSGX_ERR_DEVICE_WAIT where a bounded wait ran out."""
-    if x.dim() != 2:
-        raise ValueError(f"linear_decode: x has shape {tuple(x.shape)}")
-    M, dev = x.shape[0], w.device
-    if not 1 <= M <= _lib.MAX_STEP_ROWS:
-        raise ValueError(f"linear_decode: {M} rows; 1..{_lib.MAX_STEP_ROWS} are taken")
-    ldx = _rows(x, M, w.K, "x", (torch.bfloat16,), dev)
+    dev, bf16 = w.device, torch.bfloat16
+    if x.dim() != 2 or not 1 <= x.shape[0] <= _lib.MAX_STEP_ROWS:
+        raise ValueError(f"linear_decode: x has shape {tuple(x.shape)}; 1..{_lib.MAX_STEP_ROWS} rows of {w.K} are taken")
+    M = x.shape[0]
+    ldx = _lead(x, M, w.K, "x", dev)
     if out is None:
         out = torch.empty(M, w.N, dtype=out_dtype, device=dev)
-    ldo = _rows(out, M, w.N, "out", (torch.bfloat16, torch.float32), dev)
-    ldr = 0 if res is None else _rows(res, M, w.N, "res", (torch.bfloat16,), dev)
+    ldo = _lead(out, M, w.N, "out", dev)
+    ldr, resp = (0, None) if res is None else (_lead(res, M, w.N, "res", dev), res.data_ptr())
+    if x.dtype is not bf16 or (out.dtype is not bf16 and out.dtype is not torch.float32) or (res is not None and res.dtype is not bf16):
+        raise ValueError(f"linear_decode: x {x.dtype}, out {out.dtype}, res {None if res is None else res.dtype}; wanted bf16, out bf16 or f32")
     if status is not None and (status.dtype != torch.int32 or status.device != dev or status.numel() < 1):
         raise ValueError("linear_decode: status is an int32 tensor on the weights' device")
-    with torch.cuda.device(dev):
-        check(lib().dsgx_linear_decode(C.byref(w.c), x.data_ptr(), ldx, M, None if res is None else res.data_ptr(), ldr, out.data_ptr(),
-                                       ldo, int(out.dtype == torch.float32), None if status is None else status.data_ptr(),
-                                       torch.cuda.current_stream(dev).cuda_stream), "dsgx_linear_decode")
+    args = (w.ref, x.data_ptr(), ldx, M, resp, ldr, out.data_ptr(), ldo, 0 if out.dtype is bf16 else 1,
+            None if status is None else status.data_ptr())
+    if torch.cuda.current_device() == dev.index:
+        rc = _decode()(*args, _raw_stream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = _decode()(*args, _raw_stream(dev.index))
+    if rc:
+        check(rc, "dsgx_linear_decode")
     return out
+
+
+_fn = None
+
+
+def _decode():
+    global _fn
+    if _fn is None:
+        _fn = lib().dsgx_linear_decode
+    return _fn

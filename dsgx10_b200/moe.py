@@ -194,19 +194,20 @@ class MoeBlock:
         self.w = torch.empty(_lib.MAX_STEP_ROWS, shp.topk, dtype=torch.float32, device=self.device)
         self.ws = torch.zeros(n, dtype=torch.uint8, device=self.device)
         self.c = _lib.MoeBlock(_ptr(wr), _ptr(bias), _ptr(self.idx), _ptr(self.w), _ptr(self.ws), None)
+        self.ref, self.shp_ref = C.byref(self.c), C.byref(shp)
 
     def run(self, layer_w, x, res=None, out=None):
         """x, res: contiguous bf16 [M][H] -> (out bf16 [M][H], idx int32 [M][topk], w f32 [M][topk]); idx and w are this
         object's buffers, overwritten by the next run.  out may be x or res."""
-        M = x.shape[0]
+        M, dev = x.shape[0], self.device
         if out is None:
             out = torch.empty_like(x)
         for t, what in ((x, "x"), (res, "res"), (out, "out")):
-            if t is not None and (t.dtype != torch.bfloat16 or tuple(t.shape) != (M, self.shp.H) or not t.is_contiguous() or t.device != self.device):
-                raise ValueError(f"MoeBlock: {what} must be contiguous bf16 [M][{self.shp.H}] on {self.device}")
-        with torch.cuda.device(self.device):
-            check(lib().dsgx_moe_block_decode(C.byref(self.shp), C.byref(layer_w), _ptr(x), M, C.byref(self.c), _ptr(res), _ptr(out),
-                                              torch.cuda.current_stream(self.device).cuda_stream), "dsgx_moe_block_decode")
+            if t is not None and (t.dtype is not torch.bfloat16 or t.shape != (M, self.shp.H) or not t.is_contiguous() or t.device != dev):
+                raise ValueError(f"MoeBlock: {what} must be contiguous bf16 [M][{self.shp.H}] on {dev}")
+        with torch.cuda.device(dev):
+            check(lib().dsgx_moe_block_decode(self.shp_ref, C.byref(layer_w), x.data_ptr(), M, self.ref, _ptr(res), out.data_ptr(),
+                                              torch.cuda.current_stream(dev).cuda_stream), "dsgx_moe_block_decode")
         return out, self.idx[:M], self.w[:M]
 
 
