@@ -2,8 +2,9 @@
 // SwiGLU, down, the bf16 shared expert, the weighted sum in ascending expert id, the residual, the rounding.
 //
 // Bound: the weights of the distinct picked experts are read once, so HBM.  One CTA a SM, launched cooperatively (all resident
-// together, so CTAs may wait for one another; every wait is bounded and a run-out is recorded in the workspace).  Twelve
-// warps compute: eleven stream weights through private rings of bulk copies, one joins their sums; four prepare activations.
+// together, so CTAs may wait for one another; every wait is bounded and a run-out is recorded in the workspace).  Of a
+// CTA's warps W stream weights through private rings of bulk copies, one joins their sums and one keeps track of what the other
+// CTAs have done; whoever is free turns activations into the MMAs' operands.
 //
 //   front    every CTA but the last M: the router's logit slices (route.cuh's order).  The last M CTAs route a row each; the
 //            last of them builds the step's table: the picked experts in ascending id with the rows that picked them.
@@ -61,7 +62,6 @@ struct BlockSync {
 
 namespace {
 
-constexpr int kStreamW = 11, kStageW0 = kStreamW + 1, kWarps = 16, kStagers = kWarps - kStageW0, kThreads = kWarps * 32;
 constexpr int kStage = 2 * kQBlk;        // a ring stage: an INT4 block pair (a pair of bf16 blocks, 4096 B, fits)
 constexpr int kFront = 300 * 1024;       // bytes an SM streams from the end of the logits until the table is known (7 us)
 constexpr int kP = 16;                   // tasks' sums in flight
@@ -91,7 +91,7 @@ struct Seg {
 DSGX_DEV int tasks_of(int nb) { return nb <= 1 ? 1 : nb / 2 < 8 ? nb / 2 : 8; }  // tasks a unit
 
 // ---- the tile of activations: [nb x 8 spans][rows][128 B], then group sums [spans][rows][2], then scales [nb][rows]
-__host__ __device__ inline size_t tile_bytes(int K, int rows) { return (size_t)K / 512 * rows * (1024 + 64 + 4) + 16; }
+__host__ __device__ inline size_t tile_bytes(int K, int rows) { return ((size_t)K / 512 * rows * (1024 + 64 + 4) + 127) & ~(size_t)127; }
 struct Tile {
   uint8_t* x;
   float *sum, *scale;
@@ -234,8 +234,16 @@ DSGX_DEV void build_block_tab(BlockTab* out, int* s_idx, int* s_first, const Blo
   }
 }
 
-template <int NST>
-__global__ void __launch_bounds__(kThreads, 1) k_block(const BlockParams p) {
+// W stream warps with NST ring stages each, the joining warp, the control warp, and the rest of sixteen help with activations
+// (sixteen: the routing wants a thread an expert)
+template <int W_, int NST_>
+struct BlkVar {
+  static constexpr int W = W_, NST = NST_, kThreads = 512;
+};
+
+template <class V>
+__global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
+  constexpr int kStreamW = V::W, NST = V::NST, kThreads = V::kThreads, kLogitW = kStreamW + 1;
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int G = gridDim.x, cta = blockIdx.x;
@@ -246,11 +254,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const BlockParams p) {
   uint8_t* tiles = reinterpret_cast<uint8_t*>(&tab + 1);  // [nbuf] activation tiles
   uint8_t* zero = tiles + (size_t)p.nbuf * p.tile + 16;   // 32 bytes, off the banks that the tile's lines use
   uint64_t* bars = reinterpret_cast<uint64_t*>(zero + 48);
-  uint64_t* tile_full = bars + kStreamW * NST;            // [kMaxSegs] the segment's activations are in their tile
+  uint64_t* seg_open = bars + kStreamW * NST;             // [kMaxSegs] the segment's activations exist and their tile is free
+  uint64_t* tile_full = seg_open + kMaxSegs;              // [kMaxSegs] they are in the tile (an arrival a row and block)
   uint64_t* tile_free = tile_full + kMaxSegs;             // [kMaxSegs] no stream warp reads them any more
   uint64_t* tabbar = tile_free + kMaxSegs;                // the table and all segments are known
   Seg* segs = reinterpret_cast<Seg*>(tabbar + 2);
-  int* cnt = reinterpret_cast<int*>(segs + kMaxSegs);     // [kP] tasks summed of a unit in flight
+  int* claim = reinterpret_cast<int*>(segs + kMaxSegs);   // [kMaxSegs] rows and blocks that a warp has taken on
+  int* cnt = claim + kMaxSegs;                            // [kP] tasks summed of a unit in flight
   int* done = cnt + kP;                                   // tasks whose unit has been joined
   int* s_nseg = done + 1;
   int* s_fail = done + 2;
@@ -259,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const BlockParams p) {
 
   if (warp < kStreamW && lane == 0)
     for (int s = 0; s < NST; ++s) mbar_init(bars + warp * NST + s, 1);
-  for (int i = threadIdx.x; i < kMaxSegs; i += kThreads) mbar_init(tile_full + i, kStagers), mbar_init(tile_free + i, kStreamW);
+  for (int i = threadIdx.x; i < kMaxSegs; i += kThreads) mbar_init(seg_open + i, 1), mbar_init(tile_free + i, kStreamW), claim[i] = 0;
   if (threadIdx.x < kP) cnt[threadIdx.x] = 0;
   if (threadIdx.x < 8) reinterpret_cast<uint32_t*>(zero)[threadIdx.x] = 0;
 
@@ -272,6 +282,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const BlockParams p) {
     mbar_init(tabbar, 1);
     *done = 0, *s_nseg = 0, *s_fail = 0;
     segs[0] = Seg{0, 1, kShared, p.M, a0, a1 - a0, (a1 - a0) * QH, 0};
+    mbar_init(tile_full, p.M * nbH);
+    if (a1 > a0) mbar_init(tile_full + 1, p.M * nbH);  // (the down segments' are set when they are known, each once)
   }
   mbar_fence_init();
   __syncthreads();
@@ -360,19 +372,51 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const BlockParams p) {
       *s_fail = 1;
     }
     __syncthreads();
-  } else if (warp < kStageW0) {
+  } else if (warp < kLogitW) {
     // ---- the router's logit slices, one warp a (expert, 1024 k); a CTA reports when all of its are in memory.  (The rings
     // filled first: 2.4 us later logits and not a microsecond gained on the shared expert.) ------------------------------------
     const int KS = (p.H + 1023) / 1024, ntask = p.E * KS;
     int i = warp * Gs + cta;
-    for (; i < ntask; i += kStageW0 * Gs) logit_slice_task(p.x, p.wr, p.M, p.H, p.E, i / KS, i % KS, p.lpart, lane);
+    for (; i < ntask; i += kLogitW * Gs) logit_slice_task(p.x, p.wr, p.M, p.H, p.E, i / KS, i % KS, p.lpart, lane);
     __threadfence();
-    asm volatile("bar.sync 1, %0;" ::"n"(kStageW0 * 32) : "memory");
+    asm volatile("bar.sync 1, %0;" ::"n"(kLogitW * 32) : "memory");
     if (threadIdx.x == 0) {
       __threadfence();
       atomicAdd(&sy->cnt_lp, 1);
     }
   }
+
+  // ---- a segment's activation tile: the shared expert's x, the routed experts' x, then the down segments in the first tile's place
+  auto tile_at = [&](int k) { return tiles + (k <= nb_first ? (k == nb_first ? (p.nbuf - 1) * p.tile : 0) : (k - nb_first - 1) % p.nbuf_down * p.tile_down); };
+  // every warp that waits for a segment takes on some of its rows and blocks first
+  auto prepare = [&](int k, bool b16, int down, int slot, int rows) {
+    if (!mbar_wait(seg_open + k, 0, 20)) return false;
+    const int nb = down ? nbI : nbH, K = down ? p.I : p.H, items = nb * rows;
+    const Tile tile(tile_at(k), nb, rows);
+    const __nv_bfloat16* src = down ? p.h + (size_t)slot * kMaxRows * p.I : p.x;
+    const uint32_t span = rows * 128;
+    for (;;) {
+      int i = 0;
+      if (lane == 0) i = atomicAdd(claim + k, 1);
+      i = __shfl_sync(0xffffffffu, i, 0);
+      if (i >= items) return true;
+      const int b = i / rows, r = i - b * rows;
+      uint8_t* xt = tile.x + (size_t)b * 8 * span + r * 128;
+      uint32_t w[8];
+      load_16<true>(w, src + (size_t)r * K, b * 512 + 16 * lane, K, true);
+      if (b16) {
+        uint4 o[2];
+        nibble_order(o, w);
+        uint4* d = reinterpret_cast<uint4*>(xt + (size_t)(lane >> 2) * span + (lane & 3) * 32);
+        d[0] = o[0], d[1] = o[1];
+      } else {
+        stage_row<4>(w, xt, span, false, tile.sum + (size_t)b * 16 * rows + 2 * r, rows * 8, tile.scale + b * rows + r, lane);
+      }
+      __threadfence_block();
+      __syncwarp();
+      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(tile_full + k)) : "memory");
+    }
+  };
 
   if (warp < kStreamW) {
     // ---- stream warps --------------------------------------------------------------------------------------------------------
@@ -391,18 +435,22 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const BlockParams p) {
     };
 
     for (int k = 0; ok; ++k) {
-      if (k >= nb_first) {  // (the table is needed from here on)
+      if (k <= nb_first && !prepare(k, k < nb_first || p.b16, 0, 0, p.M)) {  // (x needs no table)
+        ok = false;
+        break;
+      }
+      if (k >= nb_first) {  // (the units do, from here on)
         if (k == nb_first && !mbar_wait(tabbar, 0, 20)) ok = false;
         if (!ok || *s_fail || k >= *s_nseg) break;
         if (lane == 0) fill();
       }
       const Seg s = segs[k];
-      if (!mbar_wait(tile_full + k, 0, 20)) {
+      if ((k > nb_first && !prepare(k, s.b16, 1, s.slot, s.rows)) || !mbar_wait(tile_full + k, 0, 20)) {
         ok = false;
         break;
       }
       const int Q = s.down ? QI : QH, nb = s.down ? nbI : nbH;
-      const Tile tile(tiles + (size_t)(k % p.nbuf) * p.tile, nb, s.rows);
+      const Tile tile(tile_at(k), nb, s.rows);
       const uint32_t span = s.rows * 128, x0 = smem_u32(tile.x), z0 = smem_u32(zero);
       for (int i = first_task(s); i < s.tasks && ok; i += kStreamW) {
         const int u = s.u0 + i / Q, q = i % Q, b0 = nb * q / Q, b1 = nb * (q + 1) / Q;
@@ -539,91 +587,87 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const BlockParams p) {
     } else {
       *s_fail = 1;
     }
-  } else {
-    // ---- the staging warps: the table, then every segment's activations ---------------------------------------------------------
-    const int sw = warp - kStageW0;
-    auto stage = [&](int k, bool b16, int rows, int nb, const __nv_bfloat16* src, int K) {
-      const Tile tile(tiles + (size_t)(k % p.nbuf) * p.tile, nb, rows);
-      const uint32_t span = rows * 128;
-      constexpr int kAhead = 3;  // rows whose loads a warp has in flight
-      for (int i0 = sw; i0 < nb * rows; i0 += kAhead * kStagers) {
-        uint32_t w[kAhead][8];
-#pragma unroll
-        for (int c = 0; c < kAhead; ++c) {
-          const int i = i0 + c * kStagers, b = i / rows, r = i - b * rows;
-          if (i < nb * rows) load_16<true>(w[c], src + (size_t)r * K, b * 512 + 16 * lane, K, true);
-        }
-#pragma unroll
-        for (int c = 0; c < kAhead; ++c) {
-          const int i = i0 + c * kStagers, b = i / rows, r = i - b * rows;
-          if (i >= nb * rows) break;
-          uint8_t* xt = tile.x + (size_t)b * 8 * span + r * 128;
-          if (b16) {
-            uint4 o[2];
-            nibble_order(o, w[c]);
-            uint4* d = reinterpret_cast<uint4*>(xt + (size_t)(lane >> 2) * span + (lane & 3) * 32);
-            d[0] = o[0], d[1] = o[1];
-          } else {
-            stage_row<4>(w[c], xt, span, false, tile.sum + (size_t)b * 16 * rows + 2 * r, rows * 8, tile.scale + b * rows + r, lane);
-          }
-        }
+  } else if (warp > kStreamW + 1) {
+    // ---- helpers (the narrow variant's): their share of every segment's activations
+    bool ok = true;
+    for (int k = 0; ok; ++k) {
+      if (k > nb_first) {
+        if (k == nb_first + 1) ok = mbar_wait(tabbar, 0, 20);
+        if (!ok || *s_fail || k >= *s_nseg) break;
       }
-      __threadfence_block();
+      ok = k <= nb_first ? prepare(k, k < nb_first || p.b16, 0, 0, p.M) : prepare(k, segs[k].b16, 1, segs[k].slot, segs[k].rows);
+    }
+    if (!ok) *s_fail = 1;
+  } else {
+    // ---- the control warp: opens the segments, the table when it is there ------------------------------------------------------
+    auto open_seg = [&](int k) {
+      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(seg_open + k)) : "memory");
       __syncwarp();
-      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(tile_full + k)) : "memory");
     };
     bool ok = true;
-    // x: for the shared expert in bf16, for the routed ones as their format wants it
+    // x: in bf16 for the shared expert, as their format wants it for the routed ones
     for (int k = 0; k <= nb_first && ok; ++k) {
-      if (k >= p.nbuf) ok = mbar_wait(tile_free + k - p.nbuf, 0, 20);
-      if (ok) stage(k, k < nb_first || p.b16, p.M, nbH, p.x, p.H);
+      if (k > 0 && p.nbuf == 1) ok = mbar_wait(tile_free, 0, 20);
+      open_seg(k);
+      if (ok) ok = prepare(k, k < nb_first || p.b16, 0, 0, p.M);
     }
     // the table, and from it this CTA's segments
     int got = 0;
     if (lane == 0) got = ok && !*s_fail && poll_near(&sy->tab_ready, 1);
-    got = __shfl_sync(0xffffffffu, got, 0);
-    if (got) {
+    ok = __shfl_sync(0xffffffffu, got, 0) != 0;
+    if (ok) {
       const int n16 = (int)(offsetof(BlockTab, ent) + min(p.M * p.topk, kMaxEnt) * sizeof(BlockEnt)) / 16;
-      for (int i = sw * 32 + lane; i < n16; i += kStagers * 32) reinterpret_cast<uint4*>(&tab)[i] = __ldcg(reinterpret_cast<const uint4*>(p.tab) + i);
-      __threadfence_block();
-    } else {
-      ok = false;
-      *s_fail = 1;
-    }
-    asm volatile("bar.sync 4, %0;" ::"n"(kStagers * 32) : "memory");
-    if (sw == 0) {
-      if (!*s_fail) {
-        // costs of 8 rows x 512 k in 64 bytes; lanes 0 and 1: this CTA's and the next one's first up unit, 2 and 3: down
-        const int cI = p.b16 ? 4 * kHBlk / 64 : kQBlk / 64, cS = 4 * kHBlk / 64, up = lane < 2;
-        const int NU = tab.nslots * upp, ND = tab.nslots * NT, nsh = has_sh ? upp : 0, nd = has_sh ? NT : 0;
-        const int at = routed_begin(cta + (lane & 1), up ? NU : ND, cI, up ? nsh : nd, cS, up ? Gs : G, G, up ? kFront / (64 * nbH) : 0);
-        const int u0 = __shfl_sync(0xffffffffu, at, 0), u1 = __shfl_sync(0xffffffffu, at, 1);
-        const int d0 = __shfl_sync(0xffffffffu, at, 2), d1 = __shfl_sync(0xffffffffu, at, 3);
-        if (lane == 0) {
-          int nseg = nb_first, base = (a1 - a0) * QH;
-          segs[nseg++] = Seg{0, p.b16, 0, p.M, u0, u1 - u0, (u1 - u0) * QH, base}, base += (u1 - u0) * QH;
-          const int s0 = shared_begin(cta, nd, G), s1 = shared_begin(cta + 1, nd, G);
-          if (s1 > s0) segs[nseg++] = Seg{1, 1, kShared, p.M, s0, s1 - s0, (s1 - s0) * QI, base}, base += (s1 - s0) * QI;
-          for (int d = d0; d < d1;) {
-            const int slot = d / NT, e = min(d1, (slot + 1) * NT);
-            segs[nseg++] = Seg{1, p.b16, slot, tab.ent[slot].n, d - slot * NT, e - d, (e - d) * QI, base}, base += (e - d) * QI;
-            d = e;
-          }
-          *s_nseg = nseg;
+      for (int i0 = lane; i0 < n16; i0 += 128) {
+        uint4 v[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (i0 + 32 * c < n16) v[c] = __ldcg(reinterpret_cast<const uint4*>(p.tab) + i0 + 32 * c);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (i0 + 32 * c < n16) reinterpret_cast<uint4*>(&tab)[i0 + 32 * c] = v[c];
+      }
+      __syncwarp();
+      // costs of 8 rows x 512 k in 64 bytes; lanes 0 and 1: this CTA's and the next one's first up unit, 2 and 3: down
+      const int cI = p.b16 ? 4 * kHBlk / 64 : kQBlk / 64, cS = 4 * kHBlk / 64, up = lane < 2;
+      const int NU = tab.nslots * upp, ND = tab.nslots * NT, nsh = has_sh ? upp : 0, nd = has_sh ? NT : 0;
+      const int at = routed_begin(cta + (lane & 1), up ? NU : ND, cI, up ? nsh : nd, cS, up ? Gs : G, G, up ? kFront / (64 * nbH) : 0);
+      const int u0 = __shfl_sync(0xffffffffu, at, 0), u1 = __shfl_sync(0xffffffffu, at, 1);
+      const int d0 = __shfl_sync(0xffffffffu, at, 2), d1 = __shfl_sync(0xffffffffu, at, 3);
+      if (lane == 0) {
+        int nseg = nb_first, base = (a1 - a0) * QH;
+        segs[nseg++] = Seg{0, p.b16, 0, p.M, u0, u1 - u0, (u1 - u0) * QH, base}, base += (u1 - u0) * QH;
+        const int s0 = shared_begin(cta, nd, G), s1 = shared_begin(cta + 1, nd, G);
+        if (s1 > s0) {
+          mbar_init(tile_full + nseg, p.M * nbI);
+          segs[nseg++] = Seg{1, 1, kShared, p.M, s0, s1 - s0, (s1 - s0) * QI, base}, base += (s1 - s0) * QI;
         }
+        for (int d = d0; d < d1;) {
+          const int slot = d / NT, e = min(d1, (slot + 1) * NT), n = tab.ent[slot].n;
+          mbar_init(tile_full + nseg, n * nbI);
+          segs[nseg++] = Seg{1, p.b16, slot, n, d - slot * NT, e - d, (e - d) * QI, base}, base += (e - d) * QI;
+          d = e;
+        }
+        *s_nseg = nseg;
       }
       __threadfence_block();
-      __syncwarp();
-      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(tabbar)) : "memory");
+    } else {
+      *s_fail = 1;
     }
-    if (ok) ok = mbar_wait(tabbar, 0, 20);
-    for (int k = nb_first + 1; ok && !*s_fail && k < *s_nseg; ++k) {
-      const Seg s = segs[k];
-      if (k >= p.nbuf) ok = mbar_wait(tile_free + k - p.nbuf, 0, 20);
+    __syncwarp();
+    if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(tabbar)) : "memory");
+    __syncwarp();
+    const int nseg = ok ? *s_nseg : 0;
+    for (int k = nb_first + 1; ok && k < nseg; ++k) {
+      // the tile: the first tile's place (one tile: once the routed experts' x is done with), then the segments' before
+      const int j = k - nb_first - 1, before = j >= p.nbuf_down ? k - p.nbuf_down : p.nbuf == 1 ? nb_first : nb_first - 1;
+      if (before >= 0) ok = mbar_wait(tile_free + before, 0, 20);
       int there = 0;  // the slot's h, once all of its units are in memory
-      if (lane == 0) there = ok && poll_near(&sy->cnt_h[s.slot], upp);
-      if (!(ok = __shfl_sync(0xffffffffu, there, 0) != 0)) break;
-      stage(k, s.b16, s.rows, nbI, p.h + (size_t)s.slot * kMaxRows * p.I, p.I);
+      if (lane == 0) there = ok && poll_near(&sy->cnt_h[segs[k].slot], upp);
+      ok = __shfl_sync(0xffffffffu, there, 0) != 0;
+      if (ok) {
+        open_seg(k);
+        ok = prepare(k, segs[k].b16, 1, segs[k].slot, segs[k].rows);
+      }
     }
     if (!ok) *s_fail = 1;
   }
@@ -670,34 +714,35 @@ __global__ void __launch_bounds__(kThreads, 1) k_block(const BlockParams p) {
   }
 }
 
-template <int NST>
+template <class V>
 size_t block_smem(size_t tile, int nbuf) {
-  return (size_t)kStreamW * NST * kStage + kP * kPart + sizeof(BlockTab) + nbuf * tile + 64 + (kStreamW * NST + 2 * kMaxSegs + 2) * 8 +
-         kMaxSegs * sizeof(Seg) + (kP + 4) * 4 + 16;
+  return (size_t)V::W * V::NST * kStage + kP * kPart + sizeof(BlockTab) + nbuf * tile + 64 + (V::W * V::NST + 3 * kMaxSegs + 2) * 8 +
+         kMaxSegs * (sizeof(Seg) + 4) + (kP + 4) * 4 + 16;
 }
 size_t block_tile(int H, int I, int M) {
   size_t t = tile_bytes(H, M) > tile_bytes(I, M) ? tile_bytes(H, M) : tile_bytes(I, M);
-  t = t > sizeof(RouteSmem) ? t : sizeof(RouteSmem);  // (the routing's scratch before the first tile)
-  return (t + 127) & ~(size_t)127;
+  return t > sizeof(RouteSmem) ? t : (sizeof(RouteSmem) + 127) & ~(size_t)127;  // (the routing's scratch before the first tile)
 }
 
-template <int NST>
+template <class V>
 cudaError_t launch(const BlockParams& p, cudaStream_t st) {
   static std::atomic<bool> done[64];  // (per device; two host threads may both set the attribute: harmless)
   int dev = 0;
   cudaGetDevice(&dev);
   if (!done[dev & 63].load(std::memory_order_acquire)) {
-    cudaError_t e = cudaFuncSetAttribute(k_block<NST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMax);
+    cudaError_t e = cudaFuncSetAttribute(k_block<V>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMax);
     if (e != cudaSuccess) return e;
     done[dev & 63].store(true, std::memory_order_release);
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(sm_count()), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = block_smem<NST>(p.tile, p.nbuf), cfg.stream = st;
+  cfg.gridDim = dim3(sm_count()), cfg.blockDim = dim3(V::kThreads), cfg.dynamicSmemBytes = block_smem<V>(p.tile, p.nbuf), cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeCooperative, at[0].val.cooperative = 1;
   cfg.attrs = at, cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k_block<NST>, p);
+  return cudaLaunchKernelEx(&cfg, k_block<V>, p);
 }
+using Wide = BlkVar<14, 2>;
+using Narrow = BlkVar<11, 2>;  // (leaves more shared memory to the activations)
 
 size_t al256(size_t v) { return (v + 255) & ~(size_t)255; }
 
@@ -711,8 +756,8 @@ size_t block_ws_bytes(int H, int I) {
 // The rows of one launch: as many of M as the activations' shared memory holds (every row's weights are streamed once a launch).
 int block_rows(int H, int I, int M) {
   int r = M < kMaxRows ? M : kMaxRows;
-  while (r > 1 && block_smem<2>(block_tile(H, I, r), 1) > kSmemMax) r = (r + 1) / 2;
-  return block_smem<2>(block_tile(H, I, r), 1) > kSmemMax || sm_count() < 2 * kMaxRows ? 0 : r;
+  while (r > 1 && block_smem<Narrow>(block_tile(H, I, r), 1) > kSmemMax) r = (r + 1) / 2;
+  return block_smem<Narrow>(block_tile(H, I, r), 1) > kSmemMax || sm_count() < 2 * kMaxRows ? 0 : r;
 }
 
 cudaError_t launch_block_int4(BlockParams p, void* ws, cudaStream_t st) {
@@ -723,12 +768,12 @@ cudaError_t launch_block_int4(BlockParams p, void* ws, cudaStream_t st) {
   p.lpart = reinterpret_cast<float*>(w), w += al256((size_t)((p.H + 1023) / 1024) * kMaxRows * 512 * 4);
   p.h = reinterpret_cast<__nv_bfloat16*>(w), w += al256((size_t)(kMaxEnt + 1) * kMaxRows * p.I * 2);
   p.y = reinterpret_cast<float*>(w);
-  p.tile = block_tile(p.H, p.I, p.M);
-  // two tiles (the next segment's activations are prepared while the present ones are in use) and three ring stages where
-  // they fit, in this order
-  p.nbuf = block_smem<2>(p.tile, 2) <= kSmemMax ? 2 : 1;
-  if (p.nbuf == 2 && block_smem<3>(p.tile, 2) <= kSmemMax) return launch<3>(p, st);
-  return launch<2>(p, st);
+  // Two tiles where they fit (the routed experts' activations are prepared while the shared expert's are in use), and the wide
+  // variant where it fits.
+  p.tile = block_tile(p.H, p.I, p.M), p.tile_down = tile_bytes(p.I, p.M), p.nbuf_down = 2 * p.tile_down <= p.tile ? 2 : 1;
+  const bool wide = block_smem<Wide>(p.tile, 1) <= kSmemMax;
+  p.nbuf = (wide ? block_smem<Wide>(p.tile, 2) : block_smem<Narrow>(p.tile, 2)) <= kSmemMax ? 2 : 1;
+  return wide ? launch<Wide>(p, st) : launch<Narrow>(p, st);
 }
 
 }  // namespace dsgx

@@ -91,6 +91,18 @@ DSGX_DEV float2 add2(float2 a, float2 b) {
   return d;
 }
 
+DSGX_DEV float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+DSGX_DEV __nv_bfloat162 abs_bf16x2(uint32_t w) {
+  w &= 0x7FFF7FFFu;
+  return *reinterpret_cast<const __nv_bfloat162*>(&w);
+}
+
 constexpr uint32_t kNib0 = 0x000F000Fu, kNib1 = 0x00F000F0u;  // nibbles 0 and 4 of a word; 1 and 5 (2, 6 and 3, 7 after a shift by 8)
 // minus the zero point in byte b of a word of them: 0x4B0000zz is 2^23 + z
 DSGX_DEV float minus_zero(uint32_t zeros, int b) { return 8388608.f - __uint_as_float(__byte_perm(zeros, 0x4B000000u, 0x7440u + b)); }
@@ -123,28 +135,39 @@ DSGX_DEV void nibble_order(uint4 (&o)[2], const uint32_t (&w)[8]) {
   }
 }
 
-// One row's 512 k of a block into the activation tile, by one warp (w: a lane's 16 k): f16 times 2^E; the groups' sums times
-// 2^(E - 24); 2^(12 - E).  xt: the row's 128-byte line in the block's first span of 64 k, the next span's `span` bytes on; flip:
-// the line's two groups exchanged; sx: the row's first group sum, GB bytes to the span's second, `sspan` to the next span.
+// One row's 512 k of a block into the activation tile, by one warp (w: a lane's 16 k): f16 times 2^E; the groups' sums times 2^(E - 24); 2^(12 - E).
+// xt: the row's 128-byte line in the block's first span of 64 k, the next span's `span` bytes on; flip: its two groups exchanged; sx: the row's first group sum, GB bytes to the span's second, `sspan` to the next span.
 template <int GB>
 DSGX_DEV void stage_row(const uint32_t (&w)[8], uint8_t* xt, uint32_t span, bool flip, float* sx, uint32_t sspan, float* scale, int lane) {
-  uint32_t top = 0;  // the largest finite magnitude's bits
+  // the largest magnitude (bf16 bits order like numbers; a NaN loses against a number) of the row's 512 values
+  __nv_bfloat162 m2 = abs_bf16x2(w[0]);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t lo = w[i] & 0x7FFFu, hi = w[i] >> 16 & 0x7FFFu;
-    top = max(top, max(lo < 0x7F80u ? lo : 0u, hi < 0x7F80u ? hi : 0u));
+  for (int i = 1; i < 8; ++i) m2 = __hmax2(m2, abs_bf16x2(w[i]));
+  const uint32_t mb = *reinterpret_cast<const uint32_t*>(&m2);
+  uint32_t top = __reduce_max_sync(0xffffffffu, max(mb & 0xffffu, mb >> 16));
+  if (top >= 0x7F80u) {  // an infinity, or nothing but NaN: the largest finite one
+    top = 0;
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t lo = w[i] & 0x7FFFu, hi = w[i] >> 16 & 0x7FFFu;
+      top = max(top, max(lo < 0x7F80u ? lo : 0u, hi < 0x7F80u ? hi : 0u));
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
   }
-  top = __reduce_max_sync(0xffffffffu, top);
   const int E = top >= 0x80u ? min(14 + 127 - (int)(top >> 7), 126) : 126;  // (subnormal or zero: as small as it gets)
-  const float even = __uint_as_float((uint32_t)(E + 127) << 23), off = __uint_as_float((uint32_t)(E - 4 + 127) << 23);
+  const float2 f = make_float2(__uint_as_float((uint32_t)(E + 127) << 23), __uint_as_float((uint32_t)(E - 4 + 127) << 23));
   uint32_t h[8];
-  float sum = 0.f;
+  float2 v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const __half lo = __float2half_rn(bf16_bits_to_f(w[i] & 0xffffu) * even), hi = __float2half_rn(bf16_bits_to_f(w[i] >> 16) * off);
-    sum = __fadd_rn(__fadd_rn(sum, __half2float(lo)), __half2float(hi) * 16.f);
-    h[i] = (uint32_t)__half_as_ushort(lo) | (uint32_t)__half_as_ushort(hi) << 16;
+    v[i] = mul2(make_float2(scale_lo(w[i]), scale_hi(w[i])), f);
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h[i]) : "f"(v[i].y), "f"(v[i].x));
   }
+#pragma unroll
+  for (int n = 4; n > 0; n >>= 1)
+#pragma unroll
+    for (int i = 0; i < n; ++i) v[i] = add2(v[i], v[i + n]);
+  float sum = fmaf(v[0].y, 16.f, v[0].x);
   sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, 1));
   uint4 o[2];
   nibble_order(o, h);

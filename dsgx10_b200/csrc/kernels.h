@@ -186,8 +186,8 @@ struct BlockParams {
   float* lpart;        // [H / 1024 slices][8][E] partial router logits
   __nv_bfloat16* h;    // [64 + 1 slots][8][I]
   float* y;            // [64 + 1 slots][8][H]
-  size_t tile;         // bytes of an activation tile in shared memory
-  int nbuf;
+  size_t tile, tile_down;  // bytes of an activation tile in shared memory; of one of a down segment
+  int nbuf, nbuf_down;     // tiles of x; tiles of h in the first one's place
 };
 size_t block_ws_bytes(int H, int I);
 int block_rows(int H, int I, int M);  // rows one launch takes (0: the shape does not fit)
