@@ -3,8 +3,8 @@
 //
 // Bound: the weights of the distinct picked experts are read once, so HBM.  One CTA a SM, launched cooperatively (all resident
 // together, so CTAs may wait for one another; every wait is bounded and a run-out is recorded in the workspace).  Of a
-// CTA's warps W stream weights through private rings of bulk copies, one joins their sums and one keeps track of what the other
-// CTAs have done; whoever is free turns activations into the MMAs' operands.
+// CTA's warps W stream weights, each from a ring of bulk copies that one warp fills for all, one joins their sums and one keeps
+// track of what the other CTAs have done; whoever is free turns activations into the MMAs' operands.
 //
 //   front    every CTA but the last M: the router's logit slices (route.cuh's order).  The last M CTAs route a row each; the
 //            last of them builds the step's table: the picked experts in ascending id with the rows that picked them.
@@ -234,8 +234,8 @@ DSGX_DEV void build_block_tab(BlockTab* out, int* s_idx, int* s_first, const Blo
   }
 }
 
-// W stream warps with NST ring stages each, the joining warp, the control warp, and the rest of sixteen help with activations
-// (sixteen: the routing wants a thread an expert)
+// W stream warps with NST ring stages each, the joining warp, the control warp, the producer, and the rest of sixteen help with
+// activations (sixteen: the routing wants a thread an expert)
 template <int W_, int NST_>
 struct BlkVar {
   static constexpr int W = W_, NST = NST_, kThreads = 512;
@@ -254,12 +254,14 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
   uint8_t* tiles = reinterpret_cast<uint8_t*>(&tab + 1);  // [nbuf] activation tiles
   uint8_t* zero = tiles + (size_t)p.nbuf * p.tile + 16;   // 32 bytes, off the banks that the tile's lines use
   uint64_t* bars = reinterpret_cast<uint64_t*>(zero + 48);
-  uint64_t* seg_open = bars + kStreamW * NST;             // [kMaxSegs] the segment's activations exist and their tile is free
+  uint64_t* freed = bars + kStreamW * NST;                // [kStreamW][NST] a stage has been used
+  uint64_t* seg_open = freed + kStreamW * NST;             // [kMaxSegs] the segment's activations exist and their tile is free
   uint64_t* tile_full = seg_open + kMaxSegs;              // [kMaxSegs] they are in the tile (an arrival a row and block)
   uint64_t* tile_free = tile_full + kMaxSegs;             // [kMaxSegs] no stream warp reads them any more
   uint64_t* tabbar = tile_free + kMaxSegs;                // the table and all segments are known
   Seg* segs = reinterpret_cast<Seg*>(tabbar + 2);
-  int* claim = reinterpret_cast<int*>(segs + kMaxSegs);   // [kMaxSegs] rows and blocks that a warp has taken on
+  int* first_blk = reinterpret_cast<int*>(segs + kMaxSegs);  // [2][12] a task's first block, of K = H and of K = I
+  int* claim = first_blk + 24;                            // [kMaxSegs] rows and blocks that a warp has taken on
   int* cnt = claim + kMaxSegs;                            // [kP] tasks summed of a unit in flight
   int* done = cnt + kP;                                   // tasks whose unit has been joined
   int* s_nseg = done + 1;
@@ -268,10 +270,11 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
   BlockSync* sy = p.sync;
 
   if (warp < kStreamW && lane == 0)
-    for (int s = 0; s < NST; ++s) mbar_init(bars + warp * NST + s, 1);
+    for (int s = 0; s < NST; ++s) mbar_init(bars + warp * NST + s, 1), mbar_init(freed + warp * NST + s, 1);
   for (int i = threadIdx.x; i < kMaxSegs; i += kThreads) mbar_init(seg_open + i, 1), mbar_init(tile_free + i, kStreamW), claim[i] = 0;
   if (threadIdx.x < kP) cnt[threadIdx.x] = 0;
   if (threadIdx.x < 8) reinterpret_cast<uint32_t*>(zero)[threadIdx.x] = 0;
+  if (threadIdx.x <= 8) first_blk[threadIdx.x] = nbH * (int)threadIdx.x / QH, first_blk[12 + threadIdx.x] = nbI * (int)threadIdx.x / QI;
 
   const bool has_sh = p.sh_d != nullptr;
   const int Gs = G - p.M;  // the CTAs that do not route
@@ -288,61 +291,25 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
   mbar_fence_init();
   __syncthreads();
 
-  // ---- stream warps: the producer's state (lane 0): segment, task, block, quarter of a bf16 block
+  // ---- a stream warp's way through the tasks of a segment, without divisions (W tasks on: some units and a part of one)
+  const int duH = kStreamW / QH, dqH = kStreamW % QH, duI = kStreamW / QI, dqI = kStreamW % QI;
+  struct Cursor {
+    int i, u, q, slot;  // task, unit (of the slot, in an up run of the routed experts), task of the unit
+  };
+  auto enter = [&](Cursor& c, const Seg& s, int w) {
+    const int Q = s.down ? QI : QH;
+    c.i = (int)((unsigned)(w + kStreamW - s.base % kStreamW) % kStreamW);
+    c.u = s.u0 + c.i / Q, c.q = c.i % Q, c.slot = s.slot;
+    if (!s.down && s.slot != kShared) c.slot = c.u / upp, c.u -= c.slot * upp;
+  };
+  auto next = [&](Cursor& c, const Seg& s) {
+    c.i += kStreamW, c.u += s.down ? duI : duH, c.q += s.down ? dqI : dqH;
+    const int Q = s.down ? QI : QH;
+    if (c.q >= Q) c.q -= Q, ++c.u;
+    if (!s.down && s.slot != kShared)
+      while (c.u >= upp) c.u -= upp, ++c.slot;
+  };
   const int nb_first = a1 > a0 ? 1 : 0;  // segments whose units are known without the table
-  uint8_t* myring = ring + (size_t)warp * NST * kStage;
-  uint64_t* mybar = bars + warp * NST;
-  const uint64_t pol = policy_evict_first();
-  uint32_t issued = 0, consumed = 0;
-  int nknown = nb_first, ps = 0, pt = -1, pb = 0, pe = 0, pc = 0;
-  bool all_known = false;
-  const uint8_t *pa = nullptr, *pz = nullptr;
-  auto first_task = [&](const Seg& s) { return (int)((unsigned)(warp + kStreamW - s.base % kStreamW) % kStreamW); };
-  auto open_task = [&]() {
-    while (pb == pe) {
-      if (ps >= nknown) {
-        if (!all_known && mbar_test_wait(tabbar, 0)) all_known = true, nknown = *s_nseg;
-        if (ps >= nknown) return false;
-      }
-      const Seg& s = segs[ps];
-      if (pt < 0) pt = first_task(s);
-      if (pt >= s.tasks) {
-        ++ps, pt = -1;
-        continue;
-      }
-      const int Q = s.down ? QI : QH, nb = s.down ? nbI : nbH;
-      int u = s.u0 + pt / Q;
-      const int q = pt % Q;
-      pb = nb * q / Q, pe = nb * (q + 1) / Q, pc = 0, pt += kStreamW;
-      const size_t blk = s.b16 ? 4 * kHBlk : kQBlk;  // bytes of 8 rows x 512 k
-      if (s.down) {
-        const uint8_t* d = s.slot == kShared ? p.sh_d : tab.ent[s.slot].d;
-        pa = d + (size_t)(2 * u) * nb * blk, pz = pa + nb * blk;
-      } else if (s.slot == kShared) {
-        if (p.sh_bgu) pa = p.sh_bgu + (size_t)(2 * u) * nb * blk, pz = pa + nb * blk;
-        else pa = p.sh_g + (size_t)u * nb * blk, pz = p.sh_u + (size_t)u * nb * blk;
-      } else {
-        const BlockEnt& e = tab.ent[u / upp];
-        u %= upp;
-        pa = e.g + (size_t)u * nb * blk, pz = e.u + (size_t)u * nb * blk;
-      }
-      pa += pb * blk, pz += pb * blk;
-    }
-    return true;
-  };
-  auto issue = [&]() {
-    const int b16 = segs[ps].b16;
-    const uint32_t slot = issued % NST, bytes = b16 ? kHBlk : kQBlk;
-    uint8_t* st = myring + slot * kStage;
-    mbar_expect_tx(mybar + slot, 2 * bytes);
-    bulk_g2s_hint(st, pa, bytes, mybar + slot, pol);
-    bulk_g2s_hint(st + kQBlk, pz, bytes, mybar + slot, pol);
-    ++issued, pa += bytes, pz += bytes;
-    if (!b16 || ++pc == 4) ++pb, pc = 0;
-  };
-  auto fill = [&]() {
-    while (issued - consumed < (uint32_t)NST && open_task()) issue();
-  };
 
   if (router) {
     // ---- a row each; the last one to be routed builds the table -------------------------------------------------------------
@@ -420,18 +387,19 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
 
   if (warp < kStreamW) {
     // ---- stream warps --------------------------------------------------------------------------------------------------------
-    const uint32_t ring_at = smem_u32(myring);
+    const uint32_t ring_at = smem_u32(ring + (size_t)warp * NST * kStage);
+    uint64_t *mybar = bars + warp * NST, *myfreed = freed + warp * NST;
+    uint32_t consumed = 0;
     bool ok = true;
-    if (lane == 0) fill();
     auto stage_ready = [&]() {
       const uint32_t si = consumed % NST;
       if (!mbar_wait(mybar + si, (consumed / NST) & 1)) ok = false;
       return ring_at + si * kStage;
     };
     auto stage_used = [&]() {
-      ++consumed;
       __syncwarp();
-      if (lane == 0) fill();
+      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(myfreed + consumed % NST)) : "memory");
+      ++consumed;
     };
 
     for (int k = 0; ok; ++k) {
@@ -442,7 +410,6 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
       if (k >= nb_first) {  // (the units do, from here on)
         if (k == nb_first && !mbar_wait(tabbar, 0, 20)) ok = false;
         if (!ok || *s_fail || k >= *s_nseg) break;
-        if (lane == 0) fill();
       }
       const Seg s = segs[k];
       if ((k > nb_first && !prepare(k, s.b16, 1, s.slot, s.rows)) || !mbar_wait(tile_full + k, 0, 20)) {
@@ -452,13 +419,15 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
       const int Q = s.down ? QI : QH, nb = s.down ? nbI : nbH;
       const Tile tile(tile_at(k), nb, s.rows);
       const uint32_t span = s.rows * 128, x0 = smem_u32(tile.x), z0 = smem_u32(zero);
-      for (int i = first_task(s); i < s.tasks && ok; i += kStreamW) {
-        const int u = s.u0 + i / Q, q = i % Q, b0 = nb * q / Q, b1 = nb * (q + 1) / Q;
-        // the rows of this unit: the place in the tile of the j-th
-        unsigned long long rows = 0x0706050403020100ull;
-        int n = s.rows;
-        if (!s.down && s.slot != kShared) rows = tab.ent[u / upp].rows, n = tab.ent[u / upp].n;
-        auto row = [&](int j) { return (int)(rows >> (8 * min(j, n - 1)) & 0xff); };
+      Cursor c;
+      enter(c, s, warp);
+      int slot = -1, n = s.rows;
+      unsigned long long rows = 0x0706050403020100ull;  // the unit's rows: the place in the tile of the j-th
+      auto row = [&](int j) { return (int)(rows >> (8 * min(j, n - 1)) & 0xff); };
+      for (; c.i < s.tasks && ok; next(c, s)) {
+        if (!s.down && s.slot != kShared && c.slot != slot) slot = c.slot, rows = tab.ent[slot].rows, n = tab.ent[slot].n;
+        const int* fb = first_blk + (s.down ? 12 : 0) + c.q;
+        const int b0 = fb[0], b1 = fb[1];
         float acc[2][2] = {{0.f, 0.f}, {0.f, 0.f}};  // [rows t, t + 4][strip]
         if (s.b16) {
           const uint32_t xr = x0 + row((g >> 1) + 4 * (g & 1)) * 128 + t * 32;
@@ -504,19 +473,17 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
           else run(std::integral_constant<int, 1>());
         }
         if (!ok) break;
-        const int j = s.base + i;
+        const int j = s.base + c.i;
         if (!(ok = wait_shared_ge(done, j - kP + 1, 100))) break;
         float2* d = reinterpret_cast<float2*>(part + (j % kP) * kPart) + lane;
         d[0] = make_float2(acc[0][0], acc[0][1]), d[32] = make_float2(acc[1][0], acc[1][1]);
         __threadfence_block();
         __syncwarp();
-        if (lane == 0) atomicAdd(cnt + (j - q) % kP, 1);
+        if (lane == 0) atomicAdd(cnt + (j - c.q) % kP, 1);
       }
       if (ok && lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(tile_free + k)) : "memory");
     }
     if (!ok) *s_fail = 1;
-    if (lane == 0)  // (only after a wait that ran out: no copy is left in flight)
-      for (; consumed < issued; ++consumed) mbar_wait(mybar + consumed % NST, (consumed / NST) & 1);
   } else if (warp == kStreamW) {
     // ---- the joining warp: a unit's tasks in ascending k, then SwiGLU or the picks' outputs -----------------------------------
     bool ok = true;
@@ -587,7 +554,76 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
     } else {
       *s_fail = 1;
     }
-  } else if (warp > kStreamW + 1) {
+  } else if (warp == kStreamW + 2) {
+    // ---- the producer: lane w fills stream warp w's ring as its stages are freed (a warp that fills its own spends 650 to 1000 of
+    // 4400 cycles a stage on it, all of them in its way)
+    const int w = lane;
+    uint8_t* myring = ring + (size_t)w * NST * kStage;
+    uint64_t *mybar = bars + w * NST, *myfreed = freed + w * NST;
+    const uint64_t pol = policy_evict_first();
+    uint32_t issued = 0;
+    int nknown = nb_first, ps = 0, pslot = -1, pb = 0, pe = 0, pc = 0;
+    bool all_known = false, inside = false, more = w < kStreamW;
+    Cursor cur{0, 0, 0, 0};
+    Seg sg = segs[0];
+    const uint8_t *pa = nullptr, *pz = nullptr, *base_a = nullptr, *base_z = nullptr;
+    long long t0 = clock64();
+    while (__any_sync(0xffffffffu, more)) {
+      bool moved = false;
+      // the next task with a block to fetch, if its segment is known
+      if (more && pb == pe) {
+        if (inside) next(cur, sg);
+        if (inside && cur.i >= sg.tasks) ++ps, inside = false;
+        if (!inside) {
+          if (ps >= nknown && !all_known && mbar_test_wait(tabbar, 0)) all_known = true, nknown = *s_nseg;
+          if (ps < nknown) sg = segs[ps], inside = true, pslot = -1, enter(cur, sg, w), moved = true;
+          else if (all_known) more = false;
+        }
+        if (more && inside && cur.i < sg.tasks) {
+          const int nb = sg.down ? nbI : nbH;
+          const uint32_t blk = sg.b16 ? 4 * kHBlk : kQBlk;  // bytes of 8 rows x 512 k
+          if (cur.slot != pslot) {
+            pslot = cur.slot;
+            if (sg.down) {
+              base_a = pslot == kShared ? p.sh_d : tab.ent[pslot].d, base_z = base_a + (size_t)nb * blk;
+            } else if (pslot == kShared) {
+              base_a = p.sh_bgu ? p.sh_bgu : p.sh_g, base_z = p.sh_bgu ? base_a + (size_t)nb * blk : p.sh_u;
+            } else {
+              base_a = tab.ent[pslot].g, base_z = tab.ent[pslot].u;
+            }
+          }
+          const int* fb = first_blk + (sg.down ? 12 : 0) + cur.q;
+          pb = fb[0], pe = fb[1], pc = 0;
+          const bool both = sg.down || (pslot == kShared && p.sh_bgu);  // the unit's two strips follow each other in one matrix
+          const size_t off = (size_t)((both ? 2 * cur.u : cur.u) * nb + pb) * blk;
+          pa = base_a + off, pz = base_z + off, moved = true;
+        }
+      }
+      if (more && pb < pe) {
+        const uint32_t slot = issued % NST;
+        if (issued < (uint32_t)NST || mbar_test_wait(myfreed + slot, (issued / NST - 1) & 1)) {
+          const uint32_t bytes = sg.b16 ? kHBlk : kQBlk;
+          uint8_t* st = myring + slot * kStage;
+          mbar_expect_tx(mybar + slot, 2 * bytes);
+          bulk_g2s_hint(st, pa, bytes, mybar + slot, pol);
+          bulk_g2s_hint(st + kQBlk, pz, bytes, mybar + slot, pol);
+          ++issued, pa += bytes, pz += bytes, moved = true;
+          if (!sg.b16 || ++pc == 4) ++pb, pc = 0;
+        }
+      }
+      if (__any_sync(0xffffffffu, moved)) {
+        t0 = clock64();
+      } else {
+        if (*reinterpret_cast<volatile int*>(s_fail) || clock64() - t0 > kWaitCycles) break;
+        __nanosleep(20);
+      }
+    }
+    if (__any_sync(0xffffffffu, more)) {  // given up: no copy is left in flight
+      *s_fail = 1;
+      for (uint32_t n = issued > (uint32_t)NST ? issued - NST : 0; w < kStreamW && n < issued; ++n) mbar_wait(mybar + n % NST, (n / NST) & 1);
+    }
+    __syncwarp();
+  } else if (warp > kStreamW + 2) {
     // ---- helpers (the narrow variant's): their share of every segment's activations
     bool ok = true;
     for (int k = 0; ok; ++k) {
@@ -716,8 +752,8 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
 
 template <class V>
 size_t block_smem(size_t tile, int nbuf) {
-  return (size_t)V::W * V::NST * kStage + kP * kPart + sizeof(BlockTab) + nbuf * tile + 64 + (V::W * V::NST + 3 * kMaxSegs + 2) * 8 +
-         kMaxSegs * (sizeof(Seg) + 4) + (kP + 4) * 4 + 16;
+  return (size_t)V::W * V::NST * kStage + kP * kPart + sizeof(BlockTab) + nbuf * tile + 64 + (2 * V::W * V::NST + 3 * kMaxSegs + 2) * 8 +
+         kMaxSegs * (sizeof(Seg) + 4) + 24 * 4 + (kP + 4) * 4 + 16;
 }
 size_t block_tile(int H, int I, int M) {
   size_t t = tile_bytes(H, M) > tile_bytes(I, M) ? tile_bytes(H, M) : tile_bytes(I, M);
@@ -741,7 +777,7 @@ cudaError_t launch(const BlockParams& p, cudaStream_t st) {
   cfg.attrs = at, cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, k_block<V>, p);
 }
-using Wide = BlkVar<14, 2>;
+using Wide = BlkVar<13, 2>;
 using Narrow = BlkVar<11, 2>;  // (leaves more shared memory to the activations)
 
 size_t al256(size_t v) { return (v + 255) & ~(size_t)255; }
