@@ -390,6 +390,7 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
     const uint32_t ring_at = smem_u32(ring + (size_t)warp * NST * kStage);
     uint64_t *mybar = bars + warp * NST, *myfreed = freed + warp * NST;
     uint32_t consumed = 0;
+    int joined = 0;  // tasks joined when last looked at
     bool ok = true;
     auto stage_ready = [&]() {
       const uint32_t si = consumed % NST;
@@ -421,52 +422,62 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
       const uint32_t span = s.rows * 128, x0 = smem_u32(tile.x), z0 = smem_u32(zero);
       Cursor c;
       enter(c, s, warp);
+      // where this lane finds the slot's rows: set e's column in the tile (zeros: step 0), its row's sums and scales
       int slot = -1, n = s.rows;
-      unsigned long long rows = 0x0706050403020100ull;  // the unit's rows: the place in the tile of the j-th
-      auto row = [&](int j) { return (int)(rows >> (8 * min(j, n - 1)) & 0xff); };
+      uint32_t xr[2], step[2], sr[2], fr[2];
+      auto rows_of = [&](unsigned long long rows) {
+        auto row = [&](int j) { return (int)(rows >> (8 * min(j, n - 1)) & 0xff); };
+        if (s.b16) {
+          xr[0] = x0 + row((g >> 1) + 4 * (g & 1)) * 128 + t * 32;
+          return;
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int col = 4 * e + (g >> 1), me = row(4 * e + t);
+          const bool on = (t >> 1) == (g & 1) && col < n;
+          xr[e] = on ? x0 + row(col) * 128 + t * 32 : z0, step[e] = on ? span : 0u;
+          sr[e] = smem_u32(tile.sum) + me * 8, fr[e] = smem_u32(tile.scale) + me * 4;
+        }
+      };
+      rows_of(0x0706050403020100ull);
       for (; c.i < s.tasks && ok; next(c, s)) {
-        if (!s.down && s.slot != kShared && c.slot != slot) slot = c.slot, rows = tab.ent[slot].rows, n = tab.ent[slot].n;
+        if (!s.down && s.slot != kShared && c.slot != slot) slot = c.slot, n = tab.ent[slot].n, rows_of(tab.ent[slot].rows);
         const int* fb = first_blk + (s.down ? 12 : 0) + c.q;
         const int b0 = fb[0], b1 = fb[1];
         float acc[2][2] = {{0.f, 0.f}, {0.f, 0.f}};  // [rows t, t + 4][strip]
         if (s.b16) {
-          const uint32_t xr = x0 + row((g >> 1) + 4 * (g & 1)) * 128 + t * 32;
           for (int b = b0; b < b1 && ok; ++b) {
             float d[4] = {0.f, 0.f, 0.f, 0.f};
-            for (int c = 0; c < 4; ++c) {
+            for (int q = 0; q < 4; ++q) {
               const uint32_t st = stage_ready();
               if (!ok) break;
-              pair_b16(d, st, xr + (8 * b + 2 * c) * span, span, lane);
+              pair_b16(d, st, xr[0] + (8 * b + 2 * q) * span, span, lane);
               stage_used();
             }
             acc[0][0] = __fadd_rn(acc[0][0], d[0]), acc[1][0] = __fadd_rn(acc[1][0], d[1]);
             acc[0][1] = __fadd_rn(acc[0][1], d[2]), acc[1][1] = __fadd_rn(acc[1][1], d[3]);
           }
         } else {
-          const bool mine = (t >> 1) == (g & 1);
           auto run = [&](auto sets) {
             constexpr int S = decltype(sets)::value;
-            uint32_t xr[S], step[S], sr[S], fr[S];
-#pragma unroll
-            for (int e = 0; e < S; ++e) {
-              const int col = 4 * e + (g >> 1), me = row(4 * e + t);
-              const bool on = mine && col < n;
-              xr[e] = on ? x0 + b0 * 8 * span + row(col) * 128 + t * 32 : z0, step[e] = on ? span : 0u;
-              sr[e] = smem_u32(tile.sum) + (b0 * 8 * s.rows + me) * 8, fr[e] = smem_u32(tile.scale) + (b0 * s.rows + me) * 4;
-            }
             for (int b = b0; b < b1; ++b) {
+              uint32_t xb[S], st_[S], sb[S];
+              float f[S];
+#pragma unroll
+              for (int e = 0; e < S; ++e) {
+                xb[e] = xr[e] + b * 8 * step[e], st_[e] = step[e], sb[e] = sr[e] + b * (s.rows * 64);
+                f[e] = lds_f(fr[e] + b * (s.rows * 4));
+              }
               const uint32_t st = stage_ready();
               if (!ok) break;
               float2 blk[S][2];
-              pair_int4<S>(blk, st, xr, step, sr, s.rows * 8, lane);
+              pair_int4<S>(blk, st, xb, st_, sb, s.rows * 8, lane);
+              stage_used();
 #pragma unroll
               for (int e = 0; e < S; ++e) {  // times 2^(24 - E), in two steps that cannot leave f32's range by themselves
-                const float f = lds_f(fr[e]);
-                acc[e][0] = fmaf(__fadd_rn(blk[e][0].x, blk[e][0].y) * 4096.f, f, acc[e][0]);
-                acc[e][1] = fmaf(__fadd_rn(blk[e][1].x, blk[e][1].y) * 4096.f, f, acc[e][1]);
-                xr[e] += 8 * step[e], sr[e] += s.rows * 64, fr[e] += s.rows * 4;
+                acc[e][0] = fmaf(__fadd_rn(blk[e][0].x, blk[e][0].y) * 4096.f, f[e], acc[e][0]);
+                acc[e][1] = fmaf(__fadd_rn(blk[e][1].x, blk[e][1].y) * 4096.f, f[e], acc[e][1]);
               }
-              stage_used();
             }
           };
           if (n > 4) run(std::integral_constant<int, 2>());
@@ -474,12 +485,14 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
         }
         if (!ok) break;
         const int j = s.base + c.i;
-        if (!(ok = wait_shared_ge(done, j - kP + 1, 100))) break;
+        if (j >= joined + kP) {  // (the place of the sums is free once the unit that had it has been joined)
+          if (!(ok = wait_shared_ge(done, j - kP + 1, 100))) break;
+          joined = ld_shared_acquire(done);
+        }
         float2* d = reinterpret_cast<float2*>(part + (j % kP) * kPart) + lane;
         d[0] = make_float2(acc[0][0], acc[0][1]), d[32] = make_float2(acc[1][0], acc[1][1]);
-        __threadfence_block();
         __syncwarp();
-        if (lane == 0) atomicAdd(cnt + (j - c.q) % kP, 1);
+        if (lane == 0) red_shared_release(cnt + (j - c.q) % kP, 1);
       }
       if (ok && lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(tile_free + k)) : "memory");
     }
