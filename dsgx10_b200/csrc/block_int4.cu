@@ -567,10 +567,10 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
     } else {
       *s_fail = 1;
     }
-  } else if (warp == kStreamW + 2) {
+  } else if (warp == kStreamW + 2 || warp == kStreamW + 3) {
     // ---- the producer: lane w fills stream warp w's ring as its stages are freed (a warp that fills its own spends 650 to 1000 of
     // 4400 cycles a stage on it, all of them in its way)
-    const int w = lane;
+    const int w = 2 * lane + (warp - kStreamW - 2);
     uint8_t* myring = ring + (size_t)w * NST * kStage;
     uint64_t *mybar = bars + w * NST, *myfreed = freed + w * NST;
     const uint64_t pol = policy_evict_first();
@@ -636,7 +636,7 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
       for (uint32_t n = issued > (uint32_t)NST ? issued - NST : 0; w < kStreamW && n < issued; ++n) mbar_wait(mybar + n % NST, (n / NST) & 1);
     }
     __syncwarp();
-  } else if (warp > kStreamW + 2) {
+  } else if (warp > kStreamW + 3) {
     // ---- helpers (the narrow variant's): their share of every segment's activations
     bool ok = true;
     for (int k = 0; ok; ++k) {
@@ -790,7 +790,7 @@ cudaError_t launch(const BlockParams& p, cudaStream_t st) {
   cfg.attrs = at, cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, k_block<V>, p);
 }
-using Wide = BlkVar<13, 2>;
+using Wide = BlkVar<12, 2>;
 using Narrow = BlkVar<11, 2>;  // (leaves more shared memory to the activations)
 
 size_t al256(size_t v) { return (v + 255) & ~(size_t)255; }
