@@ -234,11 +234,12 @@ DSGX_DEV void build_block_tab(BlockTab* out, int* s_idx, int* s_first, const Blo
   }
 }
 
-// W stream warps with NST ring stages each, the joining warp, the control warp, the producer, and the rest of sixteen help with
+// W stream warps with NST ring stages each, the joining warp, the control warp, NP producers, and the rest of sixteen help with
 // activations (sixteen: the routing wants a thread an expert)
-template <int W_, int NST_>
+template <int W_, int NST_, int NP_>
 struct BlkVar {
-  static constexpr int W = W_, NST = NST_, kThreads = 512;
+  static constexpr int W = W_, NST = NST_, NP = NP_, kThreads = 512;
+  static_assert(W + 2 + NP <= 16, "warps");
 };
 
 template <class V>
@@ -346,11 +347,13 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
     int i = warp * Gs + cta;
     for (; i < ntask; i += kLogitW * Gs) logit_slice_task(p.x, p.wr, p.M, p.H, p.E, i / KS, i % KS, p.lpart, lane);
     __threadfence();
-    asm volatile("bar.sync 1, %0;" ::"n"(kLogitW * 32) : "memory");
+    asm volatile("bar.sync 1, %0;" ::"n"((kLogitW + V::NP) * 32) : "memory");
     if (threadIdx.x == 0) {
       __threadfence();
       atomicAdd(&sy->cnt_lp, 1);
     }
+  } else if (warp > kStreamW + 1 && warp < kStreamW + 2 + V::NP) {
+    asm volatile("bar.sync 1, %0;" ::"n"((kLogitW + V::NP) * 32) : "memory");  // (the producers begin when the logits are done)
   }
 
   // ---- a segment's activation tile: the shared expert's x, the routed experts' x, then the down segments in the first tile's place
@@ -567,10 +570,10 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
     } else {
       *s_fail = 1;
     }
-  } else if (warp == kStreamW + 2 || warp == kStreamW + 3) {
+  } else if (warp < kStreamW + 2 + V::NP && warp > kStreamW + 1) {
     // ---- the producer: lane w fills stream warp w's ring as its stages are freed (a warp that fills its own spends 650 to 1000 of
     // 4400 cycles a stage on it, all of them in its way)
-    const int w = 2 * lane + (warp - kStreamW - 2);
+    const int w = V::NP * lane + (warp - kStreamW - 2);
     uint8_t* myring = ring + (size_t)w * NST * kStage;
     uint64_t *mybar = bars + w * NST, *myfreed = freed + w * NST;
     const uint64_t pol = policy_evict_first();
@@ -636,7 +639,7 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
       for (uint32_t n = issued > (uint32_t)NST ? issued - NST : 0; w < kStreamW && n < issued; ++n) mbar_wait(mybar + n % NST, (n / NST) & 1);
     }
     __syncwarp();
-  } else if (warp > kStreamW + 3) {
+  } else if (warp > kStreamW + 1) {
     // ---- helpers (the narrow variant's): their share of every segment's activations
     bool ok = true;
     for (int k = 0; ok; ++k) {
@@ -790,8 +793,8 @@ cudaError_t launch(const BlockParams& p, cudaStream_t st) {
   cfg.attrs = at, cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, k_block<V>, p);
 }
-using Wide = BlkVar<12, 2>;
-using Narrow = BlkVar<11, 2>;  // (leaves more shared memory to the activations)
+using Wide = BlkVar<12, 2, 2>;
+using Narrow = BlkVar<11, 2, 3>;  // (leaves more shared memory to the activations)
 
 size_t al256(size_t v) { return (v + 255) & ~(size_t)255; }
 
