@@ -81,6 +81,9 @@ DSGX_DEV bool poll_near(const int* p, int target) {
   return true;
 }
 
+// g / (1 + e^-g) by the fast exponential and division: within 100 x 2^-23 of the value for |g| up to 80, and h is rounded to bf16 next
+DSGX_DEV float quick_silu(float g) { return __fdividef(g, 1.f + __expf(-g)); }
+
 // A CTA's run of units of one phase.
 struct Seg {
   int down, b16, slot, rows;  // slot: of a down run (an up run covers several); rows: of the activation tile
@@ -173,6 +176,35 @@ DSGX_DEV int routed_begin(int i, int N, int c, int n, int cs, int Gs, int G, int
   return (int)min((long long)N, max(0ll, (total * i / G - used) / c));
 }
 
+// One (expert, 1024 k) slice of the router logits for rows [m0, m1): decode_common.cuh's logit_slice_task, sum for sum, with two
+// rows' loads in flight (row after row, eight rows took 7 us).
+DSGX_DEV void logit_rows(const __nv_bfloat16* __restrict__ x, const float* __restrict__ wr, int m0, int m1, int H, int E, int e, int sl,
+                         float* __restrict__ lpart, int lane) {
+  float4 wv[8];
+  logit_slice_weights(wr, H, e, sl, lane, wv);
+  const int base = sl * 1024, nit = min(1024, H - base) / 128;
+  for (int m = m0; m < m1; m += 2) {
+    uint2 xv[2][8];
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        xv[c][i] = i < nit && m + c < m1 ? __ldg(reinterpret_cast<const uint2*>(x + (size_t)(m + c) * H + base + 128 * i + 4 * lane)) : make_uint2(0, 0);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float a = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < nit) {
+          a = fmaf(bf16_bits_to_f(xv[c][i].x & 0xffffu), wv[i].x, a), a = fmaf(bf16_bits_to_f(xv[c][i].x >> 16), wv[i].y, a);
+          a = fmaf(bf16_bits_to_f(xv[c][i].y & 0xffffu), wv[i].z, a), a = fmaf(bf16_bits_to_f(xv[c][i].y >> 16), wv[i].w, a);
+        }
+      a = warp_sum(a);
+      if (lane == 0 && m + c < m1) lpart[((size_t)sl * kMaxRows + m + c) * E + e] = a;
+    }
+  }
+}
+
 // ---- the table, by the first 64 threads of a CTA, a thread a pick, written straight to global memory.  s_idx, s_first: kMaxEnt
 // words of shared memory each.
 DSGX_DEV void build_block_tab(BlockTab* out, int* s_idx, int* s_first, const BlockParams& p) {
@@ -191,20 +223,26 @@ DSGX_DEV void build_block_tab(BlockTab* out, int* s_idx, int* s_first, const Blo
   asm volatile("bar.sync 3, 64;" ::: "memory");
   bool first = e != kNone;
   uint32_t mask = 0;  // the rows that picked the expert
-  const int row = i / p.topk;
-  int place = 0, r = 0, c = 0;  // the pick's place in its row's ascending order
-  for (int j = 0; j < np; ++j) {
-    const int o = s_idx[j];
-    if (o == e) mask |= 1u << r, first = first && j >= i;
-    if (r == row) place += o < e;
-    if (++c == p.topk) c = 0, ++r;
+  const int row = i / p.topk, recip = 65536 / p.topk + 1;  // (j recip >> 16 = j / topk for j < 64)
+  int place = 0;  // the pick's place in its row's ascending order
+#pragma unroll 4
+  for (int j4 = 0; j4 < (np + 3) / 4; ++j4) {
+    const int4 o4 = reinterpret_cast<const int4*>(s_idx)[j4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int j = 4 * j4 + c, o = c == 0 ? o4.x : c == 1 ? o4.y : c == 2 ? o4.z : o4.w, r = j * recip >> 16;
+      if (o == e) mask |= 1u << r, first = first && j >= i;
+      place += r == row && o < e;
+    }
   }
   s_first[i] = first ? e : kNone;
   asm volatile("bar.sync 3, 64;" ::: "memory");
   int slot = 0, n = 0;
-  for (int j = 0; j < np; ++j) {
-    const int o = s_first[j];
-    slot += o < e, n += o != kNone;
+#pragma unroll 4
+  for (int j4 = 0; j4 < (np + 3) / 4; ++j4) {
+    const int4 o4 = reinterpret_cast<const int4*>(s_first)[j4];
+    slot += (o4.x < e) + (o4.y < e) + (o4.z < e) + (o4.w < e);
+    n += (o4.x != kNone) + (o4.y != kNone) + (o4.z != kNone) + (o4.w != kNone);
   }
   int bad = bad_id ? DSGX_ERR_ARG : 0;
   if (first) {
@@ -344,8 +382,12 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
     // ---- the router's logit slices, one warp a (expert, 1024 k); a CTA reports when all of its are in memory.  (The rings
     // filled first: 2.4 us later logits and not a microsecond gained on the shared expert.) ------------------------------------
     const int KS = (p.H + 1023) / 1024, ntask = p.E * KS;
-    int i = warp * Gs + cta;
-    for (; i < ntask; i += kLogitW * Gs) logit_slice_task(p.x, p.wr, p.M, p.H, p.E, i / KS, i % KS, p.lpart, lane);
+    // (more warps than slices: a slice's rows over several warps)
+    const int parts = min(p.M, max(1, kLogitW * Gs / ntask)), per = (p.M + parts - 1) / parts;
+    for (int i = warp * Gs + cta; i < ntask * parts; i += kLogitW * Gs) {
+      const int slice = i / parts, m = (i - slice * parts) * per;
+      logit_rows(p.x, p.wr, m, min(p.M, m + per), p.H, p.E, slice / KS, slice % KS, p.lpart, lane);
+    }
     __threadfence();
     asm volatile("bar.sync 1, %0;" ::"n"((kLogitW + V::NP) * 32) : "memory");
     if (threadIdx.x == 0) {
@@ -510,11 +552,15 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
       }
       const Seg s = segs[k];
       const int Q = s.down ? QI : QH;
-      int reported = 0;
-      for (int i = 0; i < s.n && ok; ++i) {
-        const int j = s.base + i * Q;
+      const bool inter = s.slot == kShared && p.sh_bgu;
+      // the unit's slot, and its number among the slot's units
+      int slot = s.slot, u = s.u0, reported = 0;
+      if (!s.down && s.slot != kShared) slot = u / upp, u -= slot * upp;
+      int n = slot == kShared ? p.M : tab.ent[slot].n;
+      for (int i = 0, j = s.base; i < s.n && ok; ++i, j += Q, ++u) {
+        if (!s.down && s.slot != kShared && u == upp) u = 0, n = tab.ent[++slot].n;
         int* c = cnt + j % kP;
-        if (!(ok = wait_shared_ge(c, Q, 40))) break;
+        if (!(ok = wait_shared_ge(c, Q, 0))) break;
         float2 v[2];
         for (int q = 0; q < Q; ++q) {
           const float2* d = reinterpret_cast<const float2*>(part + ((j + q) % kP) * kPart) + lane;
@@ -527,35 +573,31 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
           *c = 0;
           st_shared_release(done, j + Q);
         }
-        const int u = s.u0 + i;
         if (s.down) {
-          const int n = s.slot == kShared ? p.M : tab.ent[s.slot].n;
-          float* y = p.y + ((size_t)s.slot * kMaxRows + t) * p.H + 16 * u + g;
+          float* y = p.y + ((size_t)slot * kMaxRows + t) * p.H + 16 * u + g;
 #pragma unroll
           for (int e = 0; e < 2; ++e)
             if (4 * e + t < n) y[(size_t)4 * e * p.H] = v[e].x, y[(size_t)4 * e * p.H + 8] = v[e].y;
           continue;
         }
-        const int slot = s.slot == kShared ? kShared : u / upp, ch = (s.slot == kShared ? u : u % upp) * 8;
-        const int n = slot == kShared ? p.M : tab.ent[slot].n;
-        __nv_bfloat16* h = p.h + ((size_t)slot * kMaxRows + t) * p.I + ch;
-        if (slot == kShared && p.sh_bgu) {
+        __nv_bfloat16* h = p.h + ((size_t)slot * kMaxRows + t) * p.I + 8 * u;
+        if (inter) {
           // interleaved rows: strip rows 2 i and 2 i + 1 are gate and up of a channel (first strip: channels 0-3, second: 4-7)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const float ua = __shfl_down_sync(0xffffffffu, v[e].x, 4), ub = __shfl_down_sync(0xffffffffu, v[e].y, 4);
             if (!(g & 1) && 4 * e + t < n) {
-              h[(size_t)4 * e * p.I + (g >> 1)] = __float2bfloat16_rn(__fmul_rn(silu(v[e].x), ua));
-              h[(size_t)4 * e * p.I + 4 + (g >> 1)] = __float2bfloat16_rn(__fmul_rn(silu(v[e].y), ub));
+              h[(size_t)4 * e * p.I + (g >> 1)] = __float2bfloat16_rn(__fmul_rn(quick_silu(v[e].x), ua));
+              h[(size_t)4 * e * p.I + 4 + (g >> 1)] = __float2bfloat16_rn(__fmul_rn(quick_silu(v[e].y), ub));
             }
           }
         } else {
 #pragma unroll
           for (int e = 0; e < 2; ++e)
-            if (4 * e + t < n) h[(size_t)4 * e * p.I + g] = __float2bfloat16_rn(__fmul_rn(silu(v[e].x), v[e].y));
+            if (4 * e + t < n) h[(size_t)4 * e * p.I + g] = __float2bfloat16_rn(__fmul_rn(quick_silu(v[e].x), v[e].y));
         }
         // the run's units of a slot are reported together: h is read when all of the slot's are there
-        if (i + 1 == s.n || (s.slot != kShared && (u + 1) / upp != slot)) {
+        if (i + 1 == s.n || (s.slot != kShared && u + 1 == upp)) {
           __threadfence();
           __syncwarp();
           if (lane == 0) atomicAdd(&sy->cnt_h[slot], i + 1 - reported);

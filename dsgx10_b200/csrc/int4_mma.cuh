@@ -57,7 +57,7 @@ DSGX_DEV bool wait_shared_ge(const int* p, int v, unsigned sleep_ns) {
   if (ld_shared_acquire(p) >= v) return true;
   const long long t0 = clock64();
   while (ld_shared_acquire(p) < v) {
-    __nanosleep(sleep_ns);
+    if (sleep_ns) __nanosleep(sleep_ns);
     if (clock64() - t0 > kWaitCycles) return false;
   }
   return true;

@@ -45,7 +45,7 @@ def _ffn(x, mats):
     dg, du = _gamma(x.shape[1]) * (ax @ bg.T), _gamma(x.shape[1]) * (ax @ bu.T)
     act = g * torch.sigmoid(g)
     h = act * u
-    dh = 1.1 * dg * (u.abs() + du) + act.abs() * du + h.abs() * (2.0 ** -8 + 8 * 2.0 ** -24)
+    dh = 1.1 * dg * (u.abs() + du) + act.abs() * du + h.abs() * (2.0 ** -8 + 2.0 ** -16)
     return h @ wd.T, dh @ wd.abs().T + _gamma(h.shape[1]) * ((h.abs() + dh) @ bd.T)
 
 
