@@ -70,6 +70,14 @@ constexpr int kShared = kMaxEnt;         // the shared expert's place among the 
 constexpr int kMaxSegs = kMaxEnt + 4;
 constexpr size_t kSmemMax = 227 * 1024;
 
+// Signals to other CTAs: releases of what this thread has written or has seen written behind a barrier of its CTA or warp.
+DSGX_DEV void red_release(int* p, int v) { asm volatile("red.release.gpu.global.add.s32 [%0], %1;" ::"l"(p), "r"(v) : "memory"); }
+DSGX_DEV void st_release(int* p, int v) { asm volatile("st.release.gpu.global.s32 [%0], %1;" ::"l"(p), "r"(v) : "memory"); }
+DSGX_DEV int atom_add_acq_rel(int* p, int v) {
+  int o;
+  asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], %2;" : "=r"(o) : "l"(p), "r"(v) : "memory");
+  return o;
+}
 // bounded poll until *p >= target (decode_common.cuh's poll_ge with a shorter sleep: these waits are on the critical path)
 DSGX_DEV bool poll_near(const int* p, int target) {
   if (ld_acquire(p) >= target) return true;
@@ -206,13 +214,13 @@ DSGX_DEV void logit_rows(const __nv_bfloat16* __restrict__ x, const float* __res
 }
 
 // ---- the table, by the first 64 threads of a CTA, a thread a pick, written straight to global memory.  s_idx, s_first: kMaxEnt
-// words of shared memory each.
-DSGX_DEV void build_block_tab(BlockTab* out, int* s_idx, int* s_first, const BlockParams& p) {
+// words of shared memory each.  idx, ws: the picks in shared memory (one row), or null: p.idx, p.w.
+DSGX_DEV void build_block_tab(BlockTab* out, int* s_idx, int* s_first, const int* idx, const float* ws, const BlockParams& p) {
   constexpr int kNone = 0x7fffffff;
   const int i = threadIdx.x, np = p.M * p.topk;
   const bool in = i < np;
-  int e = in ? __ldcg(p.idx + i) : kNone;
-  const float w = in ? __ldcg(p.w + i) : 0.f;
+  int e = in ? (idx ? idx[i] : __ldcg(p.idx + i)) : kNone;
+  const float w = in ? (ws ? ws[i] : __ldcg(p.w + i)) : 0.f;
   const bool bad_id = in && (e < 0 || e >= p.E);
   if (bad_id) e = kNone;
   uint4 d[3];  // off, s2, fmt of the expert's three descriptors
@@ -261,14 +269,12 @@ DSGX_DEV void build_block_tab(BlockTab* out, int* s_idx, int* s_first, const Blo
     out->w[row][place] = w;
   }
   s_idx[i] = bad;  // (read as picks only before the barrier above)
-  __threadfence();
   asm volatile("bar.sync 3, 64;" ::: "memory");
   if (i == 0) {
     for (int j = 0; j < np; ++j) bad = bad ? bad : s_idx[j];
     if (bad) atomicCAS(p.status, 0, bad);
     out->nslots = bad ? 0 : n, out->npick = bad ? 0 : p.topk;
-    __threadfence();
-    atomicExch(&p.sync->tab_ready, 1);
+    st_release(&p.sync->tab_ready, 1);
   }
 }
 
@@ -354,6 +360,8 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
     // ---- a row each; the last one to be routed builds the table -------------------------------------------------------------
     RouteSmem& rs = *reinterpret_cast<RouteSmem*>(tiles);
     int* s_idx = reinterpret_cast<int*>(part);
+    int* s_pick = s_idx + 2 * kMaxEnt;
+    float* s_w = reinterpret_cast<float*>(s_pick + kMaxTopK);
     const int row = cta - Gs, KS = (p.H + 1023) / 1024, nt = (p.E + 31) & ~31;
     for (int i = threadIdx.x; i < p.E * 3; i += kThreads) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.desc + i));
     if (threadIdx.x == 0) *s_tick = poll_near(&sy->cnt_lp, Gs) ? 1 : 0;
@@ -363,17 +371,14 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
     if (ok) {
       if ((int)threadIdx.x < nt)
         route_row_cta(p.rp, p.lpart + (size_t)row * p.E, KS, (size_t)kMaxRows * p.E, p.bias, rs, nullptr, p.idx + row * p.topk,
-                      p.w + row * p.topk, nullptr, nullptr, CtaPart{nt, 2});
+                      p.w + row * p.topk, p.M == 1 ? s_pick : nullptr, s_w, CtaPart{nt, 2});
       if (warp == 0) {  // (warp 0 wrote the picks)
-        __threadfence();
         __syncwarp();
-        if (lane == 0) *s_tick = p.M > 1 ? atomicAdd(&sy->cnt_rt, 1) : 0;
+        if (lane == 0) *s_tick = p.M > 1 ? atom_add_acq_rel(&sy->cnt_rt, 1) : 0;
       }
       __syncthreads();
-      if (*s_tick == p.M - 1 && threadIdx.x < 64) {
-        __threadfence();
-        build_block_tab(p.tab, s_idx, s_idx + kMaxEnt, p);
-      }
+      if (*s_tick == p.M - 1 && threadIdx.x < 64)
+        build_block_tab(p.tab, s_idx, s_idx + kMaxEnt, p.M == 1 ? s_pick : nullptr, p.M == 1 ? s_w : nullptr, p);
     } else if (threadIdx.x == 0) {
       *s_fail = 1;
     }
@@ -388,12 +393,8 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
       const int slice = i / parts, m = (i - slice * parts) * per;
       logit_rows(p.x, p.wr, m, min(p.M, m + per), p.H, p.E, slice / KS, slice % KS, p.lpart, lane);
     }
-    __threadfence();
     asm volatile("bar.sync 1, %0;" ::"n"((kLogitW + V::NP) * 32) : "memory");
-    if (threadIdx.x == 0) {
-      __threadfence();
-      atomicAdd(&sy->cnt_lp, 1);
-    }
+    if (threadIdx.x == 0) red_release(&sy->cnt_lp, 1);
   } else if (warp > kStreamW + 1 && warp < kStreamW + 2 + V::NP) {
     asm volatile("bar.sync 1, %0;" ::"n"((kLogitW + V::NP) * 32) : "memory");  // (the producers begin when the logits are done)
   }
@@ -598,17 +599,15 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
         }
         // the run's units of a slot are reported together: h is read when all of the slot's are there
         if (i + 1 == s.n || (s.slot != kShared && u + 1 == upp)) {
-          __threadfence();
           __syncwarp();
-          if (lane == 0) atomicAdd(&sy->cnt_h[slot], i + 1 - reported);
+          if (lane == 0) red_release(&sy->cnt_h[slot], i + 1 - reported);
           reported = i + 1;
         }
       }
     }
     if (ok && !*s_fail) {
-      __threadfence();
       __syncwarp();
-      if (lane == 0) atomicAdd(&sy->cnt_done, 1);
+      if (lane == 0) red_release(&sy->cnt_done, 1);
     } else {
       *s_fail = 1;
     }
