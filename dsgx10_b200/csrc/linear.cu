@@ -1,20 +1,32 @@
 // Dense INT4-g32 matrix-vector products for 1..16 rows: out[m][n] = sum_k x[m][k] W[n][k], W = (u - z) s, f32 sums; the
 // residual added, or with a second matrix silu(x W^T) * (x W_up^T).
 //
-// Bound: the weights are read once (0.578 bytes a weight), so HBM; the conversion of the nibbles in registers is the next
-// limit (int4_mma.cuh).  Work is cut in units of 16 output rows (SwiGLU: 8 gate + 8 up), a unit along K in 1, 2, 4 or 8 tasks, a task in
-// blocks of 16 rows x 512 k.  A CTA owns a run of units and its stream warps take the run's tasks in turn, each through a
-// private ring of bulk copies (one a block), so that every SM streams one contiguous run and the launch ends within a
-// task on every SM.  A task's sums go to shared memory; one more warp joins the tasks of a unit and writes the outputs,
-// so that the stream never waits for a reduction.
+// Bound: the weights are read once (0.578 bytes a weight), so HBM: 131072 x 4096 takes 58 us for one row and 59 for four, 83 %
+// and 81 % of a copy's rate; the copies alone, with nothing computed, take 50.  What is lost beside the launch and the first
+// blocks' latency (3.6 us together, all of a small matrix's time) is the conversion and the products (int4_mma.cuh): with
+// eight rows (69 us) the schedulers issue every other cycle, none of the pipes is above half, and a warp waits for its own
+// chain of loads, MMAs and f32 operations; fewer stream warps lose more (thirteen 70 us), more have no registers.
+//
+// Work is cut in units of 16 output rows (SwiGLU: 8 gate + 8 up), a unit along K in 1, 2, 4 or 8 tasks, a task in blocks of 16
+// rows x 512 k.  A CTA owns a run of units and its stream warps take the run's tasks in turn, each through a private ring of bulk
+// copies (one a block), so that every SM streams one contiguous run and the launch ends within a task on every SM.  One warp
+// fills all the rings (a copy takes its issuer 130 to 250 cycles; each warp for itself: 12288 x 6144 pair, one row 20.7 us
+// instead of 19.5); a task's sums go to shared memory, and one more warp joins the tasks of a unit and writes the outputs, so
+// that the stream never waits for a reduction.
+//
+// Rows 9..16: the clusters of a pair take eight rows and the rest over the same units, the second reads them from L2.  (One
+// cluster for all sixteen, two columns of MMAs a weight, took 45 us instead of 38 for 32768 x 4096: its activations leave room
+// for eleven warps only, and its loads of them double.)
 //
 // Weight layout (k_linear_prepare makes it from the experts' 8-row blocks): the blocks of a unit one after the other, 4736
-// bytes each, [8 spans of 64 k][32 lanes][four words: row g of the first strip and of the second in the span's first group of
-// 32, then both in its second], a word = the 8 nibbles k = 32 group + 8 t + 0..7 of lane 4 g + t (nibbles i and i + 4 meet in one f16 pair); [4 x 128 k][8 g][eight bf16
-// scales: (strip, group) by (first span, second span)]; [8 g][4 x 128 k][the eight zero points' nibbles in that order].
+// bytes each.  [8 spans of 64 k][32 lanes][four words]: row g of the first strip and of the second in the span's first group of
+// 32, then both in its second; a word = the 8 nibbles k = 32 group + 8 t + 0..7 of lane 4 g + t (nibbles i and i + 4 meet in one
+// f16 pair).  [4 x 128 k][8 g][eight bf16 scales: (strip, group) by (first span, second span)].  [8 g][4 x 128 k][the eight zero
+// points' nibbles in that order].
 // In the experts' blocks a lane's 16 bytes mix two groups in every MMA, so their scales have to go onto the weights (and
 // round them) or the MMAs' columns be halved (block_int4.cu: twice the MMAs and activation loads from five rows on; 131072 x
-// 4096 and eight rows took 87 us that way, 71 this way); here an MMA stays inside one group, its f32 sums take the scale, and all eight columns are rows of x.
+// 4096 and eight rows took 87 us that way).  Here an MMA stays inside one group, its f32 sums take the scale, and all eight
+// columns are rows of x.
 //
 // K over a cluster: with C > 1 (2, 4 or 8 CTAs) the ranks of a cluster take consecutive parts of K of the same units.  The
 // activations of M rows are held in shared memory for a rank's own part only, and a matrix with few units still occupies
@@ -41,16 +53,17 @@ constexpr size_t kSmemMax = 227 * 1024;
 
 constexpr int kUnitBlk = 4736;   // 16 rows x 512 k
 
-// W stream warps with NST ring stages each, P tasks' sums in flight (a power of two); kCol: four rows at most (unit_block4)
-template <bool kCol_, int W_, int NST_, int P_>
+// W stream warps with NST ring stages each, NP warps that fill the rings, P tasks' sums in flight (a power of two); kCol: four
+// rows at most (unit_block4)
+template <bool kCol_, int W_, int NP_, int NST_, int P_>
 struct LinVar {
-  static constexpr int W = W_, NST = NST_, P = P_;
+  static constexpr int W = W_, NP = NP_, NST = NST_, P = P_;
   static constexpr bool kCol = kCol_;
-  static constexpr int kThreads = (W + 1) * 32;
+  static constexpr int kThreads = (W + 1 + NP) * 32;
   static constexpr int kPart = 512;  // bytes of a task's (or a rank's) sums: [32 lanes][4] f32
   static size_t smem(int M, int kblocks, int C) {
     return (size_t)W * NST * kUnitBlk + (size_t)P * kPart + (C > 1 ? (size_t)kSlotsOwned * C * kPart : 0) +
-           (size_t)kblocks * (M * 1024 + even(M) * 68) + (kCol ? 256 : 0) + (W * NST + kSlotsOwned * (1 + kMaxCluster)) * 8 + P * 4 + 16 + 128;
+           (size_t)kblocks * (M * 1024 + even(M) * 68) + (kCol ? 256 : 0) + (2 * W * NST + kSlotsOwned * (1 + kMaxCluster)) * 8 + P * 4 + 16 + 128;
   }
   __host__ __device__ static int even(int M) { return (M + 1) & ~1; }
 };
@@ -198,7 +211,7 @@ DSGX_DEV float4 add4(float4 a, float4 b) {
 }
 template <class V>
 __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearParams p) {
-  constexpr int W = V::W, NST = V::NST, P = V::P, kPart = V::kPart;
+  constexpr int W = V::W, NP = V::NP, NST = V::NST, P = V::P, kPart = V::kPart;
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int C = p.cluster;
@@ -219,14 +232,15 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
   float* xscale = xsum + (size_t)p.xblocks * Me * 16;                           // [blocks][rows]: 2^(12 - E)
   uint8_t* zero = smem + (((xscale + (size_t)p.xblocks * Me) - reinterpret_cast<float*>(smem)) * 4 + 127) / 128 * 128;  // kCol: 128 zeros
   uint64_t* bars = reinterpret_cast<uint64_t*>(V::kCol ? zero + 128 : reinterpret_cast<uint8_t*>(xscale + (size_t)p.xblocks * Me));
-  uint64_t* rfull = bars + W * NST;                                    // [kSlotsOwned] every rank's sums are in my buffer
+  uint64_t* freed = bars + W * NST;                                    // a stage has been read
+  uint64_t* rfull = freed + W * NST;                                    // [kSlotsOwned] every rank's sums are in my buffer
   uint64_t* rfree = rfull + kSlotsOwned;                               // [owner][kSlotsOwned] that owner's buffer may be written
   int* cnt = reinterpret_cast<int*>(rfree + kMaxCluster * kSlotsOwned);  // [P] block pairs summed of a unit in flight
   int* done = cnt + P;                                                 // block pairs whose unit has been added up
   int* fail = done + 1;                                                // a bounded wait ran out
 
   if (warp < W && lane == 0)
-    for (int s = 0; s < NST; ++s) mbar_init(bars + warp * NST + s, 1);
+    for (int s = 0; s < NST; ++s) mbar_init(bars + warp * NST + s, 1), mbar_init(freed + warp * NST + s, 1);
   if (threadIdx.x == W * 32) {
     for (int s = 0; s < kSlotsOwned; ++s) mbar_init(rfull + s, 1), mbar_expect_tx(rfull + s, C * kPart);
     for (int s = 0; s < kMaxCluster * kSlotsOwned; ++s) mbar_init(rfree + s, 1);
@@ -244,33 +258,52 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
   const int total = (u1 - u0) << lq;                          // this CTA's tasks
   const int r0 = (int)rank * (kRuns / C);                     // this rank's first run
   const bool glu = p.glu != 0;
+  // a warp's next task: one place on in every round of W tasks (blocks that do not divide by eight make every other run longer,
+  // and an even number of warps would give half of them all the long ones: 6144 x 6144 and one row took 9.1 us)
+  auto next_task = [&](int j, int& place) { return ++place < W ? j + W + 1 : (place = 0, j + 1); };
 
-  // ---- the first weights are requested before the activations are there (they do not depend on the launches before) ------
-  uint8_t* myring = ring + (size_t)warp * NST * kUnitBlk;
-  uint64_t* mybar = bars + warp * NST;
-  uint32_t issued = 0;
-  int pj = warp, pb = 0, pe = 0;  // the producer's task and its next and last block
-  const uint8_t* pa = nullptr;
-  const uint64_t pol = policy_evict_first();
-  auto open_task = [&]() {  // the next task with a block in it (K shorter than eight blocks: some runs are empty)
-    while (pb == pe && pj < total) {
-      const int u = u0 + (pj >> lq), r = r0 + (pj & (Q - 1)) * RPT;
-      pb = p.nb * r / kRuns, pe = p.nb * (r + RPT) / kRuns;
-      if (pb == pe) pj += W;
-      else pa = p.w + ((size_t)u * p.nb + pb) * kUnitBlk;
+  if (warp > W) {
+    // ---- the producers: lane l of warp W + 1 + q fills stream warp NP l + q's ring as its stages are freed.  The first weights are
+    // requested before the activations are there: they do not depend on the launches before
+    const int w = NP * lane + (warp - W - 1);
+    uint8_t* myring = ring + (size_t)w * NST * kUnitBlk;
+    uint64_t *mybar = bars + w * NST, *myfreed = freed + w * NST;
+    const uint64_t pol = policy_evict_first();
+    uint32_t issued = 0;
+    int pj = w, place = w, pb = 0, pe = 0;  // the task and its next and last block
+    const uint8_t* pa = nullptr;
+    bool more = w < W;
+    long long t0 = clock64();
+    for (;;) {
+      while (more && pb == pe) {  // the next task with a block in it (K shorter than eight blocks: some runs are empty)
+        if (pj >= total) {
+          more = false;
+          break;
+        }
+        const int u = u0 + (pj >> lq), r = r0 + (pj & (Q - 1)) * RPT;
+        pb = p.nb * r / kRuns, pe = p.nb * (r + RPT) / kRuns, pj = next_task(pj, place);
+        pa = p.w + ((size_t)u * p.nb + pb) * kUnitBlk;
+      }
+      if (!__any_sync(0xffffffffu, more)) break;
+      const uint32_t slot = issued % NST;
+      const bool go = more && (issued < (uint32_t)NST || mbar_test_wait(myfreed + slot, (issued / NST - 1) & 1));
+      if (go) {
+        mbar_expect_tx(mybar + slot, kUnitBlk);
+        bulk_g2s_hint(myring + slot * kUnitBlk, pa, kUnitBlk, mybar + slot, pol);
+        ++issued, ++pb, pa += kUnitBlk;
+      }
+      if (__any_sync(0xffffffffu, go)) {
+        t0 = clock64();
+      } else {
+        if (*reinterpret_cast<volatile int*>(fail) || clock64() - t0 > kWaitCycles) break;
+        __nanosleep(20);
+      }
     }
-    return pj < total;
-  };
-  auto issue = [&]() {
-    const uint32_t slot = issued % NST;
-    mbar_expect_tx(mybar + slot, kUnitBlk);
-    bulk_g2s_hint(myring + slot * kUnitBlk, pa, kUnitBlk, mybar + slot, pol);
-    ++issued, pa += kUnitBlk;
-    if (++pb == pe) pj += W;
-  };
-  if (warp < W && lane == 0)
-    for (int s = 0; s < NST && open_task(); ++s) issue();
-
+    if (__any_sync(0xffffffffu, more)) {  // given up: no copy is left in flight
+      *fail = 1;
+      for (uint32_t n = issued > (uint32_t)NST ? issued - NST : 0; w < W && n < issued; ++n) mbar_wait(mybar + n % NST, (n / NST) & 1);
+    }
+  } else {
   // ---- this rank's activations ------------------------------------------------------------------------------------------
   pdl_wait();
   // tile: [span of 64 k][row][the span's 8 pieces of 8 f16], a piece = the k a lane's word covers, in the words' nibble order;
@@ -284,12 +317,13 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
     stage_row<V::kCol ? 4 : 8>(w, xt + (size_t)b * 8 * span + r * 128, span, !V::kCol && (r & 1),
                                xsum + (size_t)b * 16 * Me + (V::kCol ? 2 * r : (r >> 1) * 4 + (r & 1)), sspan, xscale + b * Me + r, lane);
   }
-  __syncthreads();
+  asm volatile("bar.sync 1, %0;" ::"n"((W + 1) * 32) : "memory");
 
   if (warp < W) {
     // ---- stream warps ---------------------------------------------------------------------------------------------------
     const int g = lane >> 2, t = lane & 3;
-    const uint32_t ring_at = smem_u32(myring);
+    const uint32_t ring_at = smem_u32(ring + (size_t)warp * NST * kUnitBlk);
+    uint64_t *mybar = bars + warp * NST, *myfreed = freed + warp * NST;
     // the lane's column of B is row g of x, or (kCol) row g / 2 in group g % 2; rows past M repeat the last, their sums go unused
     const int half = g & 1, r = min(V::kCol ? g >> 1 : g, M - 1), me = V::kCol ? min(t, M - 1) : min(t, Me / 2 - 1);
     const uint32_t xl = smem_u32(xt) + r * 128 + (V::kCol ? 64 * half + t * 16 : (t * 16) ^ ((r & 1) * 64));
@@ -297,7 +331,7 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
     const uint32_t sl = smem_u32(xsum) + me * (V::kCol ? 8 : 16), fl = smem_u32(xscale) + me * (V::kCol ? 4 : 8);
     uint32_t consumed = 0;
     bool ok = true;
-    for (int j = warp; j < total && ok; j += W) {
+    for (int j = warp, place = warp; j < total && ok; j = next_task(j, place)) {
       const int rt = r0 + (j & (Q - 1)) * RPT;
       float acc[4], lv[3][4];  // the run's sums; the subtrees that wait for their right halves
       int b = p.nb * rt / kRuns;
@@ -327,7 +361,7 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
           }
           ++consumed;
           __syncwarp();
-          if (lane == 0 && open_task()) issue();
+          if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(myfreed + si)) : "memory");
         }
         if (!ok) break;
         // run r closes as many waiting subtrees as it has trailing ones
@@ -361,8 +395,6 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
       if (lane == 0) atomicAdd(cnt + ((j >> lq) & (P - 1)), 1);
     }
     if (!ok) *fail = 1;
-    if (lane == 0)  // (only after a wait that ran out: no copy is left in flight)
-      for (; consumed < issued; ++consumed) mbar_wait(mybar + consumed % NST, (consumed / NST) & 1);
   } else {
     // ---- the adding warp ------------------------------------------------------------------------------------------------
     const int g = lane >> 2, t = lane & 3, n = u1 - u0, lc = p.lc;
@@ -437,6 +469,7 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
     }
     if (!ok) *fail = 1;
   }
+  }
   // (a rank's shared memory is written by the others: nobody leaves before all are done)
   __syncwarp();
   if (C > 1) cluster_sync_all();
@@ -480,10 +513,10 @@ cudaError_t resident_clusters(int C, int* n) {
   return cudaSuccess;
 }
 
-// The division of a launch: a cluster size C (1, 2, 4, 8) and 15 or 11 stream warps (fewer leave more shared memory to the
+// The division of a launch: a cluster size C (1, 2, 4, 8) and 14 or 11 stream warps (fewer leave more shared memory to the
 // activations).  What is compared is the busiest SM's block count, ceil(units / clusters) ceil(blocks / C), where eleven warps
 // stream a tenth slower and a cluster's exchange costs a quarter (12288 x 6144 pair, eight rows: 26 us with eleven warps
-// alone, 31 us with fifteen in clusters of two).
+// alone, 31 us with more in clusters of two).
 struct Division {
   long long cost = 0;
   int C = 0, clusters = 0;
@@ -528,8 +561,8 @@ cudaError_t launch(LinearParams p, const Division& d, cudaStream_t st) {
 // One launch for M rows, or *fits = false where a row's activations do not fit shared memory.
 template <bool kCol>
 static cudaError_t launch_rows(const LinearParams& p, cudaStream_t st, bool* fits) {
-  using Wide = LinVar<kCol, 15, 2, 32>;
-  using Narrow = LinVar<kCol, 11, 2, 32>;
+  using Wide = LinVar<kCol, 14, 1, 2, 32>;
+  using Narrow = LinVar<kCol, 11, 1, 2, 32>;
   Division d;
   bool wide = false, narrow = false;
   cudaError_t e = divide<Wide>(p, &d, &wide);

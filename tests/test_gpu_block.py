@@ -2,8 +2,10 @@
 
 Tolerance, by arithmetic, per output element.  With gamma(K) = (80 + K / 512) 2^-23 a product's f32 sum is off by at most gamma A,
 A = sum |x| (u + z) s (INT4: see the dense products' tests; bf16 weights: exact products, A = sum |x| |W|).  dg, du for gate and
-up; silu's slope is below 1.1, expf, the division and the product are within 8 x 2^-24 of the value, and h is rounded once to bf16:
-    dh = 1.1 dg (|u| + du) + |silu(g)| du + |h| (2^-8 + 8 x 2^-24)      (2^-8: half a step of bf16 relative to the value)
+up; silu's slope is below 1.1, and h is rounded once to bf16.  silu's exponential is the fast one, within 2 + 1.16 |g| steps of
+2^-23 by CUDA's error table: below 95 for |g| <= 80 (beyond that silu is g or below 2^-100), with the division's 2 and the
+product's half a step less than 128 x 2^-23 = 2^-16 of the value:
+    dh = 1.1 dg (|u| + du) + |silu(g)| du + |h| (2^-8 + 2^-16)      (2^-8: half a step of bf16 relative to the value)
     dy = sum_c |W| dh_c + gamma(I) sum_c (|h| + dh)_c (u + z) s
     dout = sum_e w_e dy_e + dy_shared + 2^-20 (sum_e w_e |y_e| + |y_shared| + |res|) + 2^-8 |out|
 (the adds of at most eight picks, the shared expert and the residual, and w's last bits, stay below 2^-20 of what is added).
