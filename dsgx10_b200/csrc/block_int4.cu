@@ -3,8 +3,8 @@
 //
 // Bound: the weights of the distinct picked experts are read once, so HBM.  One CTA a SM, launched cooperatively (all resident
 // together, so CTAs may wait for one another; every wait is bounded and a run-out is recorded in the workspace).  Of a
-// CTA's warps W stream weights, each from a ring of bulk copies that one warp fills for all, one joins their sums and one keeps
-// track of what the other CTAs have done; whoever is free turns activations into the MMAs' operands.
+// CTA's warps W stream weights, each from a ring of bulk copies that two or three more fill for all, one joins their sums and one
+// keeps track of what the other CTAs have done; whoever is free turns activations into the MMAs' operands.
 //
 //   front    every CTA but the last M: the router's logit slices (route.cuh's order).  The last M CTAs route a row each; the
 //            last of them builds the step's table: the picked experts in ascending id with the rows that picked them.
@@ -278,12 +278,12 @@ DSGX_DEV void build_block_tab(BlockTab* out, int* s_idx, int* s_first, const int
   }
 }
 
-// W stream warps with NST ring stages each, the joining warp, the control warp, NP producers, and the rest of sixteen help with
-// activations (sixteen: the routing wants a thread an expert)
+// W stream warps with NST ring stages each, the joining warp, the control warp and NP producers, sixteen together (the routing
+// wants a thread an expert).
 template <int W_, int NST_, int NP_>
 struct BlkVar {
   static constexpr int W = W_, NST = NST_, NP = NP_, kThreads = 512;
-  static_assert(W + 2 + NP <= 16, "warps");
+  static_assert(W + 2 + NP == 16, "warps");
 };
 
 template <class V>
@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
     }
     asm volatile("bar.sync 1, %0;" ::"n"((kLogitW + V::NP) * 32) : "memory");
     if (threadIdx.x == 0) red_release(&sy->cnt_lp, 1);
-  } else if (warp > kStreamW + 1 && warp < kStreamW + 2 + V::NP) {
+  } else if (warp > kStreamW + 1) {
     asm volatile("bar.sync 1, %0;" ::"n"((kLogitW + V::NP) * 32) : "memory");  // (the producers begin when the logits are done)
   }
 
@@ -611,9 +611,9 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
     } else {
       *s_fail = 1;
     }
-  } else if (warp < kStreamW + 2 + V::NP && warp > kStreamW + 1) {
-    // ---- the producer: lane w fills stream warp w's ring as its stages are freed (a warp that fills its own spends 650 to 1000 of
-    // 4400 cycles a stage on it, all of them in its way)
+  } else if (warp > kStreamW + 1) {
+    // ---- the producers: a lane fills one stream warp's ring as its stages are freed (a warp that fills its own spends 650 to 1000 of
+    // 4400 cycles a stage on it, all of them in its way: 168 experts and four rows took 182 us instead of 147)
     const int w = V::NP * lane + (warp - kStreamW - 2);
     uint8_t* myring = ring + (size_t)w * NST * kStage;
     uint64_t *mybar = bars + w * NST, *myfreed = freed + w * NST;
@@ -680,17 +680,6 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
       for (uint32_t n = issued > (uint32_t)NST ? issued - NST : 0; w < kStreamW && n < issued; ++n) mbar_wait(mybar + n % NST, (n / NST) & 1);
     }
     __syncwarp();
-  } else if (warp > kStreamW + 1) {
-    // ---- helpers (the narrow variant's): their share of every segment's activations
-    bool ok = true;
-    for (int k = 0; ok; ++k) {
-      if (k > nb_first) {
-        if (k == nb_first + 1) ok = mbar_wait(tabbar, 0, 20);
-        if (!ok || *s_fail || k >= *s_nseg) break;
-      }
-      ok = k <= nb_first ? prepare(k, k < nb_first || p.b16, 0, 0, p.M) : prepare(k, segs[k].b16, 1, segs[k].slot, segs[k].rows);
-    }
-    if (!ok) *s_fail = 1;
   } else {
     // ---- the control warp: opens the segments, the table when it is there ------------------------------------------------------
     auto open_seg = [&](int k) {
