@@ -473,6 +473,7 @@ int dsgx_linear_decode(const dsgx_linear_w* W, const void* x, int64_t ldx, int M
   if (res && W->glu) return DSGX_ERR_UNSUPPORTED;
   if (((uintptr_t)W->w & 15) || ((uintptr_t)x | (uintptr_t)res) & 1 || (uintptr_t)out & (out_f32 ? 3 : 1) || (uintptr_t)status_word & 3)
     return DSGX_ERR_ARG;
+  if (out == x) return DSGX_ERR_ARG;  // (rows of x are read until the end)
   LinearParams p;
   p.w = W->w, p.glu = W->glu != 0, p.x = reinterpret_cast<const __nv_bfloat16*>(x), p.res = reinterpret_cast<const __nv_bfloat16*>(res);
   p.out = out, p.ldx = ldx, p.ldr = ldr, p.ldo = ldo, p.M = M, p.N = W->N, p.K = W->K;

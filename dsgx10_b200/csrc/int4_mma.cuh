@@ -138,8 +138,9 @@ DSGX_DEV void nibble_order(uint4 (&o)[2], const uint32_t (&w)[8]) {
   }
 }
 
-// One row's 512 k of a block into the activation tile, by one warp (w: a lane's 16 k): f16 times 2^E; the groups' sums times 2^(E - 24); 2^(12 - E).
-// xt: the row's 128-byte line in the block's first span of 64 k, the next span's `span` bytes on; flip: its two groups exchanged; sx: the row's first group sum, GB bytes to the span's second, `sspan` to the next span.
+// One row's 512 k of a block into the activation tile, by one warp (w: a lane's 16 k): f16 times 2^E; the groups' sums times
+// 2^(E - 24); 2^(12 - E).  xt: the row's 128-byte line in the block's first span of 64 k, the next span's `span` bytes on; flip:
+// its two groups exchanged; sx: the row's first group sum, GB bytes to the span's second, `sspan` to the next span.
 template <int GB>
 DSGX_DEV void stage_row(const uint32_t (&w)[8], uint8_t* xt, uint32_t span, bool flip, float* sx, uint32_t sspan, float* scale, int lane) {
   // the largest magnitude (bf16 bits order like numbers; a NaN loses against a number) of the row's 512 values

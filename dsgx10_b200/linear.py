@@ -55,7 +55,7 @@ def _lead(t, M, width, what, device):
 
 def linear_decode(w, x, res=None, out=None, out_dtype=torch.bfloat16, status=None):
     """x bf16 [M][K], M = 1..16 -> out [M][N] (bf16 or f32): x W^T (+ res bf16 [M][N]), or silu(x W^T) * (x Wup^T) where w has
-    an `up` matrix.  x, res and out may be rows of larger tensors (last dimension contiguous); out may be res.
+    an `up` matrix.  x, res and out may be rows of larger tensors (last dimension contiguous); out may be res, not x.
     status: an int32 device tensor that gets DSGX_ERR_DEVICE_WAIT where a bounded wait ran out."""
     dev, bf16 = w.device, torch.bfloat16
     if x.dim() != 2 or not 1 <= x.shape[0] <= _lib.MAX_STEP_ROWS:

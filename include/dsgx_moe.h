@@ -309,7 +309,7 @@ int dsgx_moe_layer_decode(const dsgx_moe_shape* shape, const dsgx_layer_w* L, co
 int dsgx_moe_layer_decode_host(const dsgx_moe_shape* shape, const dsgx_layer_w* L, const void* x_host, int M,
                                const dsgx_layer_step* step, void* out_host, void* stream);
 
-/* ---- a whole INT4 layer in one launch (1..DSGX_MAX_STEP_ROWS rows) -----------------------------------------------------
+/* ---- a whole layer in one launch (1..DSGX_MAX_STEP_ROWS rows) -----------------------------------------------------------
  * out = bf16(res + MoE(x)) of an INT4-g32 or BF16 layer (DSGX_FMT_INT4, DSGX_FMT_BF16; the bf16 shared expert in either form of
  * dsgx_shared_w, or none): router logits, selection, the picked experts, the weighted sum, the residual, in ONE kernel.
  * dsgx_moe_layer_decode runs the same layer as four launches with f32 partial sums for other GPUs; this call is the whole
@@ -347,7 +347,7 @@ int dsgx_moe_block_decode(const dsgx_moe_shape* shape, const dsgx_layer_w* L, co
  * dsgx_linear_prepare re-tiles a matrix once at load, from the experts' blocks (DSGX_FMT_INT4: 8 rows x 512 k,
  * [ceil(N / 8)][ceil(K / 512)], made by dsgx10_b200/weights.py pack_linear_int4 for any N and K >= 1) into the order the
  * product's MMAs want: dsgx_linear_bytes(N, K, glu) bytes at out, 0 for sizes beyond the limits.  w_up not null (glu): two
- * matrices of one shape, gate and up, in one.  One small kernel, nothing allocated; w and w_up may be released after it.
+ * matrices of one shape, gate and up, in one.  Nothing is allocated; w and w_up may be released after it in stream order.
  * What the packer fills rows and columns up with is never seen: rows past N are not written, and columns past K meet
  * zero activations (their scales must be finite). */
 size_t dsgx_linear_bytes(int N, int K, int glu);
@@ -357,7 +357,7 @@ int dsgx_linear_prepare(const void* w, const void* w_up, uint32_t fmt, int N, in
  * res set (not with glu): res[m][n] (bf16) is added to the f32 sum; out may be res.
  * x bf16 [M][ldx], res bf16 [M][ldr], out [M][ldo] bf16, or f32 with out_f32; leading dimensions in elements, any values >= K
  * or N, rows need no alignment beyond their type's (16-byte aligned rows of x are read faster).  out must not overlap x
- * or the weights.  A row's bits depend neither on the other rows of the call nor on their number, and are the same run
+ * (out = x is refused) or the weights.  A row's bits depend neither on the other rows of the call nor on their number, and are the same run
  * after run.  No workspace; asynchronous, graph capturable; calls on several streams may overlap.  The weights must be
  * complete before the launch in front of this one in the stream starts (they are requested early: programmatic dependent
  * launch).  status_word (device, may be null) gets DSGX_ERR_DEVICE_WAIT where a bounded wait ran out.

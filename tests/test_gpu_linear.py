@@ -183,3 +183,56 @@ def test_python_refusals():
     from dsgx10_b200 import _lib
     with pytest.raises(_lib.DsgxError):
         linear.linear_decode(linear.LinearW(N, K, blocks, up=blocks), x, res=torch.zeros(2, N, dtype=torch.bfloat16, device="cuda"))
+
+
+FIRST_USE = """
+import torch
+from dsgx10_b200 import linear, moe, synth, _lib
+cases = []
+for M, N, K, up in ((1, 512, 1024, False), (3, 1000, 5000, False), (16, 256, 9000, False), (8, 512, 6144, True)):
+    n = -(-N // 8) * -(-K // 512)
+    b = torch.randint(0, 256, (n, 2368), dtype=torch.uint8, device="cuda")
+    b[:, 2048:2304].view(n, 128, 2)[:, :, 1] = 0x3B
+    cases.append((linear.LinearW(N, K, b.view(-1), up=b.view(-1) if up else None), torch.randn(M, K, device="cuda").bfloat16()))
+shp = moe.shape(1024, 512, 16, 4, fmt=_lib.FMT_INT4)
+layer, wr = synth.Int4Layer.on_device(1024, 512, 16, 5, "cuda"), synth.router_weights(16, 1024, 7).cuda()
+block, lw, x = moe.MoeBlock(shp, wr), layer.layer_w(), synth.activations(5, 1024, 6).cuda()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = [linear.linear_decode(w, x) for w, x in cases] + [block.run(lw, x)[0]]
+graph.replay()
+torch.cuda.synchronize()
+want = [linear.linear_decode(w, x) for w, x in cases] + [block.run(lw, x)[0]]
+assert all(torch.equal(a, b) for a, b in zip(got, want)) and moe.ws_status(block.ws) == 0
+print("first use captured")
+"""
+
+
+def test_first_use_inside_a_capture():
+    """A process whose first call of each form is captured (device attributes and residencies are asked for on the first call)."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_USE], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "first use captured" in r.stdout, r.stdout + r.stderr
+
+
+def test_prepare_then_product():
+    """Weights used by the very next calls, again and again into the same memory: never the bytes that were there before."""
+    from dsgx10_b200 import linear
+    N, K = 4096, 2048
+    x = _x(1, K, 90).cuda()
+    made = [_make(N, K, 91 + i)[0] for i in range(2)]
+    want = []
+    for b in made:
+        w = linear.LinearW(N, K, b)
+        torch.cuda.synchronize()
+        want.append(linear.linear_decode(w, x).clone())
+    torch.cuda.synchronize()
+    for i in range(40):
+        w = linear.LinearW(N, K, made[i % 2])
+        got = linear.linear_decode(w, x)
+        del w
+        assert torch.equal(got, want[i % 2]), i

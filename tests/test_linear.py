@@ -81,3 +81,10 @@ def test_refused_block_calls():
     shp = moe.shape(1024, 512, 16, 4, fmt=_lib.FMT_FP8)
     assert L.dsgx_moe_block_ws_bytes(C.byref(shp)) == 0
     assert L.dsgx_moe_block_ws_bytes(C.byref(moe.shape(6144, 2048, 168, 8, fmt=_lib.FMT_INT4))) > 0
+
+
+def test_product_in_place_is_refused():
+    """The outputs of one CTA would be another's inputs: out = x is refused, out = res is not looked at."""
+    L, x = _lib.lib(), 1 << 20
+    W = _lib.LinearW(x, 512, 512, _lib.FMT_INT4, 0)
+    assert L.dsgx_linear_decode(C.byref(W), x, 512, 1, None, 0, x, 512, 0, None, None) == _lib.ERR_ARG
