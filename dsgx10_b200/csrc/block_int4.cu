@@ -170,19 +170,35 @@ DSGX_DEV void pair_b16(float (&d)[4], uint32_t st, uint32_t x, uint32_t span, in
 }
 
 // ---- the division of a phase's units over the CTAs.  n shared units of cost cs over the first Gs CTAs, then N routed ones of cost c
-// so that all CTAs end alike; none begins its routed units before a time worth `front` has passed.  Where CTA i's routed run
-// begins.
+// so that all G CTAs end alike; none begins its routed units before a time worth `front` has passed.  N is known with the table
+// only, and every CTA waits for its bounds then: everything else is worked out before, one multiplication and a correction are left.
 DSGX_DEV int shared_begin(int i, int n, int Gs) { return (int)((unsigned)(n * min(i, Gs)) / (unsigned)Gs); }
-DSGX_DEV int routed_begin(int i, int N, int c, int n, int cs, int Gs, int G, int front) {
-  if (i <= 0) return 0;
-  if (i >= G) return N;
-  const int a = n / Gs, few = max(cs * a, front), many = max(cs * (a + 1), front);  // a CTA has a or a + 1 shared units
-  const int extra = shared_begin(i, n, Gs) - a * min(i, Gs), all_extra = n - a * Gs;
-  const long long used = (long long)few * (i - extra) + (long long)many * extra - (i > Gs ? (long long)(few - front) * (i - Gs) : 0);
-  const long long total = (long long)N * c + (long long)few * (G - all_extra) + (long long)many * all_extra - (long long)(few - front) * (G - Gs);
-  if (total < (long long)G * 2 * many) return (int)((long long)N * i / G);  // (few routed units: an even deal)
-  return (int)min((long long)N, max(0ll, (total * i / G - used) / c));
-}
+struct Deal {
+  int i, G, c, many;
+  long long used, rest, D;  // used: G times the cost of what CTAs before i do otherwise; rest: of all; D = c G
+  double inv;
+  DSGX_DEV Deal(int i_, int c_, int n, int cs, int Gs, int G_, int front) : i(i_), G(G_), c(c_) {
+    const int a = n / Gs, few = max(cs * a, front), all_extra = n - a * Gs;  // a CTA has a or a + 1 shared units
+    const int extra = shared_begin(i, n, Gs) - a * min(i, Gs);
+    many = max(cs * (a + 1), front);
+    used = ((long long)few * (i - extra) + (long long)many * extra - (i > Gs ? (long long)(few - front) * (i - Gs) : 0)) * G;
+    rest = (long long)few * (G - all_extra) + (long long)many * all_extra - (long long)(few - front) * (G - Gs);
+    D = (long long)c * G, inv = 1. / (double)D;
+  }
+  // where CTA i's run begins
+  DSGX_DEV int begin(int N) const {
+    if (i <= 0) return 0;
+    if (i >= G) return N;
+    const long long total = (long long)N * c + rest;
+    const bool even = total < (long long)G * 2 * many;  // (few routed units: an even deal)
+    const long long num = even ? (long long)N * i * c : total * i - used;
+    if (num <= 0) return 0;
+    long long q = (long long)((double)num * inv);  // floor(num / D): off by at most one
+    const long long r = num - q * D;
+    q += r < 0 ? -1 : r >= D ? 1 : 0;
+    return (int)min((long long)N, q);
+  }
+};
 
 // One (expert, 1024 k) slice of the router logits for rows [m0, m1): decode_common.cuh's logit_slice_task, sum for sum, with two
 // rows' loads in flight (row after row, eight rows took 7 us).
@@ -268,10 +284,11 @@ DSGX_DEV void build_block_tab(BlockTab* out, int* s_idx, int* s_first, const int
     out->pick[row][place] = slot | __popc(mask & ((1u << row) - 1u)) << 8;
     out->w[row][place] = w;
   }
-  s_idx[i] = bad;  // (read as picks only before the barrier above)
+  bad = (int)__reduce_max_sync(0xffffffffu, (unsigned)bad);
+  if (i == 32) s_idx[0] = bad;  // (read as picks only before the barrier above)
   asm volatile("bar.sync 3, 64;" ::: "memory");
   if (i == 0) {
-    for (int j = 0; j < np; ++j) bad = bad ? bad : s_idx[j];
+    bad = max(bad, s_idx[0]);
     if (bad) atomicCAS(p.status, 0, bad);
     out->nslots = bad ? 0 : n, out->npick = bad ? 0 : p.topk;
     st_release(&p.sync->tab_ready, 1);
@@ -693,7 +710,12 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
       open_seg(k);
       if (ok) ok = prepare(k, k < nb_first || p.b16, 0, 0, p.M);
     }
-    // the table, and from it this CTA's segments
+    // the table, and from it this CTA's segments.  Costs of 8 rows x 512 k in 64 bytes; lanes 0 and 1: this CTA's and the next one's
+    // first up unit, 2 and 3: down
+    const int cI = p.b16 ? 4 * kHBlk / 64 : kQBlk / 64, cS = 4 * kHBlk / 64, nsh = has_sh ? upp : 0, nd = has_sh ? NT : 0;
+    const bool up = lane < 2;
+    const Deal deal(cta + (lane & 1), cI, up ? nsh : nd, cS, up ? Gs : G, G, up ? kFront / (64 * nbH) : 0);
+    const int s0 = shared_begin(cta, nd, G), s1 = shared_begin(cta + 1, nd, G);
     int got = 0;
     if (lane == 0) got = ok && !*s_fail && poll_near(&sy->tab_ready, 1);
     ok = __shfl_sync(0xffffffffu, got, 0) != 0;
@@ -709,22 +731,18 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
           if (i0 + 32 * c < n16) reinterpret_cast<uint4*>(&tab)[i0 + 32 * c] = v[c];
       }
       __syncwarp();
-      // costs of 8 rows x 512 k in 64 bytes; lanes 0 and 1: this CTA's and the next one's first up unit, 2 and 3: down
-      const int cI = p.b16 ? 4 * kHBlk / 64 : kQBlk / 64, cS = 4 * kHBlk / 64, up = lane < 2;
-      const int NU = tab.nslots * upp, ND = tab.nslots * NT, nsh = has_sh ? upp : 0, nd = has_sh ? NT : 0;
-      const int at = routed_begin(cta + (lane & 1), up ? NU : ND, cI, up ? nsh : nd, cS, up ? Gs : G, G, up ? kFront / (64 * nbH) : 0);
+      const int at = deal.begin(tab.nslots * (up ? upp : NT));
       const int u0 = __shfl_sync(0xffffffffu, at, 0), u1 = __shfl_sync(0xffffffffu, at, 1);
       const int d0 = __shfl_sync(0xffffffffu, at, 2), d1 = __shfl_sync(0xffffffffu, at, 3);
       if (lane == 0) {
         int nseg = nb_first, base = (a1 - a0) * QH;
         segs[nseg++] = Seg{0, p.b16, 0, p.M, u0, u1 - u0, (u1 - u0) * QH, base}, base += (u1 - u0) * QH;
-        const int s0 = shared_begin(cta, nd, G), s1 = shared_begin(cta + 1, nd, G);
         if (s1 > s0) {
           mbar_init(tile_full + nseg, p.M * nbI);
           segs[nseg++] = Seg{1, 1, kShared, p.M, s0, s1 - s0, (s1 - s0) * QI, base}, base += (s1 - s0) * QI;
         }
-        for (int d = d0; d < d1;) {
-          const int slot = d / NT, e = min(d1, (slot + 1) * NT), n = tab.ent[slot].n;
+        for (int d = d0, slot = d0 / NT; d < d1; ++slot) {
+          const int e = min(d1, (slot + 1) * NT), n = tab.ent[slot].n;
           mbar_init(tile_full + nseg, n * nbI);
           segs[nseg++] = Seg{1, p.b16, slot, n, d - slot * NT, e - d, (e - d) * QI, base}, base += (e - d) * QI;
           d = e;
