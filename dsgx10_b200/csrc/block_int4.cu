@@ -229,45 +229,56 @@ DSGX_DEV void logit_rows(const __nv_bfloat16* __restrict__ x, const float* __res
   }
 }
 
-// ---- the table, by the first 64 threads of a CTA, a thread a pick, written straight to global memory.  s_idx, s_first: kMaxEnt
-// words of shared memory each.  idx, ws: the picks in shared memory (one row), or null: p.idx, p.w.
-DSGX_DEV void build_block_tab(BlockTab* out, int* s_idx, int* s_first, const int* idx, const float* ws, const BlockParams& p) {
+// ---- the table, by the first 64 threads of a CTA, a thread a pick, written straight to global memory.  An expert's picks and the
+// experts picked are bit masks in shared memory (zero at the start), so that a slot is a count of bits.
+struct alignas(16) TabSmem {
+  uint32_t of[512][2];  // the picks of an expert
+  uint32_t any[16];     // the experts that were picked
+  int idx[kMaxEnt];
+  int bad;
+  int pick[kMaxTopK];   // one row's picks and weights, from the routing
+  float w[kMaxTopK];
+};
+static_assert(sizeof(TabSmem) <= kP * kPart, "in the place of the tasks' sums");
+DSGX_DEV void build_block_tab(BlockTab* out, TabSmem& sm, const BlockParams& p) {
   constexpr int kNone = 0x7fffffff;
   const int i = threadIdx.x, np = p.M * p.topk;
   const bool in = i < np;
-  int e = in ? (idx ? idx[i] : __ldcg(p.idx + i)) : kNone;
-  const float w = in ? (ws ? ws[i] : __ldcg(p.w + i)) : 0.f;
+  int e = in ? (p.M == 1 ? sm.pick[i] : __ldcg(p.idx + i)) : kNone;
+  const float w = in ? (p.M == 1 ? sm.w[i] : __ldcg(p.w + i)) : 0.f;
   const bool bad_id = in && (e < 0 || e >= p.E);
   if (bad_id) e = kNone;
   uint4 d[3];  // off, s2, fmt of the expert's three descriptors
-  if (e != kNone)
+  if (e != kNone) {
 #pragma unroll
     for (int m = 0; m < 3; ++m) d[m] = __ldg(reinterpret_cast<const uint4*>(p.desc + (size_t)e * 3 + m));
-  s_idx[i] = e;
+    atomicOr(&sm.of[e][i >> 5], 1u << (i & 31));
+    atomicOr(&sm.any[e >> 5], 1u << (e & 31));
+  }
+  sm.idx[i] = e;
   asm volatile("bar.sync 3, 64;" ::: "memory");
-  bool first = e != kNone;
+  // (rolled loops: this code runs once a launch, its instructions come from memory)
+  int upto = (i & 31) < 16 ? __popc(sm.any[i & 15]) : 0;  // distinct experts up to the lane's word
+  const int own = upto;
+#pragma unroll 1
+  for (int o = 1; o < 16; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, upto, o);
+    if ((i & 31) >= o) upto += v;
+  }
+  const int n = __shfl_sync(0xffffffffu, upto, 15);
+  int slot = __shfl_sync(0xffffffffu, upto - own, e >> 5 & 15);
+  unsigned long long of = 0;
+  if (e != kNone) slot += __popc(sm.any[e >> 5] & ((1u << (e & 31)) - 1u)), of = *reinterpret_cast<const unsigned long long*>(sm.of[e]);
+  const bool first = e != kNone && __ffsll((long long)of) - 1 == i;
   uint32_t mask = 0;  // the rows that picked the expert
-  const int row = i / p.topk, recip = 65536 / p.topk + 1;  // (j recip >> 16 = j / topk for j < 64)
+  const uint32_t picks = (1u << p.topk) - 1u;
+#pragma unroll 1
+  for (int r = 0; r < p.M; ++r, of >>= p.topk)
+    if ((uint32_t)of & picks) mask |= 1u << r;
+  const int row = in ? i / p.topk : 0;
   int place = 0;  // the pick's place in its row's ascending order
-#pragma unroll 4
-  for (int j4 = 0; j4 < (np + 3) / 4; ++j4) {
-    const int4 o4 = reinterpret_cast<const int4*>(s_idx)[j4];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int j = 4 * j4 + c, o = c == 0 ? o4.x : c == 1 ? o4.y : c == 2 ? o4.z : o4.w, r = j * recip >> 16;
-      if (o == e) mask |= 1u << r, first = first && j >= i;
-      place += r == row && o < e;
-    }
-  }
-  s_first[i] = first ? e : kNone;
-  asm volatile("bar.sync 3, 64;" ::: "memory");
-  int slot = 0, n = 0;
-#pragma unroll 4
-  for (int j4 = 0; j4 < (np + 3) / 4; ++j4) {
-    const int4 o4 = reinterpret_cast<const int4*>(s_first)[j4];
-    slot += (o4.x < e) + (o4.y < e) + (o4.z < e) + (o4.w < e);
-    n += (o4.x != kNone) + (o4.y != kNone) + (o4.z != kNone) + (o4.w != kNone);
-  }
+#pragma unroll 1
+  for (int j = 0; j < p.topk; ++j) place += sm.idx[row * p.topk + j] < e;
   int bad = bad_id ? DSGX_ERR_ARG : 0;
   if (first) {
     if (d[0].w != p.fmt || d[1].w != p.fmt || d[2].w != p.fmt) bad = DSGX_ERR_FORMAT;
@@ -275,9 +286,8 @@ DSGX_DEV void build_block_tab(BlockTab* out, int* s_idx, int* s_first, const int
     en.g = p.pool + ((uint64_t)d[0].x | (uint64_t)d[0].y << 32), en.u = p.pool + ((uint64_t)d[1].x | (uint64_t)d[1].y << 32);
     en.d = p.pool + ((uint64_t)d[2].x | (uint64_t)d[2].y << 32);
     en.rows = 0, en.n = 0, en.pad[0] = en.pad[1] = en.pad[2] = 0;
-#pragma unroll
-    for (int q = 0; q < kMaxRows; ++q)
-      if (mask >> q & 1) en.rows |= (unsigned long long)q << (8 * en.n++);
+#pragma unroll 1
+    for (uint32_t left = mask; left; left &= left - 1) en.rows |= (unsigned long long)(__ffs((int)left) - 1) << (8 * en.n++);
     out->ent[slot] = en;
   }
   if (in) {
@@ -285,10 +295,10 @@ DSGX_DEV void build_block_tab(BlockTab* out, int* s_idx, int* s_first, const int
     out->w[row][place] = w;
   }
   bad = (int)__reduce_max_sync(0xffffffffu, (unsigned)bad);
-  if (i == 32) s_idx[0] = bad;  // (read as picks only before the barrier above)
+  if (i == 32) sm.bad = bad;
   asm volatile("bar.sync 3, 64;" ::: "memory");
   if (i == 0) {
-    bad = max(bad, s_idx[0]);
+    bad = max(bad, sm.bad);
     if (bad) atomicCAS(p.status, 0, bad);
     out->nslots = bad ? 0 : n, out->npick = bad ? 0 : p.topk;
     st_release(&p.sync->tab_ready, 1);
@@ -343,6 +353,11 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
   const bool router = cta >= Gs;
   // the run that needs no routing: the shared expert's gate and up
   const int a0 = has_sh && !router ? shared_begin(cta, upp, Gs) : 0, a1 = has_sh && !router ? shared_begin(cta + 1, upp, Gs) : 0;
+  if (router) {  // (build_block_tab)
+    TabSmem& ts = *reinterpret_cast<TabSmem*>(part);
+    ts.of[threadIdx.x][0] = ts.of[threadIdx.x][1] = 0u;
+    if (threadIdx.x < 16) ts.any[threadIdx.x] = 0u;
+  }
   if (threadIdx.x == 0) {
     mbar_init(tabbar, 1);
     *done = 0, *s_nseg = 0, *s_fail = 0;
@@ -372,49 +387,6 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
       while (c.u >= upp) c.u -= upp, ++c.slot;
   };
   const int nb_first = a1 > a0 ? 1 : 0;  // segments whose units are known without the table
-
-  if (router) {
-    // ---- a row each; the last one to be routed builds the table -------------------------------------------------------------
-    RouteSmem& rs = *reinterpret_cast<RouteSmem*>(tiles);
-    int* s_idx = reinterpret_cast<int*>(part);
-    int* s_pick = s_idx + 2 * kMaxEnt;
-    float* s_w = reinterpret_cast<float*>(s_pick + kMaxTopK);
-    const int row = cta - Gs, KS = (p.H + 1023) / 1024, nt = (p.E + 31) & ~31;
-    for (int i = threadIdx.x; i < p.E * 3; i += kThreads) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.desc + i));
-    if (threadIdx.x == 0) *s_tick = poll_near(&sy->cnt_lp, Gs) ? 1 : 0;
-    __syncthreads();
-    const bool ok = *s_tick != 0;
-    __syncthreads();
-    if (ok) {
-      if ((int)threadIdx.x < nt)
-        route_row_cta(p.rp, p.lpart + (size_t)row * p.E, KS, (size_t)kMaxRows * p.E, p.bias, rs, nullptr, p.idx + row * p.topk,
-                      p.w + row * p.topk, p.M == 1 ? s_pick : nullptr, s_w, CtaPart{nt, 2});
-      if (warp == 0) {  // (warp 0 wrote the picks)
-        __syncwarp();
-        if (lane == 0) *s_tick = p.M > 1 ? atom_add_acq_rel(&sy->cnt_rt, 1) : 0;
-      }
-      __syncthreads();
-      if (*s_tick == p.M - 1 && threadIdx.x < 64)
-        build_block_tab(p.tab, s_idx, s_idx + kMaxEnt, p.M == 1 ? s_pick : nullptr, p.M == 1 ? s_w : nullptr, p);
-    } else if (threadIdx.x == 0) {
-      *s_fail = 1;
-    }
-    __syncthreads();
-  } else if (warp < kLogitW) {
-    // ---- the router's logit slices, one warp a (expert, 1024 k); a CTA reports when all of its are in memory.  (The rings
-    // filled first: 2.4 us later logits and not a microsecond gained on the shared expert.) ------------------------------------
-    const int KS = (p.H + 1023) / 1024, ntask = p.E * KS;
-    // (more warps than slices: a slice's rows over several warps)
-    const int parts = min(p.M, max(1, kLogitW * Gs / ntask)), per = (p.M + parts - 1) / parts;
-    for (int i = warp * Gs + cta; i < ntask * parts; i += kLogitW * Gs) {
-      const int slice = i / parts, m = (i - slice * parts) * per;
-      logit_rows(p.x, p.wr, m, min(p.M, m + per), p.H, p.E, slice / KS, slice % KS, p.lpart, lane);
-    }
-    asm volatile("bar.sync 1, %0;" ::"n"((kLogitW + V::NP) * 32) : "memory");
-    if (threadIdx.x == 0) red_release(&sy->cnt_lp, 1);
-  } else if (warp > kStreamW + 1) {
-    asm volatile("bar.sync 1, %0;" ::"n"((kLogitW + V::NP) * 32) : "memory");  // (the producers begin when the logits are done)
-  }
 
   // ---- a segment's activation tile: the shared expert's x, the routed experts' x, then the down segments in the first tile's place
   auto tile_at = [&](int k) { return tiles + (k <= nb_first ? (k == nb_first ? (p.nbuf - 1) * p.tile : 0) : (k - nb_first - 1) % p.nbuf_down * p.tile_down); };
@@ -447,6 +419,53 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
       if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(tile_full + k)) : "memory");
     }
   };
+
+  if (router) {
+    // ---- a row each; the last one to be routed builds the table -------------------------------------------------------------
+    RouteSmem& rs = *reinterpret_cast<RouteSmem*>(ring);  // (nothing is streamed yet)
+    TabSmem& ts = *reinterpret_cast<TabSmem*>(part);
+    const int row = cta - Gs, KS = (p.H + 1023) / 1024, nt = (p.E + 31) & ~31, ng = max(nt, 64);
+    auto sync = [&]() { asm volatile("bar.sync 4, %0;" ::"r"(ng) : "memory"); };
+    if (threadIdx.x == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(seg_open)) : "memory");
+    if ((int)threadIdx.x >= ng) {  // (the routed experts' x meanwhile; after the routing, these CTAs began to stream 5 us late)
+      prepare(0, p.b16, 0, 0, p.M);
+    } else {
+      for (int i = threadIdx.x; i < p.E * 3; i += ng) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.desc + i));
+      if (threadIdx.x == 0) *s_tick = poll_near(&sy->cnt_lp, Gs) ? 1 : 0;
+      sync();
+      const bool ok = *s_tick != 0;
+      sync();
+      if (ok) {
+        if ((int)threadIdx.x < nt)
+          route_row_cta(p.rp, p.lpart + (size_t)row * p.E, KS, (size_t)kMaxRows * p.E, p.bias, rs, nullptr, p.idx + row * p.topk,
+                        p.w + row * p.topk, p.M == 1 ? ts.pick : nullptr, ts.w, CtaPart{nt, 2});
+        if (warp == 0) {  // (warp 0 wrote the picks)
+          __syncwarp();
+          if (lane == 0) *s_tick = p.M > 1 ? atom_add_acq_rel(&sy->cnt_rt, 1) : 0;
+        }
+        sync();
+        if (*s_tick == p.M - 1 && threadIdx.x < 64) build_block_tab(p.tab, ts, p);
+      } else if (threadIdx.x == 0) {
+        *s_fail = 1;
+      }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (bulk copies write the routing's scratch next)
+    __syncthreads();
+  } else if (warp < kLogitW) {
+    // ---- the router's logit slices, one warp a (expert, 1024 k); a CTA reports when all of its are in memory.  (The rings
+    // filled first: 2.4 us later logits and not a microsecond gained on the shared expert.) ------------------------------------
+    const int KS = (p.H + 1023) / 1024, ntask = p.E * KS;
+    // (more warps than slices: a slice's rows over several warps)
+    const int parts = min(p.M, max(1, kLogitW * Gs / ntask)), per = (p.M + parts - 1) / parts;
+    for (int i = warp * Gs + cta; i < ntask * parts; i += kLogitW * Gs) {
+      const int slice = i / parts, m = (i - slice * parts) * per;
+      logit_rows(p.x, p.wr, m, min(p.M, m + per), p.H, p.E, slice / KS, slice % KS, p.lpart, lane);
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"((kLogitW + V::NP) * 32) : "memory");
+    if (threadIdx.x == 0) red_release(&sy->cnt_lp, 1);
+  } else if (warp > kStreamW + 1) {
+    asm volatile("bar.sync 1, %0;" ::"n"((kLogitW + V::NP) * 32) : "memory");  // (the producers begin when the logits are done)
+  }
 
   if (warp < kStreamW) {
     // ---- stream warps --------------------------------------------------------------------------------------------------------
@@ -707,7 +726,7 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
     // x: in bf16 for the shared expert, as their format wants it for the routed ones
     for (int k = 0; k <= nb_first && ok; ++k) {
       if (k > 0 && p.nbuf == 1) ok = mbar_wait(tile_free, 0, 20);
-      open_seg(k);
+      if (!router) open_seg(k);
       if (ok) ok = prepare(k, k < nb_first || p.b16, 0, 0, p.M);
     }
     // the table, and from it this CTA's segments.  Costs of 8 rows x 512 k in 64 bytes; lanes 0 and 1: this CTA's and the next one's
@@ -820,8 +839,7 @@ size_t block_smem(size_t tile, int nbuf) {
          kMaxSegs * (sizeof(Seg) + 4) + 24 * 4 + (kP + 4) * 4 + 16;
 }
 size_t block_tile(int H, int I, int M) {
-  size_t t = tile_bytes(H, M) > tile_bytes(I, M) ? tile_bytes(H, M) : tile_bytes(I, M);
-  return t > sizeof(RouteSmem) ? t : (sizeof(RouteSmem) + 127) & ~(size_t)127;  // (the routing's scratch before the first tile)
+  return tile_bytes(H, M) > tile_bytes(I, M) ? tile_bytes(H, M) : tile_bytes(I, M);
 }
 
 template <class V>
