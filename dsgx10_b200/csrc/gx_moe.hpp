@@ -107,4 +107,27 @@ inline void layer_decode(const MoeShape& s, const LayerW& L, const __nv_bfloat16
   check(dsgx_moe_layer_decode(&s, &L, x, M, &step, finalize ? 1 : 0, st), "gx::layer_decode");
 }
 
+// a whole INT4 or BF16 layer for 1..16 rows in one launch: out = bf16(res + MoE(x))
+using MoeBlock = dsgx_moe_block;
+inline size_t moe_block_ws_bytes(const MoeShape& s) { return dsgx_moe_block_ws_bytes(&s); }
+inline void moe_block_decode(const MoeShape& s, const LayerW& L, const __nv_bfloat16* x, int M, const MoeBlock& block,
+                             const __nv_bfloat16* res, __nv_bfloat16* out, cudaStream_t st) {
+  check(dsgx_moe_block_decode(&s, &L, x, M, &block, res, out, st), "gx::moe_block_decode");
+}
+// dense products with 4-bit weights (engine/attn/attn.h glm::gemv): prepared once at load, then x W^T (+ res), or silu(x W^T) * (x Wup^T)
+using LinearW = dsgx_linear_w;
+inline size_t linear_bytes(int N, int K, bool glu = false) { return dsgx_linear_bytes(N, K, glu ? 1 : 0); }
+inline LinearW linear_prepare(const void* blocks, const void* up_blocks, int N, int K, void* out, cudaStream_t st) {
+  check(dsgx_linear_prepare(blocks, up_blocks, DSGX_FMT_INT4, N, K, out, st), "gx::linear_prepare");
+  return LinearW{static_cast<const uint8_t*>(out), N, K, DSGX_FMT_INT4, up_blocks ? 1 : 0};
+}
+inline void linear_decode(const LinearW& w, const __nv_bfloat16* x, int64_t ldx, int M, const __nv_bfloat16* res, int64_t ldr,
+                          __nv_bfloat16* out, int64_t ldo, cudaStream_t st, int* status_word = nullptr) {
+  check(dsgx_linear_decode(&w, x, ldx, M, res, ldr, out, ldo, 0, status_word, st), "gx::linear_decode");
+}
+inline void linear_decode(const LinearW& w, const __nv_bfloat16* x, int64_t ldx, int M, float* out, int64_t ldo, cudaStream_t st,
+                          int* status_word = nullptr) {
+  check(dsgx_linear_decode(&w, x, ldx, M, nullptr, 0, out, ldo, 1, status_word, st), "gx::linear_decode");
+}
+
 }  // namespace gx
