@@ -14,6 +14,11 @@
 //            expert's h is complete; their weights are already in the rings.
 //   combine  after a grid-wide count: every element adds its row's picks, the shared expert and the residual.
 //
+// Measured (a captured chain, more weights than L2 holds): 168 experts of 6144 x 2048, eight picks a row and the shared expert, one
+// row 60 us (254 MB, 4.3 TB/s; four launches 76), four rows 147 us (717 MB, 4.9 TB/s; 231), eight rows 257 us (434); 1024 x 512
+// and 16 experts, one row: 22 us, all of it the chain of six grid-wide steps (four launches 18).  About 16 us pass until routed
+// weights stream; from then on 85 % of a copy's rate, the warps' chains of loads, MMAs and f32 operations next to HBM.
+//
 // Work items.  A unit (16 weight rows) is cut along K in tasks of about two 512-k blocks, dealt to the stream warps in turn
 // across units and phases; a task's sums go to shared memory and the joining warp adds a unit's tasks in ascending k.  The cut
 // depends on H and I alone, so a row's bits do not depend on the other rows.
