@@ -14,6 +14,7 @@ import torch
 
 from . import _lib
 from ._lib import check, lib
+from .moe import raw_stream
 
 
 class LinearW:
@@ -38,10 +39,6 @@ class LinearW:
         self.ref = C.byref(self.c)
 
 
-# (the stream's handle without building a Stream object, where torch has that call: 2 us of a 12 us host call)
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
-
-
 def _lead(t, M, width, what, device):
     """The leading dimension of a [M][width] operand, checked."""
     shape = t.shape
@@ -58,25 +55,28 @@ def linear_decode(w, x, res=None, out=None, out_dtype=torch.bfloat16, status=Non
     an `up` matrix.  x, res and out may be rows of larger tensors (last dimension contiguous); out may be res, not x.
     status: an int32 device tensor that gets DSGX_ERR_DEVICE_WAIT where a bounded wait ran out."""
     dev, bf16 = w.device, torch.bfloat16
+    if x.dtype is not bf16 or (res is not None and res.dtype is not bf16):
+        raise ValueError(f"linear_decode: x {x.dtype}, res {None if res is None else res.dtype}; wanted bf16")
     if x.dim() != 2 or not 1 <= x.shape[0] <= _lib.MAX_STEP_ROWS:
         raise ValueError(f"linear_decode: x has shape {tuple(x.shape)}; 1..{_lib.MAX_STEP_ROWS} rows of {w.K} are taken")
     M = x.shape[0]
     ldx = _lead(x, M, w.K, "x", dev)
     if out is None:
-        out = torch.empty(M, w.N, dtype=out_dtype, device=dev)
-    ldo = _lead(out, M, w.N, "out", dev)
+        out, ldo = (x.new_empty(M, w.N) if out_dtype is bf16 else torch.empty(M, w.N, dtype=out_dtype, device=dev)), w.N
+    else:
+        ldo = _lead(out, M, w.N, "out", dev)
+    if out.dtype is not bf16 and out.dtype is not torch.float32:
+        raise ValueError(f"linear_decode: out {out.dtype}; wanted bf16 or f32")
     ldr, resp = (0, None) if res is None else (_lead(res, M, w.N, "res", dev), res.data_ptr())
-    if x.dtype is not bf16 or (out.dtype is not bf16 and out.dtype is not torch.float32) or (res is not None and res.dtype is not bf16):
-        raise ValueError(f"linear_decode: x {x.dtype}, out {out.dtype}, res {None if res is None else res.dtype}; wanted bf16, out bf16 or f32")
     if status is not None and (status.dtype != torch.int32 or status.device != dev or status.numel() < 1):
         raise ValueError("linear_decode: status is an int32 tensor on the weights' device")
     args = (w.ref, x.data_ptr(), ldx, M, resp, ldr, out.data_ptr(), ldo, 0 if out.dtype is bf16 else 1,
             None if status is None else status.data_ptr())
     if torch.cuda.current_device() == dev.index:
-        rc = _decode()(*args, _raw_stream(dev.index))
+        rc = _decode()(*args, raw_stream(dev.index))
     else:
         with torch.cuda.device(dev):
-            rc = _decode()(*args, _raw_stream(dev.index))
+            rc = _decode()(*args, raw_stream(dev.index))
     if rc:
         check(rc, "dsgx_linear_decode")
     return out

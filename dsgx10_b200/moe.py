@@ -178,6 +178,10 @@ class LayerStep:
         return out_host
 
 
+# the stream's handle without building a Stream object, where torch has that call (2 us of a 16 us host call)
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
 class MoeBlock:
     """A whole INT4 or BF16 layer for 1..16 rows in one launch (dsgx_moe_block_decode): out = res + MoE(x)."""
 
@@ -205,9 +209,14 @@ class MoeBlock:
         for t, what in ((x, "x"), (res, "res"), (out, "out")):
             if t is not None and (t.dtype is not torch.bfloat16 or t.shape != (M, self.shp.H) or not t.is_contiguous() or t.device != dev):
                 raise ValueError(f"MoeBlock: {what} must be contiguous bf16 [M][{self.shp.H}] on {dev}")
-        with torch.cuda.device(dev):
-            check(lib().dsgx_moe_block_decode(self.shp_ref, C.byref(layer_w), x.data_ptr(), M, self.ref, _ptr(res), out.data_ptr(),
-                                              torch.cuda.current_stream(dev).cuda_stream), "dsgx_moe_block_decode")
+        args = (self.shp_ref, C.byref(layer_w), x.data_ptr(), M, self.ref, _ptr(res), out.data_ptr())
+        if torch.cuda.current_device() == dev.index:
+            rc = lib().dsgx_moe_block_decode(*args, raw_stream(dev.index))
+        else:
+            with torch.cuda.device(dev):
+                rc = lib().dsgx_moe_block_decode(*args, raw_stream(dev.index))
+        if rc:
+            check(rc, "dsgx_moe_block_decode")
         return out, self.idx[:M], self.w[:M]
 
 
