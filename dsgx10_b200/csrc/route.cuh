@@ -304,7 +304,9 @@ DSGX_DEV void route_row_cta(const RouteParams& p, const float* __restrict__ l, i
       if (lane == 0) sm.S = ps;
     }
     cp.sync();
-    s = __fdiv_rn(t, sm.S);
+    // (0 / S is 0: a zero, as every lane past the last expert holds, takes the division's long way, cold code of 1 to 4 us)
+    const float S = sm.S, quot = __fdiv_rn(t == 0.f ? 1.f : t, S);
+    s = t == 0.f && S == S ? 0.f : quot;
     cp.sync();
   }
   // keys as order-preserving unsigned integers in shared memory (0 = not a candidate)
