@@ -83,6 +83,15 @@ DSGX_DEV int atom_add_acq_rel(int* p, int v) {
   asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], %2;" : "=r"(o) : "l"(p), "r"(v) : "memory");
   return o;
 }
+DSGX_DEV void arrive(uint64_t* bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory"); }
+// mbar_wait without the suspended try: the joining warp's wake-up is on every unit's path
+DSGX_DEV bool mbar_spin(uint64_t* bar, uint32_t parity) {
+  if (mbar_test_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!mbar_test_wait(bar, parity))
+    if (clock64() - t0 > kWaitCycles) return false;
+  return true;
+}
 // bounded poll until *p >= target (decode_common.cuh's poll_ge with a shorter sleep: these waits are on the critical path)
 DSGX_DEV bool poll_near(const int* p, int target) {
   if (ld_acquire(p) >= target) return true;
@@ -336,20 +345,20 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
   uint64_t* tile_full = seg_open + kMaxSegs;              // [kMaxSegs] they are in the tile (an arrival a row and block)
   uint64_t* tile_free = tile_full + kMaxSegs;             // [kMaxSegs] no stream warp reads them any more
   uint64_t* tabbar = tile_free + kMaxSegs;                // the table and all segments are known
-  Seg* segs = reinterpret_cast<Seg*>(tabbar + 2);
+  uint64_t* full = tabbar + 2;                            // [kP] a task's sums are in their place
+  uint64_t* emptied = full + kP;                          // [kP] its unit has been joined
+  Seg* segs = reinterpret_cast<Seg*>(emptied + kP);
   int* first_blk = reinterpret_cast<int*>(segs + kMaxSegs);  // [2][12] a task's first block, of K = H and of K = I
   int* claim = first_blk + 24;                            // [kMaxSegs] rows and blocks that a warp has taken on
-  int* cnt = claim + kMaxSegs;                            // [kP] tasks summed of a unit in flight
-  int* done = cnt + kP;                                   // tasks whose unit has been joined
-  int* s_nseg = done + 1;
-  int* s_fail = done + 2;
-  int* s_tick = done + 3;
+  int* s_nseg = claim + kMaxSegs;
+  int* s_fail = s_nseg + 1;
+  int* s_tick = s_nseg + 2;
   BlockSync* sy = p.sync;
 
   if (warp < kStreamW && lane == 0)
     for (int s = 0; s < NST; ++s) mbar_init(bars + warp * NST + s, 1), mbar_init(freed + warp * NST + s, 1);
   for (int i = threadIdx.x; i < kMaxSegs; i += kThreads) mbar_init(seg_open + i, 1), mbar_init(tile_free + i, kStreamW), claim[i] = 0;
-  if (threadIdx.x < kP) cnt[threadIdx.x] = 0;
+  if (threadIdx.x < kP) mbar_init(full + threadIdx.x, 1), mbar_init(emptied + threadIdx.x, 1);
   if (threadIdx.x < 8) reinterpret_cast<uint32_t*>(zero)[threadIdx.x] = 0;
   if (threadIdx.x <= 8) first_blk[threadIdx.x] = nbH * (int)threadIdx.x / QH, first_blk[12 + threadIdx.x] = nbI * (int)threadIdx.x / QI;
 
@@ -365,7 +374,7 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
   }
   if (threadIdx.x == 0) {
     mbar_init(tabbar, 1);
-    *done = 0, *s_nseg = 0, *s_fail = 0;
+    *s_nseg = 0, *s_fail = 0;
     segs[0] = Seg{0, 1, kShared, p.M, a0, a1 - a0, (a1 - a0) * QH, 0};
     mbar_init(tile_full, p.M * nbH);
     if (a1 > a0) mbar_init(tile_full + 1, p.M * nbH);  // (the down segments' are set when they are known, each once)
@@ -421,7 +430,7 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
       }
       __threadfence_block();
       __syncwarp();
-      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(tile_full + k)) : "memory");
+      if (lane == 0) arrive(tile_full + k);
     }
   };
 
@@ -431,7 +440,7 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
     TabSmem& ts = *reinterpret_cast<TabSmem*>(part);
     const int row = cta - Gs, KS = (p.H + 1023) / 1024, nt = (p.E + 31) & ~31, ng = max(nt, 64);
     auto sync = [&]() { asm volatile("bar.sync 4, %0;" ::"r"(ng) : "memory"); };
-    if (threadIdx.x == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(seg_open)) : "memory");
+    if (threadIdx.x == 0) arrive(seg_open);
     if ((int)threadIdx.x >= ng) {  // (the routed experts' x meanwhile; after the routing, these CTAs began to stream 5 us late)
       prepare(0, p.b16, 0, 0, p.M);
     } else {
@@ -477,7 +486,6 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
     const uint32_t ring_at = smem_u32(ring + (size_t)warp * NST * kStage);
     uint64_t *mybar = bars + warp * NST, *myfreed = freed + warp * NST;
     uint32_t consumed = 0;
-    int joined = 0;  // tasks joined when last looked at
     bool ok = true;
     auto stage_ready = [&]() {
       const uint32_t si = consumed % NST;
@@ -486,7 +494,7 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
     };
     auto stage_used = [&]() {
       __syncwarp();
-      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(myfreed + consumed % NST)) : "memory");
+      if (lane == 0) arrive(myfreed + consumed % NST);
       ++consumed;
     };
 
@@ -582,18 +590,15 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
           else run(std::integral_constant<int, 1>());
         }
         if (!ok) break;
-        const int j = s.base + c.i;
-        if (j >= joined + kP) {  // (the place of the sums is free once the unit that had it has been joined)
-          if (!(ok = wait_shared_ge(done, j - kP + 1, 100))) break;
-          joined = ld_shared_acquire(done);
-        }
-        float2* d = reinterpret_cast<float2*>(part + (j % kP) * kPart) + lane;
+        const unsigned j = s.base + c.i, place = j % kP;
+        if (j >= kP && !(ok = mbar_wait(emptied + place, (j / kP - 1) & 1))) break;
+        float2* d = reinterpret_cast<float2*>(part + place * kPart) + lane;
 #pragma unroll
         for (int e = 0; e < S; ++e) d[32 * e] = make_float2(acc[e][0], acc[e][1]);
         __syncwarp();
-        if (lane == 0) red_shared_release(cnt + (j - c.q) % kP, 1);
+        if (lane == 0) arrive(full + place);
       }
-      if (ok && lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(tile_free + k)) : "memory");
+      if (ok && lane == 0) arrive(tile_free + k);
     }
     if (!ok) *s_fail = 1;
   } else if (warp == kStreamW) {
@@ -611,22 +616,28 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
       int slot = s.slot, u = s.u0, reported = 0;
       if (!s.down && s.slot != kShared) slot = u / upp, u -= slot * upp;
       int n = slot == kShared ? p.M : tab.ent[slot].n;
-      for (int i = 0, j = s.base; i < s.n && ok; ++i, j += Q, ++u) {
+      unsigned j = s.base;
+      for (int i = 0; i < s.n && ok; ++i, j += Q, ++u) {
         if (!s.down && s.slot != kShared && u == upp) u = 0, n = tab.ent[++slot].n;
-        int* c = cnt + j % kP;
-        if (!(ok = wait_shared_ge(c, Q, 0))) break;
-        float2 v[S];
-        for (int q = 0; q < Q; ++q) {
-          const float2* d = reinterpret_cast<const float2*>(part + ((j + q) % kP) * kPart) + lane;
+        const unsigned at = j + lane;  // lane q < Q: the unit's task q
+        const bool there = lane >= Q || mbar_spin(full + at % kP, at / kP & 1);
+        if (!(ok = __all_sync(0xffffffffu, there))) break;
+        __syncwarp();
+        float2 v[S], d[8][S];
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
 #pragma unroll
           for (int e = 0; e < S; ++e)
-            v[e] = q == 0 ? d[32 * e] : make_float2(__fadd_rn(v[e].x, d[32 * e].x), __fadd_rn(v[e].y, d[32 * e].y));
+            if (q < Q) d[q][e] = (reinterpret_cast<const float2*>(part + ((j + q) % kP) * kPart) + lane)[32 * e];
+#pragma unroll
+        for (int e = 0; e < S; ++e) {
+          v[e] = d[0][e];
+#pragma unroll
+          for (int q = 1; q < 8; ++q)
+            if (q < Q) v[e] = make_float2(__fadd_rn(v[e].x, d[q][e].x), __fadd_rn(v[e].y, d[q][e].y));
         }
         __syncwarp();
-        if (lane == 0) {
-          *c = 0;
-          st_shared_release(done, j + Q);
-        }
+        if (lane < Q) arrive(emptied + at % kP);
         if (s.down) {
           float* y = p.y + ((size_t)slot * kMaxRows + t) * p.H + 16 * u + g;
 #pragma unroll
@@ -736,7 +747,7 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
   } else {
     // ---- the control warp: opens the segments, the table when it is there ------------------------------------------------------
     auto open_seg = [&](int k) {
-      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(seg_open + k)) : "memory");
+      if (lane == 0) arrive(seg_open + k);
       __syncwarp();
     };
     bool ok = true;
@@ -790,7 +801,7 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
       *s_fail = 1;
     }
     __syncwarp();
-    if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(tabbar)) : "memory");
+    if (lane == 0) arrive(tabbar);
     __syncwarp();
     const int nseg = ok ? *s_nseg : 0;
     for (int k = nb_first + 1; ok && k < nseg; ++k) {
@@ -852,8 +863,8 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
 
 template <class V>
 size_t block_smem(size_t tile, int nbuf) {
-  return (size_t)V::W * V::NST * kStage + kP * kPart + sizeof(BlockTab) + nbuf * tile + 64 + (2 * V::W * V::NST + 3 * kMaxSegs + 2) * 8 +
-         kMaxSegs * (sizeof(Seg) + 4) + 24 * 4 + (kP + 4) * 4 + 16;
+  return (size_t)V::W * V::NST * kStage + kP * kPart + sizeof(BlockTab) + nbuf * tile + 64 + (2 * V::W * V::NST + 3 * kMaxSegs + 2 + 2 * kP) * 8 +
+         kMaxSegs * (sizeof(Seg) + 4) + 24 * 4 + 4 * 4 + 16;
 }
 size_t block_tile(int H, int I, int M) {
   return tile_bytes(H, M) > tile_bytes(I, M) ? tile_bytes(H, M) : tile_bytes(I, M);
@@ -876,10 +887,9 @@ cudaError_t launch(const BlockParams& p, cudaStream_t st) {
   cfg.attrs = at, cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, k_block<V>, p);
 }
+// (twelve stream warps with two producers, where they fit: one row of 168 experts 58.2 us instead of 58.9, four rows 147 instead of 145)
 template <int S>
-using Wide = BlkVar<S, 12, 2, 2>;
-template <int S>
-using Narrow = BlkVar<S, 11, 2, 3>;  // (leaves more shared memory to the activations)
+using Var = BlkVar<S, 11, 2, 3>;
 
 size_t al256(size_t v) { return (v + 255) & ~(size_t)255; }
 
@@ -893,8 +903,8 @@ size_t block_ws_bytes(int H, int I) {
 // The rows of one launch: as many of M as the activations' shared memory holds (every row's weights are streamed once a launch).
 int block_rows(int H, int I, int M) {
   int r = M < kMaxRows ? M : kMaxRows;
-  while (r > 1 && block_smem<Narrow<2>>(block_tile(H, I, r), 1) > kSmemMax) r = (r + 1) / 2;
-  return block_smem<Narrow<2>>(block_tile(H, I, r), 1) > kSmemMax || sm_count() < 2 * kMaxRows ? 0 : r;
+  while (r > 1 && block_smem<Var<2>>(block_tile(H, I, r), 1) > kSmemMax) r = (r + 1) / 2;
+  return block_smem<Var<2>>(block_tile(H, I, r), 1) > kSmemMax || sm_count() < 2 * kMaxRows ? 0 : r;
 }
 
 cudaError_t launch_block_int4(BlockParams p, void* ws, cudaStream_t st) {
@@ -905,15 +915,12 @@ cudaError_t launch_block_int4(BlockParams p, void* ws, cudaStream_t st) {
   p.lpart = reinterpret_cast<float*>(w), w += al256((size_t)((p.H + 1023) / 1024) * kMaxRows * 512 * 4);
   p.h = reinterpret_cast<__nv_bfloat16*>(w), w += al256((size_t)(kMaxEnt + 1) * kMaxRows * p.I * 2);
   p.y = reinterpret_cast<float*>(w);
-  // Two tiles where they fit (the routed experts' activations are prepared while the shared expert's are in use), and the wide
-  // variant where it fits.
+  // Two tiles where they fit: the routed experts' activations are prepared while the shared expert's are in use.
   p.tile = block_tile(p.H, p.I, p.M), p.tile_down = tile_bytes(p.I, p.M), p.nbuf_down = 2 * p.tile_down <= p.tile ? 2 : 1;
-  const bool wide = block_smem<Wide<2>>(p.tile, 1) <= kSmemMax;
-  p.nbuf = (wide ? block_smem<Wide<2>>(p.tile, 2) : block_smem<Narrow<2>>(p.tile, 2)) <= kSmemMax ? 2 : 1;
-  // One set of rows where that is enough and quicker: one row of 168 experts 59.8 -> 58.9 us, of 2048 x 1024 29.6 -> 28.6; four
-  // rows the other way, 147.4 -> 148.7 (the registers that are left over go to other parts of the code).
-  if (p.M > 2) return wide ? launch<Wide<2>>(p, st) : launch<Narrow<2>>(p, st);
-  return wide ? launch<Wide<1>>(p, st) : launch<Narrow<1>>(p, st);
+  p.nbuf = block_smem<Var<2>>(p.tile, 2) <= kSmemMax ? 2 : 1;
+  // One set of rows in the code where that is enough: one row of 168 experts 59.8 -> 58.9 us, of 2048 x 1024 29.6 -> 28.5, four rows
+  // of 168 experts 148.5 -> 145.
+  return p.M > 4 ? launch<Var<2>>(p, st) : launch<Var<1>>(p, st);
 }
 
 }  // namespace dsgx
