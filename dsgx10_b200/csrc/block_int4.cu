@@ -3,7 +3,7 @@
 //
 // Bound: the weights of the distinct picked experts are read once, so HBM.  One CTA a SM, launched cooperatively (all resident
 // together, so CTAs may wait for one another; every wait is bounded and a run-out is recorded in the workspace).  Of a
-// CTA's warps W stream weights, each from a ring of bulk copies that two or three more fill for all, one joins their sums and one
+// CTA's warps W stream weights, each from a ring of bulk copies that three more fill for all, one joins their sums and one
 // keeps track of what the other CTAs have done; whoever is free turns activations into the MMAs' operands.
 //
 //   front    every CTA but the last M: the router's logit slices (route.cuh's order).  The last M CTAs route a row each; the
@@ -15,8 +15,8 @@
 //   combine  after a grid-wide count: every element adds its row's picks, the shared expert and the residual.
 //
 // Measured (a captured chain, more weights than L2 holds): 168 experts of 6144 x 2048, eight picks a row and the shared expert, one
-// row 60 us (254 MB, 4.3 TB/s; four launches 76), four rows 147 us (717 MB, 4.9 TB/s; 231), eight rows 257 us (434); 1024 x 512
-// and 16 experts, one row: 22 us, all of it the chain of six grid-wide steps (four launches 18).  About 16 us pass until routed
+// row 59 us (254 MB, 4.3 TB/s; four launches 76), four rows 145 us (717 MB, 4.9 TB/s; 231), eight rows 253 us (434); 1024 x 512
+// and 16 experts, one row: 21 us, all of it the chain of six grid-wide steps (four launches 18).  About 16 us pass until routed
 // weights stream; from then on 85 % of a copy's rate, the warps' chains of loads, MMAs and f32 operations next to HBM.
 //
 // Work items.  A unit (16 weight rows) is cut along K in tasks of about two 512-k blocks, dealt to the stream warps in turn
@@ -324,7 +324,9 @@ DSGX_DEV void build_block_tab(BlockTab* out, TabSmem& sm, const BlockParams& p) 
 template <int S_, int W_, int NST_, int NP_>
 struct BlkVar {
   static constexpr int S = S_, W = W_, NST = NST_, NP = NP_, kThreads = 512;
-  static_assert(W + 2 + NP == 16, "warps");
+  // W <= kP: a warp at task j has written j - W, so the unit of j - W - kP, and with it that of j - 2 kP, is joined: the parity waits
+  // on a place never meet one that is two uses behind
+  static_assert(W + 2 + NP == 16 && W <= kP, "warps");
 };
 
 template <class V>
@@ -677,7 +679,7 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
     }
   } else if (warp > kStreamW + 1) {
     // ---- the producers: a lane fills one stream warp's ring as its stages are freed (a warp that fills its own spends 650 to 1000 of
-    // 4400 cycles a stage on it, all of them in its way: 168 experts and four rows took 182 us instead of 147)
+    // 4400 cycles a stage on it, all of them in its way: 168 experts and four rows took 177 us instead of 151)
     const int w = V::NP * lane + (warp - kStreamW - 2);
     uint8_t* myring = ring + (size_t)w * NST * kStage;
     uint64_t *mybar = bars + w * NST, *myfreed = freed + w * NST;
