@@ -49,9 +49,6 @@ DSGX_DEV int ld_shared_acquire(const int* p) {
 DSGX_DEV void st_shared_release(int* p, int v) {
   asm volatile("st.release.cta.shared::cta.s32 [%0], %1;" ::"r"(smem_u32(p)), "r"(v) : "memory");
 }
-DSGX_DEV void red_shared_release(int* p, int v) {  // (cumulative: after a __syncwarp the whole warp's writes are released)
-  asm volatile("red.release.cta.shared::cta.add.s32 [%0], %1;" ::"r"(smem_u32(p)), "r"(v) : "memory");
-}
 // bounded wait until a word of shared memory has reached v
 DSGX_DEV bool wait_shared_ge(const int* p, int v, unsigned sleep_ns) {
   if (ld_shared_acquire(p) >= v) return true;

@@ -249,3 +249,36 @@ def test_refusals():
     assert moe.ws_status(b16.ws) == _lib.ERR_FORMAT
     y, tol = _ffn(x.double(), _shared(layer))
     assert bool(((out.double() - y).abs() <= tol + 2.0 ** -8 * y.abs() + 2.0 ** -20 * y.abs()).all())
+
+
+def test_layers_and_products_at_once():
+    """Layers on one stream while dense products of all divisions (clusters, pairs of them, one CTA) run on two others."""
+    from dsgx10_b200 import linear, moe, synth
+    shp, layer, wr = _setup(1024, 512, 16, 4, 190)
+    blocks, lw = [moe.MoeBlock(shp, wr) for _ in range(2)], layer.layer_w()
+    xs = [synth.activations(m, 1024, 191 + m).cuda() for m in (1, 5, 8, 13)]
+    ws = []
+    for M, N, K in ((1, 4096, 2048), (16, 1000, 9000), (8, 512, 6144), (3, 131, 300)):
+        n = -(-N // 8) * -(-K // 512)
+        b = torch.randint(0, 256, (n, 2368), dtype=torch.uint8, device="cuda")
+        b[:, 2048:2304].view(n, 128, 2)[:, :, 1] = 0x3B
+        ws.append((linear.LinearW(N, K, b.view(-1)), synth.activations(M, K, 200 + M).cuda()))
+    want = [blocks[0].run(lw, x)[0].clone() for x in xs], [linear.linear_decode(w, x) for w, x in ws]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = [], [], []
+    for i in range(12):
+        with torch.cuda.stream(streams[0]):
+            got[0].append(blocks[0].run(lw, xs[i % 4])[0])
+        for k in (1, 2):
+            with torch.cuda.stream(streams[k]):
+                got[k].append([linear.linear_decode(w, x) for w, x in ws])
+                if k == 2:
+                    got[k][-1].append(blocks[1].run(lw, xs[(i + 1) % 4])[0])
+    torch.cuda.synchronize()
+    assert all(moe.ws_status(b.ws) == 0 for b in blocks)
+    assert all(torch.equal(y, want[0][i % 4]) for i, y in enumerate(got[0]))
+    for k in (1, 2):
+        for i, ys in enumerate(got[k]):
+            assert all(torch.equal(a, b) for a, b in zip(ys[:4], want[1]))
+            assert k == 1 or torch.equal(ys[4], want[0][(i + 1) % 4])
