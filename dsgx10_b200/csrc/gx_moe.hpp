@@ -114,7 +114,7 @@ inline void moe_block_decode(const MoeShape& s, const LayerW& L, const __nv_bflo
                              const __nv_bfloat16* res, __nv_bfloat16* out, cudaStream_t st) {
   check(dsgx_moe_block_decode(&s, &L, x, M, &block, res, out, st), "gx::moe_block_decode");
 }
-// dense products with 4-bit weights (engine/attn/attn.h glm::gemv): prepared once at load, then x W^T (+ res), or silu(x W^T) * (x Wup^T)
+// dense products with 4-bit weights (the engines' engine/attn/attn.h): prepared once at load, then x W^T (+ res), or silu(x W^T) * (x Wup^T)
 using LinearW = dsgx_linear_w;
 inline size_t linear_bytes(int N, int K, bool glu = false) { return dsgx_linear_bytes(N, K, glu ? 1 : 0); }
 inline LinearW linear_prepare(const void* blocks, const void* up_blocks, int N, int K, void* out, cudaStream_t st) {

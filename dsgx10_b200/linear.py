@@ -1,6 +1,6 @@
 """Dense products with 4-bit weights for 1..16 rows over the C ABI (dsgx_linear_decode), torch tensors as device memory.
 
-The engines' weight-streaming GEMV over INT4 matrices (altar1 engine/attn/attn.h glm::gemv): projections, dense FFN layers and
+The engines' products with INT4 matrices outside the experts (altar1 engine/attn/attn.h): projections, dense FFN layers and
 heads, next to the experts of moe.py.
 
     w = linear.LinearW(N, K, torch.from_numpy(weights.pack_linear_int4(codes, scales, zeros)).cuda())

@@ -340,8 +340,8 @@ int dsgx_moe_block_decode(const dsgx_moe_shape* shape, const dsgx_layer_w* L, co
 
 /* ---- dense products with 4-bit weights (1..DSGX_MAX_STEP_ROWS rows) ---------------------------------------------------
  * out[m][n] = sum_k x[m][k] W[n][k], W[n][k] = (u - z) s of an INT4-g32 matrix: the projections, dense FFN layers and heads of
- * a model whose experts this library runs; stands in for the engines' weight-streaming GEMV over INT4 weights (altar1
- * engine/attn/attn.h glm::gemv).  W is not rounded: the scale is applied to a group's f32 sum (the expert kernels' contract
+ * a model whose experts this library runs; stands in for the engines' products with INT4 matrices outside the experts
+ * (altar1 engine/attn/attn.h).  W is not rounded: the scale is applied to a group's f32 sum (the expert kernels' contract
  * rounds every weight to bf16).
  *
  * dsgx_linear_prepare re-tiles a matrix once at load, from the experts' blocks (DSGX_FMT_INT4: 8 rows x 512 k,
