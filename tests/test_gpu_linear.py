@@ -236,3 +236,41 @@ def test_prepare_then_product():
         got = linear.linear_decode(w, x)
         del w
         assert torch.equal(got, want[i % 2]), i
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 10, 250000), (6, 40, 60000), (16, 17, 100001)])
+def test_long_rows(M, N, K):
+    """K over all of a cluster's shared memory, and past it: the rows then go in several launches."""
+    from dsgx10_b200 import linear
+    blocks, w, wb = _make(N, K, 301)
+    x = _x(M, K, 302)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    lw = linear.LinearW(N, K, blocks)
+    got = linear.linear_decode(lw, x.cuda(), out_dtype=torch.float32, status=status)
+    assert int(status) == 0
+    _check(got, x.double() @ w.T, x.double().abs() @ wb.T, K)
+    assert torch.equal(got[-1:], linear.linear_decode(lw, x[-1:].cuda(), out_dtype=torch.float32))
+
+
+def test_too_long_rows_are_refused():
+    from dsgx10_b200 import _lib, linear
+    N, K = 8, 1000000
+    w = linear.LinearW(N, K, torch.zeros(-(-K // 512) * 2368, dtype=torch.uint8, device="cuda"))
+    for M in (1, 3, 16):
+        with pytest.raises(_lib.DsgxError):
+            linear.linear_decode(w, torch.zeros(M, K, dtype=torch.bfloat16, device="cuda"))
+
+
+def test_offsets_past_32_bits():
+    """More than 4 GiB of weights, the same 16 rows over and over: every 16 outputs are the bits of a matrix of 16 rows."""
+    from dsgx10_b200 import linear
+    N, K, M = 1 << 20, 8192, 2
+    small, _, _ = _make(16, K, 311)
+    x = _x(M, K, 312).cuda()
+    want = linear.linear_decode(linear.LinearW(16, K, small), x, out_dtype=torch.float32)
+    blocks = small.repeat(N // 16)
+    w = linear.LinearW(N, K, blocks)
+    assert w.data.numel() > 1 << 32
+    del blocks
+    got = linear.linear_decode(w, x, out_dtype=torch.float32)
+    assert torch.equal(got.view(M, N // 16, 16), want.view(M, 1, 16).expand(M, N // 16, 16))
