@@ -29,8 +29,10 @@
 // both groups' sums of row t and two packed multiply-adds finish 64 k (scale, zero point: int4_mma.cuh).  Four rows of x a
 // set of MMAs; an expert that more rows picked takes two sets.  Only the rows that picked an expert are computed for it.
 //
-// The expert's input rows and h are f16 with a power of two a 512-k block; gate, up and the down sums stay f32; h is rounded to
-// bf16 once, because it is an MMA operand (2^-9 of its value; a second half would double the down products' MMAs).
+// Gate, up and the down sums stay f32, and so does h until it is an MMA operand: f16 with a power of two a 512-k block, as the INT4
+// products take x (eleven bits, at most 2^-11 of the value; h in bf16 made the layer's error against 64 bits 0.0021 of its
+// outputs instead of 0.0017, which the outputs' own rounding is, and took 145.1 us for four rows of 168 experts instead of 146.3,
+// 253 for eight instead of 259).  A bf16 matrix meets it as two bf16 parts whose sum it is (pair_b16).
 #include <atomic>
 #include <cstddef>
 #include <type_traits>
@@ -103,7 +105,8 @@ DSGX_DEV bool poll_near(const int* p, int target) {
   return true;
 }
 
-// g / (1 + e^-g) by the fast exponential and division: within 100 x 2^-23 of the value for |g| up to 80, and h is rounded to bf16 next
+// g / (1 + e^-g) by the fast exponential and division: within 100 x 2^-23 = 2^-16.3 of the value for |g| up to 80, and h's rounding to
+// eleven bits, 2^-11, comes next (expf and an IEEE division in the joining warp: 168 experts, four rows 146.3 -> 147.2 us)
 DSGX_DEV float quick_silu(float g) { return __fdividef(g, 1.f + __expf(-g)); }
 
 // A CTA's run of units of one phase.
@@ -167,19 +170,35 @@ DSGX_DEV void pair_int4(float2 (&acc)[S][2], uint32_t st, const uint32_t (&x_at)
   }
 }
 
-// One bf16 block pair (128 k) on a bf16 tile: all eight columns are rows of x (column n: row n / 2 + 4 (n & 1), so that a lane
-// ends with rows t and t + 4).
-DSGX_DEV void pair_b16(float (&d)[4], uint32_t st, uint32_t x, uint32_t span, int lane) {
+// Two f16 values as two bf16 parts each, hi + lo = the value (eight bits and the three or fewer left)
+DSGX_DEV void split_f16(uint32_t& hi, uint32_t& lo, uint32_t w) {
+  const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(v.y), "f"(v.x));
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(__fadd_rn(v.y, -scale_hi(hi))), "f"(__fadd_rn(v.x, -scale_lo(hi))));
+}
+// One bf16 block pair (128 k) on a bf16 tile, or (f16) on an f16 one with two MMAs for one (twice the tile, split beforehand, would
+// leave no room for its rows): all eight columns are rows of x (column n: row n / 2 + 4 (n & 1), so that a lane ends with rows t
+// and t + 4).
+DSGX_DEV void pair_b16(float (&d)[4], uint32_t st, uint32_t x, uint32_t span, bool f16, int lane) {
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
-    const uint32_t a = st + 1024 * q + 16 * lane;
-    const uint4 a0 = lds_v4(a), a1 = lds_v4(a + 512), b0 = lds_v4(a + kQBlk), b1 = lds_v4(a + kQBlk + 512);
-    const uint4 x0 = lds_v4(x), x1 = lds_v4(x + 16);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const uint32_t a = st + 1024 * q + 512 * c + 16 * lane;
+      const uint4 wa = lds_v4(a), wb = lds_v4(a + kQBlk);
+      uint4 xv = lds_v4(x + 16 * c);
+      const uint32_t r0 = __byte_perm(wa.x, wa.z, 0x5410), r1 = __byte_perm(wb.x, wb.z, 0x5410), r2 = __byte_perm(wa.x, wa.z, 0x7632), r3 = __byte_perm(wb.x, wb.z, 0x7632);
+      const uint32_t r4 = __byte_perm(wa.y, wa.w, 0x5410), r5 = __byte_perm(wb.y, wb.w, 0x5410), r6 = __byte_perm(wa.y, wa.w, 0x7632), r7 = __byte_perm(wb.y, wb.w, 0x7632);
+      if (f16) {
+        uint4 lo;
+        split_f16(xv.x, lo.x, xv.x), split_f16(xv.y, lo.y, xv.y), split_f16(xv.z, lo.z, xv.z), split_f16(xv.w, lo.w, xv.w);
+        mma_bf16(d, r0, r1, r2, r3, lo.x, lo.y);
+        mma_bf16(d, r4, r5, r6, r7, lo.z, lo.w);
+      }
+      mma_bf16(d, r0, r1, r2, r3, xv.x, xv.y);
+      mma_bf16(d, r4, r5, r6, r7, xv.z, xv.w);
+    }
     x += span;
-    mma_bf16(d, __byte_perm(a0.x, a0.z, 0x5410), __byte_perm(b0.x, b0.z, 0x5410), __byte_perm(a0.x, a0.z, 0x7632), __byte_perm(b0.x, b0.z, 0x7632), x0.x, x0.y);
-    mma_bf16(d, __byte_perm(a0.y, a0.w, 0x5410), __byte_perm(b0.y, b0.w, 0x5410), __byte_perm(a0.y, a0.w, 0x7632), __byte_perm(b0.y, b0.w, 0x7632), x0.z, x0.w);
-    mma_bf16(d, __byte_perm(a1.x, a1.z, 0x5410), __byte_perm(b1.x, b1.z, 0x5410), __byte_perm(a1.x, a1.z, 0x7632), __byte_perm(b1.x, b1.z, 0x7632), x1.x, x1.y);
-    mma_bf16(d, __byte_perm(a1.y, a1.w, 0x5410), __byte_perm(b1.y, b1.w, 0x5410), __byte_perm(a1.y, a1.w, 0x7632), __byte_perm(b1.y, b1.w, 0x7632), x1.z, x1.w);
   }
 }
 
@@ -411,7 +430,6 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
     if (!mbar_wait(seg_open + k, 0, 20)) return false;
     const int nb = down ? nbI : nbH, K = down ? p.I : p.H, items = nb * rows;
     const Tile tile(tile_at(k), nb, rows);
-    const __nv_bfloat16* src = down ? p.h + (size_t)slot * kMaxRows * p.I : p.x;
     const uint32_t span = rows * 128;
     for (;;) {
       int i = 0;
@@ -421,8 +439,17 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
       const int b = i / rows, r = i - b * rows;
       uint8_t* xt = tile.x + (size_t)b * 8 * span + r * 128;
       uint32_t w[8];
-      load_16<true>(w, src + (size_t)r * K, b * 512 + 16 * lane, K, true);
-      if (b16) {
+      if (!down) load_16<true>(w, p.x + (size_t)r * K, b * 512 + 16 * lane, K, true);
+      if (down) {
+        const float4* src = reinterpret_cast<const float4*>(p.h + ((size_t)slot * kMaxRows + r) * K + b * 512 + 16 * lane);
+        float2 v[8];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float4 u = __ldcg(src + c);
+          v[2 * c] = make_float2(u.x, u.y), v[2 * c + 1] = make_float2(u.z, u.w);
+        }
+        stage_row_f32(v, !b16, xt, span, tile.sum + (size_t)b * 16 * rows + 2 * r, rows * 8, tile.scale + b * rows + r, lane);
+      } else if (b16) {
         uint4 o[2];
         nibble_order(o, w);
         uint4* d = reinterpret_cast<uint4*>(xt + (size_t)(lane >> 2) * span + (lane & 3) * 32);
@@ -526,6 +553,8 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
         auto row = [&](int j) { return (int)(rows >> (8 * min(j, n - 1)) & 0xff); };
         if (s.b16) {
           xr[0] = x0 + row((g >> 1) + 4 * (g & 1)) * 128 + t * 32;
+#pragma unroll
+          for (int e = 0; e < S; ++e) fr[e] = smem_u32(tile.scale) + row(4 * e + t) * 4;
           return;
         }
 #pragma unroll
@@ -559,11 +588,14 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
             for (int q = 0; q < 4; ++q) {
               const uint32_t st = stage_ready();
               if (!ok) break;
-              pair_b16(d, st, xr[0] + (8 * b + 2 * q) * span, span, lane);
+              pair_b16(d, st, xr[0] + (8 * b + 2 * q) * span, span, s.down, lane);
               stage_used();
             }
 #pragma unroll
-            for (int e = 0; e < S; ++e) acc[e][0] = __fadd_rn(acc[e][0], d[e]), acc[e][1] = __fadd_rn(acc[e][1], d[2 + e]);
+            for (int e = 0; e < S; ++e) {
+              const float f = s.down ? lds_f(fr[e] + b * (s.rows * 4)) * 0x1p-12f : 1.f;  // (h: times 2^-E)
+              acc[e][0] = fmaf(d[e], f, acc[e][0]), acc[e][1] = fmaf(d[2 + e], f, acc[e][1]);
+            }
           }
         } else {
           auto run = [&](auto sets) {
@@ -647,21 +679,21 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
             if (4 * e + t < n) y[(size_t)4 * e * p.H] = v[e].x, y[(size_t)4 * e * p.H + 8] = v[e].y;
           continue;
         }
-        __nv_bfloat16* h = p.h + ((size_t)slot * kMaxRows + t) * p.I + 8 * u;
+        float* h = p.h + ((size_t)slot * kMaxRows + t) * p.I + 8 * u;
         if (inter) {
           // interleaved rows: strip rows 2 i and 2 i + 1 are gate and up of a channel (first strip: channels 0-3, second: 4-7)
 #pragma unroll
           for (int e = 0; e < S; ++e) {
             const float ua = __shfl_down_sync(0xffffffffu, v[e].x, 4), ub = __shfl_down_sync(0xffffffffu, v[e].y, 4);
             if (!(g & 1) && 4 * e + t < n) {
-              h[(size_t)4 * e * p.I + (g >> 1)] = __float2bfloat16_rn(__fmul_rn(quick_silu(v[e].x), ua));
-              h[(size_t)4 * e * p.I + 4 + (g >> 1)] = __float2bfloat16_rn(__fmul_rn(quick_silu(v[e].y), ub));
+              h[(size_t)4 * e * p.I + (g >> 1)] = __fmul_rn(quick_silu(v[e].x), ua);
+              h[(size_t)4 * e * p.I + 4 + (g >> 1)] = __fmul_rn(quick_silu(v[e].y), ub);
             }
           }
         } else {
 #pragma unroll
           for (int e = 0; e < S; ++e)
-            if (4 * e + t < n) h[(size_t)4 * e * p.I + g] = __float2bfloat16_rn(__fmul_rn(quick_silu(v[e].x), v[e].y));
+            if (4 * e + t < n) h[(size_t)4 * e * p.I + g] = __fmul_rn(quick_silu(v[e].x), v[e].y);
         }
         // the run's units of a slot are reported together: h is read when all of the slot's are there
         if (i + 1 == s.n || (s.slot != kShared && u + 1 == upp)) {
@@ -899,7 +931,7 @@ size_t al256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 size_t block_ws_bytes(int H, int I) {
   return 256 + al256(sizeof(BlockSync)) + al256(sizeof(BlockTab)) + al256((size_t)((H + 1023) / 1024) * kMaxRows * 512 * 4) +
-         al256((size_t)(kMaxEnt + 1) * kMaxRows * I * 2) + al256((size_t)(kMaxEnt + 1) * kMaxRows * H * 4);
+         al256((size_t)(kMaxEnt + 1) * kMaxRows * I * 4) + al256((size_t)(kMaxEnt + 1) * kMaxRows * H * 4);
 }
 
 // The rows of one launch: as many of M as the activations' shared memory holds (every row's weights are streamed once a launch).
@@ -915,7 +947,7 @@ cudaError_t launch_block_int4(BlockParams p, void* ws, cudaStream_t st) {
   p.sync = reinterpret_cast<BlockSync*>(w), w += al256(sizeof(BlockSync));
   p.tab = reinterpret_cast<BlockTab*>(w), w += al256(sizeof(BlockTab));
   p.lpart = reinterpret_cast<float*>(w), w += al256((size_t)((p.H + 1023) / 1024) * kMaxRows * 512 * 4);
-  p.h = reinterpret_cast<__nv_bfloat16*>(w), w += al256((size_t)(kMaxEnt + 1) * kMaxRows * p.I * 2);
+  p.h = reinterpret_cast<float*>(w), w += al256((size_t)(kMaxEnt + 1) * kMaxRows * p.I * 4);
   p.y = reinterpret_cast<float*>(w);
   // Two tiles where they fit: the routed experts' activations are prepared while the shared expert's are in use.
   p.tile = block_tile(p.H, p.I, p.M), p.tile_down = tile_bytes(p.I, p.M), p.nbuf_down = 2 * p.tile_down <= p.tile ? 2 : 1;

@@ -178,4 +178,45 @@ DSGX_DEV void stage_row(const uint32_t (&w)[8], uint8_t* xt, uint32_t span, bool
   if (lane == 0) *scale = __uint_as_float((uint32_t)(12 - E + 127) << 23);
 }
 
+// The same for 16 f32 values (k = 2 i, 2 i + 1 in v[i]) that are to become a product's f16 operands: 2^E as above, then one
+// rounding to f16's eleven bits (absolute from 2^-28 of the block's largest on, 2^-24 at odd k with `nib`), and the groups' sums
+// are those of the rounded values.  nib: the weights are nibbles (odd k times 2^-4).
+DSGX_DEV void stage_row_f32(float2 (&v)[8], bool nib, uint8_t* xt, uint32_t span, float* sx, uint32_t sspan, float* scale, int lane) {
+  auto mag = [](float a) { return __float_as_uint(a) & 0x7FFFFFFFu; };
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, max(mag(v[i].x), mag(v[i].y)));
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (top >= 0x7F800000u) {  // an infinity or a NaN: the largest finite one
+    top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t a = mag(v[i].x), b = mag(v[i].y);
+      top = max(top, max(a < 0x7F800000u ? a : 0u, b < 0x7F800000u ? b : 0u));
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+  }
+  const int E = top >= 0x800000u ? min(14 + 127 - (int)(top >> 23), 126) : 126;
+  const float2 f = make_float2(__uint_as_float((uint32_t)(E + 127) << 23), __uint_as_float((uint32_t)(E - (nib ? 4 : 0) + 127) << 23));
+  uint32_t h[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    v[i] = mul2(v[i], f);
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h[i]) : "f"(v[i].y), "f"(v[i].x));
+    v[i] = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+  }
+#pragma unroll
+  for (int n = 4; n > 0; n >>= 1)
+#pragma unroll
+    for (int i = 0; i < n; ++i) v[i] = add2(v[i], v[i + n]);
+  float sum = fmaf(v[0].y, 16.f, v[0].x);
+  sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, 1));
+  uint4 o[2];
+  nibble_order(o, h);
+  uint4* d = reinterpret_cast<uint4*>(xt + (size_t)(lane >> 2) * span + (lane & 3) * 32);
+  d[0] = o[0], d[1] = o[1];
+  if (!(lane & 1)) *reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(sx) + (size_t)(lane >> 2) * sspan + 4 * (lane >> 1 & 1)) = sum * 0x1p-24f;
+  if (lane == 0) *scale = __uint_as_float((uint32_t)(12 - E + 127) << 23);
+}
+
 }  // namespace dsgx

@@ -184,7 +184,7 @@ struct BlockParams {
   BlockSync* sync;
   BlockTab* tab;
   float* lpart;        // [H / 1024 slices][8][E] partial router logits
-  __nv_bfloat16* h;    // [64 + 1 slots][8][I]
+  float* h;            // [64 + 1 slots][8][I]
   float* y;            // [64 + 1 slots][8][H]
   size_t tile, tile_down;  // bytes of an activation tile in shared memory; of one of a down segment
   int nbuf, nbuf_down;     // tiles of x; tiles of h in the first one's place

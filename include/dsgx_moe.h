@@ -315,9 +315,10 @@ int dsgx_moe_layer_decode_host(const dsgx_moe_shape* shape, const dsgx_layer_w* 
  * dsgx_moe_layer_decode runs the same layer as four launches with f32 partial sums for other GPUs; this call is the whole
  * layer on one GPU (e_lo = 0, e_hi = E; otherwise DSGX_ERR_UNSUPPORTED).
  *   idx, w: the picks, bit for bit dsgx_route's of dsgx_router_logits.
- *   The experts: W = (u - z) s unrounded, gate, up and the down sums in f32, h = bf16(silu(g) u), out_r = sum of w_e y_e in
- *   ascending expert id, then the shared expert, then the residual, one rounding.  (The four launches round W, g and u to bf16 as
- *   altar-1 does, so the two agree within those roundings, not bit for bit.)
+ *   The experts: W = (u - z) s unrounded, gate, up and the down sums in f32, h = silu(g) u in f32, rounded to eleven bits as the
+ *   down products' operand (f16 with a power of two a row and 512 channels), out_r = sum of w_e y_e in ascending expert id,
+ *   then the shared expert, then the residual, one rounding.  (The four launches round W, g, u and h to bf16 as altar-1 does, so
+ *   the two agree within those roundings, not bit for bit.)
  * A row's bits depend neither on the other rows nor on their number, and are the same run after run.  Only the rows that
  * picked an expert are computed for it.  Up to eight rows are one launch (fewer where H or I is so large that their
  * activations do not fit shared memory: 8192 and eight rows take two), more follow in stream order.
