@@ -407,6 +407,17 @@ int dsgx_moe_layer_decode_host(const dsgx_moe_shape* s, const dsgx_layer_w* L, c
   return e == cudaSuccess ? DSGX_OK : cuda_fail(e);
 }
 
+// Whether any of M rows at a (wa bytes each, la apart) shares a byte with any of M rows at b.  (Rows may lie between one another,
+// as columns of one tensor do.)
+static bool rows_meet(const void* a, size_t wa, size_t la, const void* b, size_t wb, size_t lb, int M) {
+  const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)b;
+  if (a0 + (M - 1) * la + wa <= b0 || b0 + (M - 1) * lb + wb <= a0) return false;
+  for (int i = 0; i < M; ++i)
+    for (int j = 0; j < M; ++j)
+      if (a0 + i * la < b0 + j * lb + wb && b0 + j * lb < a0 + i * la + wa) return true;
+  return false;
+}
+
 static int check_block_shape(const dsgx_moe_shape* s) {
   const int rc = check_shape(s);
   if (rc) return rc;
@@ -430,6 +441,8 @@ int dsgx_moe_block_decode(const dsgx_moe_shape* s, const dsgx_layer_w* L, const 
   if (((uintptr_t)x | (uintptr_t)b->wr | (uintptr_t)L->desc | (uintptr_t)L->sh.bg | (uintptr_t)L->sh.bu | (uintptr_t)L->sh.bd | (uintptr_t)L->sh.bgu) & 15)
     return DSGX_ERR_ARG;
   if ((((uintptr_t)res | (uintptr_t)out) & 7) || (((uintptr_t)b->bias | (uintptr_t)b->idx | (uintptr_t)b->w) & 3)) return DSGX_ERR_ARG;
+  const size_t row = (size_t)s->H * 2;  // (out is x or res, row on row, or shares nothing with them)
+  if ((out != x && rows_meet(out, row, row, x, row, row, M)) || (res && out != res && rows_meet(out, row, row, res, row, row, M))) return DSGX_ERR_ARG;
   BlockParams p{};
   p.H = s->H, p.I = s->I, p.E = s->E, p.topk = s->topk, p.b16 = s->fmt == DSGX_FMT_BF16, p.fmt = s->fmt;
   p.pool = L->pool, p.desc = L->desc, p.sh_g = L->sh.bg, p.sh_u = L->sh.bu, p.sh_d = L->sh.bd, p.sh_bgu = L->sh.bgu;
@@ -473,7 +486,11 @@ int dsgx_linear_decode(const dsgx_linear_w* W, const void* x, int64_t ldx, int M
   if (res && W->glu) return DSGX_ERR_UNSUPPORTED;
   if (((uintptr_t)W->w & 15) || ((uintptr_t)x | (uintptr_t)res) & 1 || (uintptr_t)out & (out_f32 ? 3 : 1) || (uintptr_t)status_word & 3)
     return DSGX_ERR_ARG;
-  if (out == x) return DSGX_ERR_ARG;  // (rows of x are read until the end)
+  // rows of x are read until the end, a residual by the thread that writes its output only
+  const size_t ob = out_f32 ? 4 : 2;
+  if (rows_meet(out, W->N * ob, ldo * ob, x, (size_t)W->K * 2, ldx * 2, M)) return DSGX_ERR_ARG;
+  const bool in_place = out == res && !out_f32 && (M == 1 || ldo == ldr);
+  if (res && !in_place && rows_meet(out, W->N * ob, ldo * ob, res, (size_t)W->N * 2, ldr * 2, M)) return DSGX_ERR_ARG;
   LinearParams p;
   p.w = W->w, p.glu = W->glu != 0, p.x = reinterpret_cast<const __nv_bfloat16*>(x), p.res = reinterpret_cast<const __nv_bfloat16*>(res);
   p.out = out, p.ldx = ldx, p.ldr = ldr, p.ldo = ldo, p.M = M, p.N = W->N, p.K = W->K;

@@ -52,7 +52,8 @@ def _lead(t, M, width, what, device):
 
 def linear_decode(w, x, res=None, out=None, out_dtype=torch.bfloat16, status=None):
     """x bf16 [M][K], M = 1..16 -> out [M][N] (bf16 or f32): x W^T (+ res bf16 [M][N]), or silu(x W^T) * (x Wup^T) where w has
-    an `up` matrix.  x, res and out may be rows of larger tensors (last dimension contiguous); out may be res, not x.
+    an `up` matrix.  x, res and out may be rows of larger tensors (last dimension contiguous); out may be res (bf16, the same rows), and
+    shares no memory with x or res otherwise.
     status: an int32 device tensor that gets DSGX_ERR_DEVICE_WAIT where a bounded wait ran out."""
     dev, bf16 = w.device, torch.bfloat16
     if x.dtype is not bf16 or (res is not None and res.dtype is not bf16):

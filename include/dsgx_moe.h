@@ -322,7 +322,7 @@ int dsgx_moe_layer_decode_host(const dsgx_moe_shape* shape, const dsgx_layer_w* 
  * A row's bits depend neither on the other rows nor on their number, and are the same run after run.  Only the rows that
  * picked an expert are computed for it.  Up to eight rows are one launch (fewer where H or I is so large that their
  * activations do not fit shared memory: 8192 and eight rows take two), more follow in stream order.
- * x, res (may be null), out: bf16 [M][H]; out may be x or res.  ws: dsgx_moe_block_ws_bytes(shape) bytes, zeroed once; the
+ * x, res (may be null), out: bf16 [M][H]; out may be x or res, and shares no bytes with them otherwise (DSGX_ERR_ARG).  ws: dsgx_moe_block_ws_bytes(shape) bytes, zeroed once; the
  * kernel leaves its counters at zero.  Its first word is the status (dsgx_ws_status): a descriptor of another format gives
  * DSGX_ERR_FORMAT and leaves the routed experts out; a bounded wait that ran out gives DSGX_ERR_DEVICE_WAIT and no output.
  * The CTAs (one a SM) wait for one another, so the launch is cooperative: it starts when all of them fit, and it can be
@@ -355,10 +355,11 @@ size_t dsgx_linear_bytes(int N, int K, int glu);
 int dsgx_linear_prepare(const void* w, const void* w_up, uint32_t fmt, int N, int K, void* out, void* stream);
 
 /* The product.  glu: out = silu(x W^T) * (x W_up^T) (a dense layer's gate and up in one launch), one rounding.
- * res set (not with glu): res[m][n] (bf16) is added to the f32 sum; out may be res.
+ * res set (not with glu): res[m][n] (bf16) is added to the f32 sum; out may be res where it is bf16 with the same leading dimension.
  * x bf16 [M][ldx], res bf16 [M][ldr], out [M][ldo] bf16, or f32 with out_f32; leading dimensions in elements, any values >= K
- * or N, rows need no alignment beyond their type's (16-byte aligned rows of x are read faster).  out must not overlap x
- * (out = x is refused) or the weights.  A row's bits depend neither on the other rows of the call nor on their number, and are the same run
+ * or N, rows need no alignment beyond their type's (16-byte aligned rows of x are read faster).  Rows of out that share
+ * bytes with rows of x, or with rows of res in any other way, are refused (DSGX_ERR_ARG; columns of one tensor share none); out must not
+ * overlap the weights.  A row's bits depend neither on the other rows of the call nor on their number, and are the same run
  * after run.  No workspace; asynchronous, graph capturable; calls on several streams may overlap.  The weights must be
  * complete before the launch in front of this one in the stream starts (they are requested early: programmatic dependent
  * launch).  status_word (device, may be null) gets DSGX_ERR_DEVICE_WAIT where a bounded wait ran out.
