@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
     uint32_t issued = 0;
     int pj = w, place = w, pb = 0, pe = 0;  // the task and its next and last block
     const uint8_t* pa = nullptr;
-    bool more = w < W;
+    bool more = w < W, begun = false;
     long long t0 = clock64();
     for (;;) {
       while (more && pb == pe) {  // the next task with a block in it (K shorter than eight blocks: some runs are empty)
@@ -298,6 +298,9 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
       }
       if (__any_sync(0xffffffffu, go)) {
         t0 = clock64();
+      } else if (!begun) {  // the rings are full: the time that the launches in front take is not this launch's
+        pdl_wait();
+        begun = true, t0 = clock64();
       } else {
         if (*reinterpret_cast<volatile int*>(fail) || clock64() - t0 > kWaitCycles) break;
         __nanosleep(20);
