@@ -19,7 +19,9 @@ from .moe import raw_stream
 
 class LinearW:
     """An INT4-g32 matrix [N][K], or a gate / up pair, prepared for linear_decode from the experts' blocks of 8 rows x 512 k on
-    the device (weights.pack_linear_int4).  The prepared copy is made once, on the current stream; the blocks are not kept."""
+    the device (weights.pack_linear_int4).  The prepared copy is made once, on the current stream; the blocks are not kept.
+    status: an int32 word on the device, 0 until a bounded wait of one of its products runs out (DSGX_ERR_DEVICE_WAIT; that product's
+    outputs are undefined); it stays until it is cleared."""
 
     def __init__(self, N, K, blocks, up=None):
         if N < 1 or K < 1:
@@ -33,10 +35,11 @@ class LinearW:
         self.N, self.K, self.glu, self.device = N, K, up is not None, blocks.device
         with torch.cuda.device(self.device):
             self.data = torch.empty(lib().dsgx_linear_bytes(N, K, int(self.glu)), dtype=torch.uint8, device=self.device)
+            self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
             check(lib().dsgx_linear_prepare(blocks.data_ptr(), up.data_ptr() if self.glu else None, _lib.FMT_INT4, N, K, self.data.data_ptr(),
                                             torch.cuda.current_stream(self.device).cuda_stream), "dsgx_linear_prepare")
         self.c = _lib.LinearW(self.data.data_ptr(), N, K, _lib.FMT_INT4, int(self.glu))
-        self.ref = C.byref(self.c)
+        self.ref, self.status_ptr = C.byref(self.c), self.status.data_ptr()
 
 
 def _lead(t, M, width, what, device):
@@ -54,7 +57,7 @@ def linear_decode(w, x, res=None, out=None, out_dtype=torch.bfloat16, status=Non
     """x bf16 [M][K], M = 1..16 -> out [M][N] (bf16 or f32): x W^T (+ res bf16 [M][N]), or silu(x W^T) * (x Wup^T) where w has
     an `up` matrix.  x, res and out may be rows of larger tensors (last dimension contiguous); out may be res (bf16, the same rows), and
     shares no memory with x or res otherwise.
-    status: an int32 device tensor that gets DSGX_ERR_DEVICE_WAIT where a bounded wait ran out."""
+    status: an int32 device tensor that gets DSGX_ERR_DEVICE_WAIT where a bounded wait ran out (default: w.status)."""
     dev, bf16 = w.device, torch.bfloat16
     if x.dtype is not bf16 or (res is not None and res.dtype is not bf16):
         raise ValueError(f"linear_decode: x {x.dtype}, res {None if res is None else res.dtype}; wanted bf16")
@@ -72,7 +75,7 @@ def linear_decode(w, x, res=None, out=None, out_dtype=torch.bfloat16, status=Non
     if status is not None and (status.dtype != torch.int32 or status.device != dev or status.numel() < 1):
         raise ValueError("linear_decode: status is an int32 tensor on the weights' device")
     args = (w.ref, x.data_ptr(), ldx, M, resp, ldr, out.data_ptr(), ldo, 0 if out.dtype is bf16 else 1,
-            None if status is None else status.data_ptr())
+            w.status_ptr if status is None else status.data_ptr())
     if torch.cuda.current_device() == dev.index:
         rc = _decode()(*args, raw_stream(dev.index))
     else:
