@@ -183,7 +183,9 @@ raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: 
 
 
 class MoeBlock:
-    """A whole INT4 or BF16 layer for 1..16 rows in one launch (dsgx_moe_block_decode): out = res + MoE(x)."""
+    """A whole INT4 or BF16 layer for 1..16 rows (dsgx_moe_block_decode): out = res + MoE(x), up to eight rows a launch.
+    ws_status(block.ws) is 0 until a descriptor of another format is met or a bounded wait runs out, and stays until the caller
+    clears it: read it where an output must not be trusted blindly."""
 
     def __init__(self, shp, wr, bias=None, device="cuda"):
         n = lib().dsgx_moe_block_ws_bytes(C.byref(shp))
