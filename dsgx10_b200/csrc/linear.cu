@@ -488,7 +488,8 @@ int device_index() {
   int dev = 0;
   return cudaGetDevice(&dev) == cudaSuccess ? dev & 63 : 0;
 }
-// clusters of C CTAs that the device runs at once (asked once per kernel, device and C; the shared memory is given at its most)
+// clusters of C CTAs that the device runs at once, 0: none of that size (asked once per kernel, device and C; the shared memory is given
+// at its most)
 template <class V>
 cudaError_t resident_clusters(int C, int* n) {
   static std::atomic<int> known[64][kMaxCluster + 1];
@@ -511,12 +512,10 @@ cudaError_t resident_clusters(int C, int* n) {
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = C, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
     cfg.attrs = at, cfg.numAttrs = 1;
-    cudaError_t e = cudaOccupancyMaxActiveClusters(&v, k_linear_int4<V>, &cfg);
-    if (e != cudaSuccess) return e;
-    if (v < 1) return cudaErrorInvalidConfiguration;
-    known[dev][C].store(v);
+    if (cudaOccupancyMaxActiveClusters(&v, k_linear_int4<V>, &cfg) != cudaSuccess) (void)cudaGetLastError(), v = 0;
+    else known[dev][C].store(v > 0 ? v : v = -1);
   }
-  *n = v;
+  *n = v > 0 ? v : 0;
   return cudaSuccess;
 }
 
@@ -537,6 +536,7 @@ cudaError_t divide(const LinearParams& p, Division* best, bool* mine) {
     int n = 0;
     cudaError_t e = resident_clusters<V>(C, &n);
     if (e != cudaSuccess) return e;
+    if (n < 1) continue;  // (the other sizes still serve)
     n = n / pair > 0 ? n / pair : 1;
     const long long cost = (long long)((p.units + n - 1) / n) * kb * (V::W > 11 ? 20 : 22) * (C > 1 ? 5 : 4);
     if (!best->C || cost < best->cost) *best = Division{cost, C, n}, *mine = true;
