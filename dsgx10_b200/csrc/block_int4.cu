@@ -800,6 +800,7 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_block(const BlockParams p) {
     int got = 0;
     if (lane == 0) got = ok && !*s_fail && poll_near(&sy->tab_ready, 1);
     ok = __shfl_sync(0xffffffffu, got, 0) != 0;
+    __syncwarp();  // (a shuffle orders no memory: what lane 0 has acquired is the other lanes' from here on)
     if (ok) {
       const int n16 = (int)(offsetof(BlockTab, ent) + min(p.M * p.topk, kMaxEnt) * sizeof(BlockEnt)) / 16;
       for (int i0 = lane; i0 < n16; i0 += 128) {
