@@ -8,8 +8,9 @@
 // point meet a group's f32 sum, s (sum u x - z sum x), so W itself is never rounded.
 //
 // x goes to f16 for that.  Per row and block of 512 k a power of two 2^E brings the largest magnitude into [2^14, 2^15), where
-// bf16's eight bits are exact down to 2^-32 of it (smaller values round at 2^-40 of the largest, far below an f32 sum's last
-// bit); values that meet a nibble in bits 4-7 are taken times 2^-4.  Whatever is infinite or NaN in a row makes the whole row NaN.
+// bf16's eight bits are exact down to 2^-31 of it and smaller values round by at most 2^-39 of the largest.  Values at odd k meet
+// a nibble in bits 4-7 and are taken times 2^-4: for them it is 2^-27 and 2^-35, still below an f32 sum's last bit.  Whatever is
+// infinite or NaN in a row makes the whole row NaN.
 #pragma once
 #include <cuda_fp16.h>
 
@@ -179,7 +180,7 @@ DSGX_DEV void stage_row(const uint32_t (&w)[8], uint8_t* xt, uint32_t span, bool
 }
 
 // The same for 16 f32 values (k = 2 i, 2 i + 1 in v[i]) that are to become a product's f16 operands: 2^E as above, then one
-// rounding to f16's eleven bits (absolute from 2^-28 of the block's largest on, 2^-24 at odd k with `nib`), and the groups' sums
+// rounding to f16's eleven bits (fewer below 2^-28 of the block's largest, at odd k with `nib` below 2^-24), and the groups' sums
 // are those of the rounded values.  nib: the weights are nibbles (odd k times 2^-4).
 DSGX_DEV void stage_row_f32(float2 (&v)[8], bool nib, uint8_t* xt, uint32_t span, float* sx, uint32_t sspan, float* scale, int lane) {
   auto mag = [](float a) { return __float_as_uint(a) & 0x7FFFFFFFu; };

@@ -47,12 +47,20 @@ def gamma(K, b16):
     return ((64 * 17 + 8 if b16 else 80) + K // 512) * 2.0 ** -23
 
 
+def small(x, bound):
+    """What x loses as an f16 operand of INT4 products: values far below their 512-block's largest round by at most 2^-35 of it."""
+    M, K = x.shape
+    top = x.abs().reshape(M, -1, 512).amax(-1, keepdim=True).expand(M, K // 512, 512).reshape(M, K)
+    return 2.0 ** -35 * (top @ bound.T)
+
+
 def hidden(x, gate, up, b16):
-    """h = silu(g) u and its bound: sums in f32, silu's slope below 1.1, the fast exponential and division within 2^-16."""
+    """h = silu(g) u and its bound: sums in f32, silu's slope below 1.1, the fast exponential and division within 2^-16 for |g| up to
+    80; below -80 silu is less than 80 e^-80 < 2^-108, of which nothing need be left."""
     g, u = x @ gate[0].T, x @ up[0].T
-    dg, du = (gamma(x.shape[1], b16) * (x.abs() @ m[1].T) for m in (gate, up))
+    dg, du = (gamma(x.shape[1], b16) * (x.abs() @ m[1].T) + (0 if b16 else small(x, m[1])) for m in (gate, up))
     act = g * torch.sigmoid(g)
-    return act * u, 1.1 * dg * (u.abs() + du) + act.abs() * du + (act * u).abs() * 2.0 ** -16
+    return act * u, 1.1 * dg * (u.abs() + du) + act.abs() * du + (act * u).abs() * 2.0 ** -16 + 2.0 ** -108 * (u.abs() + du)
 
 
 def as_operand(h, nib):
