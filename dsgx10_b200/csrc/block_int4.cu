@@ -55,7 +55,7 @@ struct alignas(16) BlockEnt {
   int pad[3];
 };
 struct alignas(16) BlockTab {
-  int nslots, bad, npick, pad;
+  int nslots, npick, pad[2];
   int pick[kMaxRows][kMaxTopK];   // a row's picks in ascending expert id: slot | its place among the slot's rows << 8
   float w[kMaxRows][kMaxTopK];
   BlockEnt ent[kMaxEnt];          // (last: only as many as the step can have picked are read)

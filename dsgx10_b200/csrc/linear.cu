@@ -239,8 +239,8 @@ __global__ void __launch_bounds__(V::kThreads, 1) k_linear_int4(const LinearPara
   uint64_t* freed = bars + W * NST;                                    // a stage has been read
   uint64_t* rfull = freed + W * NST;                                    // [kSlotsOwned] every rank's sums are in my buffer
   uint64_t* rfree = rfull + kSlotsOwned;                               // [owner][kSlotsOwned] that owner's buffer may be written
-  int* cnt = reinterpret_cast<int*>(rfree + kMaxCluster * kSlotsOwned);  // [P] block pairs summed of a unit in flight
-  int* done = cnt + P;                                                 // block pairs whose unit has been added up
+  int* cnt = reinterpret_cast<int*>(rfree + kMaxCluster * kSlotsOwned);  // [P] tasks summed of a unit in flight
+  int* done = cnt + P;                                                 // tasks whose unit has been added up
   int* fail = done + 1;                                                // a bounded wait ran out
 
   if (warp < W && lane == 0)
