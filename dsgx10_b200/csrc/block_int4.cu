@@ -314,7 +314,7 @@ DSGX_DEV void build_block_tab(BlockTab* out, TabSmem& sm, const BlockParams& p) 
   for (int j = 0; j < p.topk; ++j) place += sm.idx[row * p.topk + j] < e;
   int bad = bad_id ? DSGX_ERR_ARG : 0;
   if (first) {
-    if (d[0].w != p.fmt || d[1].w != p.fmt || d[2].w != p.fmt) bad = DSGX_ERR_FORMAT;
+    if (d[0].w != p.fmt || d[1].w != p.fmt || d[2].w != p.fmt || ((d[0].x | d[1].x | d[2].x) & 255)) bad = DSGX_ERR_FORMAT;  // (bulk copies fault)
     BlockEnt en;
     en.g = p.pool + ((uint64_t)d[0].x | (uint64_t)d[0].y << 32), en.u = p.pool + ((uint64_t)d[1].x | (uint64_t)d[1].y << 32);
     en.d = p.pool + ((uint64_t)d[2].x | (uint64_t)d[2].y << 32);

@@ -323,8 +323,8 @@ int dsgx_moe_layer_decode_host(const dsgx_moe_shape* shape, const dsgx_layer_w* 
  * picked an expert are computed for it.  Up to eight rows are one launch (fewer where H or I is so large that their
  * activations do not fit shared memory: 8192 and eight rows take two), more follow in stream order.
  * x, res (may be null), out: bf16 [M][H]; out may be x or res, and shares no bytes with them otherwise (DSGX_ERR_ARG).  ws: dsgx_moe_block_ws_bytes(shape) bytes, zeroed once; the
- * kernel leaves its counters at zero.  Its first word is the status (dsgx_ws_status): a descriptor of another format gives
- * DSGX_ERR_FORMAT and leaves the routed experts out; a bounded wait that ran out gives DSGX_ERR_DEVICE_WAIT, and the rows of
+ * kernel leaves its counters at zero.  Its first word is the status (dsgx_ws_status): a picked expert's descriptor of another format
+ * or with an offset that is no multiple of 256 gives DSGX_ERR_FORMAT and leaves the routed experts out; a bounded wait that ran out gives DSGX_ERR_DEVICE_WAIT, and the rows of
  * that launch are undefined (a call of several launches goes on with the next rows).  The word stays until the caller clears it; it
  * is the only sign of either, and the workspace can be used again at once.
  * The CTAs (one a SM) wait for one another, so the launch is cooperative: it starts when all of them fit, and it can be
