@@ -313,14 +313,18 @@ int dsgx_moe_layer_decode_host(const dsgx_moe_shape* shape, const dsgx_layer_w* 
  * out = bf16(res + MoE(x)) of an INT4-g32 or BF16 layer (DSGX_FMT_INT4, DSGX_FMT_BF16; the bf16 shared expert in either form of
  * dsgx_shared_w, or none): router logits, selection, the picked experts, the weighted sum, the residual, in ONE kernel.
  * dsgx_moe_layer_decode runs the same layer as four launches with f32 partial sums for other GPUs; this call is the whole
- * layer on one GPU (e_lo = 0, e_hi = E; otherwise DSGX_ERR_UNSUPPORTED).
+ * layer on one GPU (e_lo = 0, e_hi = E; otherwise DSGX_ERR_UNSUPPORTED).  Which one: of INT4 layers this call was the quicker one from
+ * three rows on, and for one or two rows from about 90 MB of weights a step (the picked experts' and the shared one's) on; below
+ * that the four launches are up to 4 us quicker.  x is the layer's input as it is (a norm in front is the caller's: the one that
+ * dsgx_finalize_add_norm makes of the block before, or dsgx_moe_layer_decode's own).
  *   idx, w: the picks, bit for bit dsgx_route's of dsgx_router_logits.
  *   The experts: W = (u - z) s unrounded, gate, up and the down sums in f32, h = silu(g) u in f32, rounded to eleven bits as the
  *   down products' operand (f16 with a power of two a row and 512 channels), out_r = sum of w_e y_e in ascending expert id,
  *   then the shared expert, then the residual, one rounding.  (The four launches round W, g, u and h to bf16 as altar-1 does, so
  *   the two agree within those roundings, not bit for bit.)
- * A row's bits depend neither on the other rows nor on their number, and are the same run after run.  Only the rows that
- * picked an expert are computed for it.  Up to eight rows are one launch (fewer where H or I is so large that their
+ * A row's bits depend neither on the other rows nor on their number, and are the same run after run.  A row with an infinity or
+ * a NaN in x, or whose h leaves f32's range, is not finite; the others are as they would be without it.  Only the rows that picked an
+ * expert are computed for it.  Up to eight rows are one launch (fewer where H or I is so large that their
  * activations do not fit shared memory: 8192 and eight rows take two), more follow in stream order.
  * x, res (may be null), out: bf16 [M][H]; out may be x or res, and shares no bytes with them otherwise (DSGX_ERR_ARG).  ws: dsgx_moe_block_ws_bytes(shape) bytes, zeroed once; the
  * kernel leaves its counters at zero.  Its first word is the status (dsgx_ws_status): a picked expert's descriptor of another format
@@ -345,7 +349,10 @@ int dsgx_moe_block_decode(const dsgx_moe_shape* shape, const dsgx_layer_w* L, co
  * out[m][n] = sum_k x[m][k] W[n][k], W[n][k] = (u - z) s of an INT4-g32 matrix: the projections, dense FFN layers and heads of
  * a model whose experts this library runs; stands in for the engines' products with INT4 matrices outside the experts
  * (altar1 engine/attn/attn.h).  W is not rounded: the scale is applied to a group's f32 sum (the expert kernels' contract
- * rounds every weight to bf16).
+ * rounds every weight to bf16).  That sum is sum u x - z sum x, so its error goes with |x| (u + z) s where a product of (u - z) s would
+ * have |x| |u - z| s: f32 outputs are off by about 2.3e-7 of their size at K = 4096 (1.9e-7 in plain f32), and a weight of exactly
+ * zero (u = z) under an x far above its neighbours' costs them that x's last bits.  An infinity or a NaN in a row of x makes all
+ * outputs of that row NaN; the other rows are as they would be without it.
  *
  * dsgx_linear_prepare re-tiles a matrix once at load, from the experts' blocks (DSGX_FMT_INT4: 8 rows x 512 k,
  * [ceil(N / 8)][ceil(K / 512)], made by dsgx10_b200/weights.py pack_linear_int4 for any N and K >= 1) into the order the
