@@ -472,6 +472,8 @@ int dsgx_linear_prepare(const void* w, const void* w_up, uint32_t fmt, int N, in
   if (fmt != DSGX_FMT_INT4) return DSGX_ERR_FORMAT;
   if (!linear_shape_ok(N, K)) return DSGX_ERR_SHAPE;
   if (((uintptr_t)w | (uintptr_t)w_up | (uintptr_t)out) & 15) return DSGX_ERR_ARG;
+  const size_t from = (((size_t)N + 7) / 8) * (((size_t)K + 511) / 512) * 2368, to = linear_bytes(N, K, w_up != nullptr);
+  if (rows_meet(out, to, 0, w, from, 0, 1) || (w_up && rows_meet(out, to, 0, w_up, from, 0, 1))) return DSGX_ERR_ARG;  // (not in place)
   cudaError_t e = launch_linear_prepare(reinterpret_cast<const uint8_t*>(w), reinterpret_cast<const uint8_t*>(w_up), N, K,
                                         reinterpret_cast<uint8_t*>(out), (cudaStream_t)stream);
   return e == cudaSuccess ? DSGX_OK : cuda_fail(e);

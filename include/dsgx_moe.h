@@ -357,7 +357,8 @@ int dsgx_moe_block_decode(const dsgx_moe_shape* shape, const dsgx_layer_w* L, co
  * dsgx_linear_prepare re-tiles a matrix once at load, from the experts' blocks (DSGX_FMT_INT4: 8 rows x 512 k,
  * [ceil(N / 8)][ceil(K / 512)], made by dsgx10_b200/weights.py pack_linear_int4 for any N and K >= 1) into the order the
  * product's MMAs want: dsgx_linear_bytes(N, K, glu) bytes at out, 0 for sizes beyond the limits.  w_up not null (glu): two
- * matrices of one shape, gate and up, in one.  Nothing is allocated; w and w_up may be released after it in stream order.
+ * matrices of one shape, gate and up, in one.  Nothing is allocated; out shares no bytes with w or w_up (DSGX_ERR_ARG), which may be
+ * released after it in stream order.
  * What the packer fills rows and columns up with is never seen: rows past N are not written, and columns past K meet
  * zero activations (their scales must be finite). */
 size_t dsgx_linear_bytes(int N, int K, int glu);

@@ -32,6 +32,14 @@ def test_layer():
         assert _lib.lib().dsgx_moe_block_decode(C.byref(shp), C.byref(W), x, 3, C.byref(B), res, out, None) == _lib.ERR_ARG, (x, res, out)
 
 
+def test_prepare_is_not_in_place():
+    L, w = _lib.lib(), 1 << 24
+    size, src = L.dsgx_linear_bytes(64, 1024, 0), 8 * 2 * 2368
+    pair = L.dsgx_linear_bytes(64, 1024, 1)
+    for a in ((w, None, w), (w, None, w + src - 16), (w, None, w - size + 16), (w, 2 * w, 2 * w), (2 * w, w, w - pair + 16)):
+        assert L.dsgx_linear_prepare(a[0], a[1], _lib.FMT_INT4, 64, 1024, a[2], None) == _lib.ERR_ARG, a
+
+
 @pytest.mark.gpu
 def test_columns_of_one_tensor_and_in_place():
     """x, res and out as columns of one tensor, and a residual in place with a leading dimension of its own: the packed call's bits."""
