@@ -15,7 +15,7 @@
 //   combine  after a grid-wide count: every element adds its row's picks, the shared expert and the residual.
 //
 // Measured (a captured chain, more weights than L2 holds): 168 experts of 6144 x 2048, eight picks a row and the shared expert, one
-// row 59 us (254 MB, 4.3 TB/s; four launches 76), four rows 145 us (717 MB, 4.9 TB/s; 231), eight rows 253 us (434); 1024 x 512
+// row 59.5 us (254 MB, 4.3 TB/s; four launches 76), four rows 146 us (717 MB, 4.9 TB/s; 231), eight rows 258 us (434); 1024 x 512
 // and 16 experts, one row: 21 us, all of it the chain of six grid-wide steps (four launches 18).  About 16 us pass until routed
 // weights stream; from then on 85 % of a copy's rate, the warps' chains of loads, MMAs and f32 operations next to HBM.
 //
